@@ -36,6 +36,33 @@ class LlamaInfo(Structure):
                 ("n_kernels_per_step", c_int32), ("kv_f16", c_int32)]
 
 
+class RopeArgs(Structure):
+    _fields_ = [("x", c_void_p), ("out", c_void_p), ("positions", c_void_p), ("inv_freq", c_void_p),
+                ("n_tokens", c_int64), ("n_heads", c_int64), ("head_dim", c_int64), ("rot_dim", c_int64),
+                ("x_token_stride", c_int64), ("x_head_stride", c_int64), ("out_token_stride", c_int64),
+                ("out_head_stride", c_int64), ("mscale", c_float), ("dtype", c_int32), ("layout", c_int32)]
+
+
+class QkNormRopeArgs(Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p),
+                ("v_out", c_void_p), ("q_gamma", c_void_p), ("k_gamma", c_void_p), ("positions", c_void_p),
+                ("inv_freq", c_void_p), ("kv_rows", c_void_p), ("n_tokens", c_int64), ("n_q_heads", c_int64),
+                ("n_kv_heads", c_int64), ("head_dim", c_int64), ("rot_dim", c_int64), ("token_stride", c_int64),
+                ("head_stride", c_int64), ("q_out_token_stride", c_int64), ("q_out_head_stride", c_int64),
+                ("kv_row_stride", c_int64), ("kv_head_stride", c_int64), ("n_rows", c_int64), ("eps", c_float),
+                ("mscale", c_float), ("dtype", c_int32), ("kv_dtype", c_int32), ("layout", c_int32)]
+
+
+class WindowAttentionArgs(Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("q_start", c_void_p),
+                ("kv_len", c_void_p), ("slots", c_void_p), ("n_seq", c_int64), ("max_q", c_int64),
+                ("n_tokens", c_int64), ("n_q_heads", c_int64), ("n_kv_heads", c_int64), ("head_dim", c_int64),
+                ("q_token_stride", c_int64), ("q_head_stride", c_int64), ("out_token_stride", c_int64),
+                ("out_head_stride", c_int64), ("kv_slot_stride", c_int64), ("kv_head_stride", c_int64),
+                ("kv_row_stride", c_int64), ("n_slots", c_int64), ("kv_rows", c_int64), ("window", c_int64),
+                ("n_sink", c_int64), ("ring", c_int32), ("scale", c_float), ("dtype", c_int32)]
+
+
 TOKEN_CB = ctypes.CFUNCTYPE(None, c_void_p, c_uint32)
 
 _SIGS = {
@@ -113,6 +140,19 @@ _SIGS = {
     "armai_dev_flash_attention_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_float,
                                               c_int64, c_int64, c_int64, c_int64, c_int64, c_int,
                                               c_void_p]),
+    "armai_rope_frequencies": (c_int, [c_size_t, c_double, c_int, c_double, c_double, c_double, c_double, c_void_p,
+                                       c_size_t]),
+    "armai_dev_rope": (c_int, [POINTER(RopeArgs), c_void_p]),
+    "armai_rope_ext_f32": (c_int, [c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_size_t, c_size_t, c_size_t,
+                                   c_size_t, c_int, c_double, c_void_p]),
+    "armai_dev_qk_norm_rope": (c_int, [POINTER(QkNormRopeArgs), c_void_p]),
+    "armai_qk_norm_rope_f32": (c_int, [c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p,
+                                       c_size_t, c_void_p, c_size_t, c_void_p, c_size_t, c_size_t, c_size_t,
+                                       c_size_t, c_int, c_double, c_double, c_void_p, c_void_p]),
+    "armai_dev_window_attention": (c_int, [POINTER(WindowAttentionArgs), c_void_p]),
+    "armai_window_attention_f32": (c_int, [c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_size_t, c_double,
+                                           c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t,
+                                           c_size_t, c_void_p]),
     "armai_quantize_q8k": (c_int, [c_void_p, c_size_t, c_size_t, c_void_p]),
     "armai_kquant_block_dots": (c_int, [c_void_p, c_int, c_size_t, c_size_t, c_void_p, c_size_t,
                                         c_void_p, c_void_p]),
@@ -191,4 +231,4 @@ def ptr(a) -> c_void_p:
 
 
 __all__ = ["load_cuda", "load_synth", "check", "ptr", "ArmaiError", "LlamaOpts", "LlamaInfo",
-           "TOKEN_CB", "c_uint16"]
+           "RopeArgs", "QkNormRopeArgs", "WindowAttentionArgs", "TOKEN_CB", "c_uint16"]

@@ -1261,3 +1261,144 @@ extern "C" int armai_dequant_matmul_f16_f32(const float* act, size_t act_len, co
                                              (int64_t)n, (int64_t)k, s));
   return finish(s, out, dout.p, rows * n * 4);
 }
+
+// ===========================================================================
+// Positions, q/k head norms, window attention: the host forms (the device
+// entry points are in positions.cu and window_attn.cu).
+// ===========================================================================
+extern "C" int armai_rope_ext_f32(const float* input, size_t input_len, const int64_t* positions, size_t n_positions,
+                                  const float* inv_freq, size_t inv_freq_len, size_t n_rows, size_t head_dim,
+                                  size_t heads_per_token, int layout, double mscale, float* out) {
+  if (input_len != n_rows * head_dim)
+    return fail(ARMAI_E_INVALID, lenmsg("rope_ext: input", input_len, "n_rows*head_dim", n_rows * head_dim));
+  if (n_rows != n_positions * heads_per_token)
+    return fail(ARMAI_E_INVALID, "rope_ext: n_rows " + std::to_string(n_rows) + " != n_tokens * heads_per_token = " +
+                                     std::to_string(n_positions * heads_per_token));
+  if (2 * inv_freq_len > head_dim)
+    return fail(ARMAI_E_INVALID, "rope_ext: inv_freq len " + std::to_string(inv_freq_len) + " exceeds head_dim/2 = " +
+                                     std::to_string(head_dim / 2));
+  if (!input_len) return ARMAI_OK;
+  cudaStream_t s;
+  ARMAI_TRY(thread_stream(&s));
+  Scoped dx(s), dp(s), df(s);
+  ARMAI_TRY(h2d(dx, input, input_len * 4));
+  ARMAI_TRY(h2d(dp, positions, n_positions * 8));
+  ARMAI_TRY(h2d(df, inv_freq, inv_freq_len * 4));
+  armai_rope_args a{};
+  a.x = dx.p;
+  a.out = dx.p;
+  a.positions = (const int64_t*)dp.p;
+  a.inv_freq = (const float*)df.p;
+  a.n_tokens = (int64_t)n_positions;
+  a.n_heads = (int64_t)heads_per_token;
+  a.head_dim = (int64_t)head_dim;
+  a.rot_dim = 2 * (int64_t)inv_freq_len;
+  a.x_token_stride = a.out_token_stride = (int64_t)(heads_per_token * head_dim);
+  a.x_head_stride = a.out_head_stride = (int64_t)head_dim;
+  a.mscale = (float)mscale;
+  a.dtype = ARMAI_F32;
+  a.layout = layout;
+  ARMAI_TRY(armai_dev_rope(&a, s));
+  return finish(s, out, dx.p, input_len * 4);
+}
+
+extern "C" int armai_qk_norm_rope_f32(const float* q, size_t q_len, const float* k, size_t k_len,
+                                      const float* q_gamma, size_t q_gamma_len, const float* k_gamma,
+                                      size_t k_gamma_len, const int64_t* positions, size_t n_positions,
+                                      const float* inv_freq, size_t inv_freq_len, size_t n_q_heads, size_t n_kv_heads,
+                                      size_t head_dim, int layout, double eps, double mscale, float* q_out,
+                                      float* k_out) {
+  const size_t t = n_positions;
+  if (q_len != t * n_q_heads * head_dim)
+    return fail(ARMAI_E_INVALID, lenmsg("qk_norm_rope: q", q_len, "T*Hq*D", t * n_q_heads * head_dim));
+  if (k_len != t * n_kv_heads * head_dim)
+    return fail(ARMAI_E_INVALID, lenmsg("qk_norm_rope: k", k_len, "T*Hkv*D", t * n_kv_heads * head_dim));
+  if (q_gamma_len != head_dim)
+    return fail(ARMAI_E_INVALID, lenmsg("qk_norm_rope: q_gamma", q_gamma_len, "head_dim", head_dim));
+  if (k_gamma_len != head_dim)
+    return fail(ARMAI_E_INVALID, lenmsg("qk_norm_rope: k_gamma", k_gamma_len, "head_dim", head_dim));
+  if (2 * inv_freq_len > head_dim)
+    return fail(ARMAI_E_INVALID, "qk_norm_rope: inv_freq len " + std::to_string(inv_freq_len) +
+                                     " exceeds head_dim/2 = " + std::to_string(head_dim / 2));
+  if (!q_len && !k_len) return ARMAI_OK;
+  cudaStream_t s;
+  ARMAI_TRY(thread_stream(&s));
+  Scoped dqk[2] = {Scoped(s), Scoped(s)};
+  Scoped dgq(s), dgk(s), dp(s), df(s);
+  ARMAI_TRY(h2d(dqk[0], q, q_len * 4));
+  ARMAI_TRY(h2d(dqk[1], k, k_len * 4));
+  ARMAI_TRY(h2d(dgq, q_gamma, head_dim * 4));
+  ARMAI_TRY(h2d(dgk, k_gamma, head_dim * 4));
+  ARMAI_TRY(h2d(dp, positions, t * 8));
+  ARMAI_TRY(h2d(df, inv_freq, inv_freq_len * 4));
+  // q, then k: each in place, as the block's one pair of input strides is q's or k's
+  for (int i = 0; i < 2; i++) {
+    armai_qk_norm_rope_args a{};
+    const int64_t heads = (int64_t)(i ? n_kv_heads : n_q_heads);
+    a.q = dqk[i].p;
+    a.q_out = dqk[i].p;
+    a.q_gamma = (const float*)(i ? dgk.p : dgq.p);
+    a.positions = (const int64_t*)dp.p;
+    a.inv_freq = (const float*)df.p;
+    a.n_tokens = (int64_t)t;
+    a.n_q_heads = heads;
+    a.head_dim = (int64_t)head_dim;
+    a.rot_dim = 2 * (int64_t)inv_freq_len;
+    a.token_stride = a.q_out_token_stride = heads * (int64_t)head_dim;
+    a.head_stride = a.q_out_head_stride = (int64_t)head_dim;
+    a.eps = (float)eps;
+    a.mscale = (float)mscale;
+    a.dtype = a.kv_dtype = ARMAI_F32;
+    a.layout = layout;
+    ARMAI_TRY(armai_dev_qk_norm_rope(&a, s));
+  }
+  if (q_len) ARMAI_CUDA(cudaMemcpyAsync(q_out, dqk[0].p, q_len * 4, cudaMemcpyDeviceToHost, s));
+  return finish(s, k_out, dqk[1].p, k_len * 4);
+}
+
+extern "C" int armai_window_attention_f32(const float* q, size_t q_len, const float* k, size_t k_len, const float* v,
+                                          size_t v_len, double scale, size_t b, size_t hq, size_t hkv, size_t sq,
+                                          size_t sk, size_t d, size_t window, size_t n_sink, float* out) {
+  if (q_len != b * hq * sq * d)
+    return fail(ARMAI_E_INVALID, lenmsg("window_attn: q", q_len, "B*Hq*Sq*D", b * hq * sq * d));
+  if (k_len != b * hkv * sk * d)
+    return fail(ARMAI_E_INVALID, lenmsg("window_attn: k", k_len, "B*Hkv*Sk*D", b * hkv * sk * d));
+  if (v_len != b * hkv * sk * d)
+    return fail(ARMAI_E_INVALID, lenmsg("window_attn: v", v_len, "B*Hkv*Sk*D", b * hkv * sk * d));
+  if (sk > 0x3fffffff || b > 65535) return fail(ARMAI_E_INVALID, "window_attn: B or Sk too large");
+  if (!q_len) return ARMAI_OK;
+  cudaStream_t s;
+  ARMAI_TRY(thread_stream(&s));
+  Scoped dq(s), dk(s), dv(s), dout(s), dlen(s);
+  const int32_t len = (int32_t)sk;
+  ARMAI_TRY(h2d(dq, q, q_len * 4));
+  ARMAI_TRY(h2d(dk, k, k_len * 4));
+  ARMAI_TRY(h2d(dv, v, v_len * 4));
+  ARMAI_TRY(h2d(dlen, &len, 4));
+  ARMAI_TRY(dalloc(dout, q_len * 4));
+  armai_window_attention_args a{};
+  a.kv_len = (const int32_t*)dlen.p;
+  a.n_seq = 1;
+  a.max_q = a.n_tokens = (int64_t)sq;
+  a.n_q_heads = (int64_t)hq;
+  a.n_kv_heads = (int64_t)hkv;
+  a.head_dim = (int64_t)d;
+  a.q_token_stride = a.out_token_stride = a.kv_row_stride = (int64_t)d;
+  a.q_head_stride = a.out_head_stride = (int64_t)(sq * d);
+  a.kv_head_stride = (int64_t)(sk * d);
+  a.kv_slot_stride = (int64_t)(hkv * sk * d);
+  a.n_slots = 1;
+  a.kv_rows = sk ? (int64_t)sk : 1;  // no keys: kv_len 0, nothing is read
+  a.window = (int64_t)window;
+  a.n_sink = (int64_t)n_sink;
+  a.scale = (float)scale;
+  a.dtype = ARMAI_F32;
+  for (size_t i = 0; i < b; i++) {  // the head-major rows of one batch entry at a time
+    a.q = (const float*)dq.p + i * hq * sq * d;
+    a.out = (float*)dout.p + i * hq * sq * d;
+    a.k = (const float*)dk.p + i * hkv * sk * d;
+    a.v = (const float*)dv.p + i * hkv * sk * d;
+    ARMAI_TRY(armai_dev_window_attention(&a, s));
+  }
+  return finish(s, out, dout.p, q_len * 4);
+}

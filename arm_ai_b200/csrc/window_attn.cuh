@@ -1,0 +1,107 @@
+// window_attn.cuh — what the window-attention kernels share: the call's
+// parameters, a sequence's place in the call, and the cache rows that a run
+// of queries can see.
+//
+// Query at position i sees key position j iff j <= i and (j > i - W or j < S)
+// (W: window, S: first positions that stay visible). The keys that queries
+// plo .. phi see together are [0, S) and [plo - W + 1, phi], one range where
+// the two touch; in a ring cache the second range may wrap once. So at most
+// three runs of consecutive cache rows with consecutive positions, and a
+// kernel walks their tiles.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "dev_call.cuh"
+
+namespace armai {
+
+struct WaParams {
+  const void *q, *k, *v;
+  void* out;
+  const int32_t *q_start, *kv_len, *slots;
+  int64_t q_token, q_head, o_token, o_head;
+  int64_t kv_slot, kv_head, kv_row;
+  int n_seq, max_q, n_tokens, n_q_heads, group, head_dim, n_slots, kv_rows;
+  int window, n_sink, ring;  // ring: rows of the ring, 0 for a linear cache
+  float scale_log2;          // scale * log2(e): the kernels use exp2
+  uint32_t* err;             // bounded waits that ran out
+};
+
+// A sequence's queries: rows q0 .. q0 + n - 1 of q, the i-th at position
+// pos0 + i.
+struct WaSeq {
+  int q0, n, pos0, slot;
+};
+__device__ __forceinline__ WaSeq wa_seq(const WaParams& p, int s) {
+  WaSeq r;
+  int len;
+  if (p.q_start) {
+    r.q0 = min(max(p.q_start[s], 0), p.n_tokens);
+    len = min(max(p.q_start[s + 1], r.q0), p.n_tokens) - r.q0;
+  } else {
+    r.q0 = (int)min((int64_t)s * p.max_q, (int64_t)p.n_tokens);
+    len = min(p.max_q, p.n_tokens - r.q0);
+  }
+  r.n = min(len, p.max_q);
+  r.slot = p.slots ? p.slots[s] : s;
+  const int kv = r.slot >= 0 && r.slot < p.n_slots ? max(p.kv_len[s], 0) : 0;
+  r.pos0 = kv - len;
+  return r;
+}
+
+struct WaRuns {
+  int row[3], pos[3], len[3];
+  int n;
+  __device__ __forceinline__ void add(int r, int p, int l) {
+    if (l <= 0) return;
+    // n is 0, 1 or 2 here: written by comparison, so that the arrays stay in registers
+#pragma unroll
+    for (int i = 0; i < 3; i++)
+      if (n == i) {
+        row[i] = r;
+        pos[i] = p;
+        len[i] = l;
+      }
+    n++;
+  }
+  // key range [a, b] at or behind the first positions, in a ring of R rows
+  __device__ __forceinline__ void add_range(const WaParams& p, int a, int b) {
+    if (a > b) return;
+    if (!p.ring) {
+      add(a, a, min(b, p.kv_rows - 1) - a + 1);
+      return;
+    }
+    const int at = (a - p.n_sink) % p.ring;
+    const int len = min(b - a + 1, p.ring), first = min(len, p.ring - at);
+    add(p.n_sink + at, a, first);
+    add(p.n_sink, a + first, len - first);
+  }
+};
+// The cache rows that queries at positions plo .. phi see (a hull: tiles
+// still need the mask).
+__device__ __forceinline__ WaRuns wa_runs(const WaParams& p, int plo, int phi) {
+  WaRuns r;
+  r.n = 0;
+#pragma unroll
+  for (int i = 0; i < 3; i++) r.row[i] = r.pos[i] = r.len[i] = 0;
+  if (phi < 0) return r;
+  const int64_t lo64 = (int64_t)plo - p.window + 1;
+  const int lo = lo64 > 0 ? (int)lo64 : 0;
+  if (lo <= p.n_sink) {  // one range from the first position on; in a ring it has not wrapped
+    r.add(0, 0, min(phi, p.kv_rows - 1) + 1);
+  } else {
+    r.add(0, 0, min(p.n_sink, p.kv_rows));
+    r.add_range(p, lo, phi);
+  }
+  return r;
+}
+
+__device__ __forceinline__ bool wa_sees(const WaParams& p, int qpos, int kpos) {
+  return kpos <= qpos && (qpos - kpos < p.window || kpos < p.n_sink);
+}
+
+int wa_simt_launch(const WaParams& p, int dtype, cudaStream_t s);
+
+}  // namespace armai

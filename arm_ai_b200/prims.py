@@ -151,3 +151,65 @@ def dequantize_q6_k_op(input, n_elements):
     out = np.empty(max(n_elements, 1), np.float32)
     _chk(load_cuda().armai_dequantize_q6_k(ptr(b), b.size, n_elements, ptr(out)))
     return out[:n_elements]
+
+
+# ---- positions, q/k head norms, window attention -------------------------
+# (no NIF of the reference; device-resident tensors of f32 / f16 / bf16 take
+# the armai_dev_* entry points with the argument blocks of _lib)
+
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "base": 2, "turns": 3}
+
+
+def _named(table, what, value):
+    if value not in table:
+        raise NifError(f"{what} {value!r} is not one of {', '.join(table)}")
+    return table[value]
+
+
+def rope_frequencies(rot_dim, base=10000.0, scaling="none", factor=1.0, orig_ctx=0, low=1.0, high=4.0):
+    """[rot_dim / 2] f32 rotary frequencies, scaled for a longer context:
+    "linear" (all divided by factor), "base" (the base raised so that the
+    lowest is divided by factor) or "turns" (kept for pairs that turn at least
+    `high` times in orig_ctx positions, divided by factor below `low` turns,
+    blended between)."""
+    f = np.empty(rot_dim // 2, np.float32)
+    _chk(load_cuda().armai_rope_frequencies(rot_dim, float(base), _named(ROPE_SCALINGS, "rope scaling", scaling),
+                                            float(factor), float(orig_ctx), float(low), float(high), ptr(f), f.size))
+    return f
+
+
+def rope_ext_f32_op(input, positions, inv_freq, n_rows, head_dim, heads_per_token, layout="interleaved", mscale=1.0):
+    """rope_f32_op with either pair layout, the first 2 * len(inv_freq) values
+    of each row rotated (the others copied) and accurate far positions."""
+    x, p, f = _c(input, np.float32), _c(positions, np.int64), _c(inv_freq, np.float32)
+    out = np.empty(max(x.size, 1), np.float32)
+    _chk(load_cuda().armai_rope_ext_f32(ptr(x), x.size, ptr(p), p.size, ptr(f), f.size, n_rows, head_dim,
+                                        heads_per_token, _named(ROPE_LAYOUTS, "rope layout", layout), float(mscale),
+                                        ptr(out)))
+    return out[: x.size]
+
+
+def qk_norm_rope_f32_op(q, k, q_gamma, k_gamma, positions, inv_freq, n_q_heads, n_kv_heads, head_dim,
+                        layout="half", eps=1e-5, mscale=1.0):
+    """RMS norm of every head of q [T, n_q_heads, head_dim] and k
+    [T, n_kv_heads, head_dim] with its gain, then the rotation: (q, k)."""
+    q, k, gq, gk = (_c(a, np.float32) for a in (q, k, q_gamma, k_gamma))
+    p, f = _c(positions, np.int64), _c(inv_freq, np.float32)
+    qo, ko = np.empty(max(q.size, 1), np.float32), np.empty(max(k.size, 1), np.float32)
+    _chk(load_cuda().armai_qk_norm_rope_f32(ptr(q), q.size, ptr(k), k.size, ptr(gq), gq.size, ptr(gk), gk.size, ptr(p),
+                                            p.size, ptr(f), f.size, n_q_heads, n_kv_heads, head_dim,
+                                            _named(ROPE_LAYOUTS, "rope layout", layout), float(eps), float(mscale),
+                                            ptr(qo), ptr(ko)))
+    return qo[: q.size], ko[: k.size]
+
+
+def window_attention_f32_op(q, k, v, scale, b, hq, hkv, sq, sk, d, window, n_sink=0):
+    """Causal attention of q [B,Hq,Sq,D] (query i at position Sk - Sq + i) to
+    k / v [B,Hkv,Sk,D], each query to the last `window` positions up to its own
+    and the first `n_sink`; a query that sees none gets zeros."""
+    q, k, v = _c(q, np.float32), _c(k, np.float32), _c(v, np.float32)
+    out = np.empty(max(b * hq * sq * d, 1), np.float32)
+    _chk(load_cuda().armai_window_attention_f32(ptr(q), q.size, ptr(k), k.size, ptr(v), v.size, float(scale), b, hq,
+                                                hkv, sq, sk, d, window, n_sink, ptr(out)))
+    return out[: b * hq * sq * d]

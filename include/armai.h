@@ -332,6 +332,129 @@ ARMAI_API int armai_dev_dequant_matmul_f16_f32(const float* act, const uint16_t*
                                                int64_t rows, int64_t n, int64_t k, void* stream);
 
 /* ------------------------------------------------------------------ */
+/* Positions, q/k head norms and window attention (no reference         */
+/* counterpart: the reference's rope_f32_op, rmsnorm_f32_op and           */
+/* flash_attention_f32_op, extended to what newer Llama-family models      */
+/* and serving with a bounded cache need).                                  */
+/*                                                                          */
+/* The armai_dev_* forms take an argument block (pointers to device memory, */
+/* strides in elements, the innermost dimension contiguous), launch on      */
+/* `stream`, neither synchronise nor allocate, and may be captured into a    */
+/* CUDA graph. A block may be reused from call to call. They run on the      */
+/* device their tensors are on, whichever is current, and refuse host        */
+/* memory that the device cannot read.                                       */
+/* ------------------------------------------------------------------ */
+#define ARMAI_F32 0
+#define ARMAI_F16 1
+#define ARMAI_BF16 2
+
+#define ARMAI_ROPE_INTERLEAVED 0 /* pairs (2i, 2i + 1), as armai_rope_f32 */
+#define ARMAI_ROPE_HALF 1        /* pairs (i, i + rot_dim / 2) */
+
+#define ARMAI_ROPE_SCALE_NONE 0
+#define ARMAI_ROPE_SCALE_LINEAR 1 /* every frequency divided by `factor` */
+#define ARMAI_ROPE_SCALE_BASE 2   /* base * factor^(rot_dim / (rot_dim - 2)): the lowest frequency divided by factor */
+#define ARMAI_ROPE_SCALE_TURNS 3  /* by the turns r_i a pair makes over orig_ctx positions: kept from `high` turns on,
+                                     divided by `factor` up to `low`, (1 - g) f / factor + g f with
+                                     g = (r_i - low) / (high - low) between */
+
+/* Host only: inv_freq[i] = base^(-2i / rot_dim), i < rot_dim / 2, scaled for a
+ * longer context as above (computed in f64, rounded once). */
+ARMAI_API int armai_rope_frequencies(size_t rot_dim, double base, int scaling, double factor, double orig_ctx,
+                                     double low, double high, float* inv_freq, size_t inv_freq_len);
+
+typedef struct armai_rope_args {
+  const void* x;            /* [n_tokens][n_heads][head_dim] */
+  void* out;                /* same shape; may be x itself (with x's strides) */
+  const int64_t* positions; /* [n_tokens]; a negative position turns backwards, so the rotation's
+                               transpose (its gradient) is the same call with the positions negated */
+  const float* inv_freq;    /* [rot_dim / 2] */
+  int64_t n_tokens, n_heads, head_dim; /* head_dim 1 .. 256 */
+  int64_t rot_dim;          /* even, 0 .. head_dim: values rot_dim .. are copied */
+  int64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+  float mscale;             /* multiplies the rotated values (1: plain rotation) */
+  int32_t dtype;            /* ARMAI_F32 / F16 / BF16, of x and out */
+  int32_t layout;           /* ARMAI_ROPE_* */
+} armai_rope_args;
+/* out[t][h] = x[t][h] with pair i turned by positions[t] * inv_freq[i]. The
+ * angle is the exact product, reduced in f64, so far positions keep their
+ * accuracy (armai_rope_f32 rounds it to f32 as the reference does). */
+ARMAI_API int armai_dev_rope(const armai_rope_args* args, void* stream);
+/* Host form, f32: input [n_rows][head_dim] as armai_rope_f32, the first
+ * 2 * inv_freq_len values of each row rotated. */
+ARMAI_API int armai_rope_ext_f32(const float* input, size_t input_len, const int64_t* positions,
+                                 size_t n_positions, const float* inv_freq, size_t inv_freq_len, size_t n_rows,
+                                 size_t head_dim, size_t heads_per_token, int layout, double mscale, float* out);
+
+typedef struct armai_qk_norm_rope_args {
+  const void *q, *k, *v;    /* [n_tokens][heads][head_dim], all three with token_stride and head_stride (a packed
+                               projection, or three tensors); v may be NULL (nothing copied) */
+  void* q_out;              /* [n_tokens][n_q_heads][head_dim]; may be q itself (with q's strides) */
+  void *k_out, *v_out;      /* rows of kv_dtype: (row, head) at row * kv_row_stride + head * kv_head_stride. A cache
+                               [slot][n_kv_heads][cap][head_dim] has kv_row_stride = head_dim, kv_head_stride =
+                               cap * head_dim, and row r of slot s is row s * n_kv_heads * cap + r */
+  const float *q_gamma, *k_gamma; /* [head_dim] gains; NULL: that tensor is rotated without a norm */
+  const int64_t* positions; /* [n_tokens] */
+  const float* inv_freq;    /* [rot_dim / 2] */
+  const int64_t* kv_rows;   /* [n_tokens] row of each token in k_out / v_out; NULL: the token's index. A token
+                               whose row is not in 0 .. n_rows - 1 (padding: -1) writes no key and no value;
+                               two tokens of a call must not name the same row */
+  int64_t n_tokens, n_q_heads, n_kv_heads, head_dim, rot_dim;
+  int64_t token_stride, head_stride, q_out_token_stride, q_out_head_stride, kv_row_stride, kv_head_stride;
+  int64_t n_rows;
+  float eps, mscale;
+  int32_t dtype, kv_dtype;  /* kv_dtype: dtype, or f16 / bf16 for f32 inputs */
+  int32_t layout;
+} armai_qk_norm_rope_args;
+/* y = rope(x / sqrt(mean(x^2) + eps) * gamma) for every head of q and k in
+ * one pass, k (and v as it is) appended to the cache. f32 in between. */
+ARMAI_API int armai_dev_qk_norm_rope(const armai_qk_norm_rope_args* args, void* stream);
+/* Host form, f32: q [T][n_q_heads][head_dim], k [T][n_kv_heads][head_dim]. */
+ARMAI_API int armai_qk_norm_rope_f32(const float* q, size_t q_len, const float* k, size_t k_len,
+                                     const float* q_gamma, size_t q_gamma_len, const float* k_gamma,
+                                     size_t k_gamma_len, const int64_t* positions, size_t n_positions,
+                                     const float* inv_freq, size_t inv_freq_len, size_t n_q_heads,
+                                     size_t n_kv_heads, size_t head_dim, int layout, double eps, double mscale,
+                                     float* q_out, float* k_out);
+
+typedef struct armai_window_attention_args {
+  const void* q;            /* [n_tokens][n_q_heads][head_dim]: the sequences' queries behind one another */
+  const void *k, *v;        /* [n_slots][n_kv_heads][kv_rows][head_dim] caches, both with the kv strides */
+  void* out;                /* like q */
+  const int32_t* q_start;   /* [n_seq + 1] first query of each sequence; NULL: max_q queries each */
+  const int32_t* kv_len;    /* [n_seq] keys of each sequence, those of this call's queries included */
+  const int32_t* slots;     /* [n_seq] cache slot of each sequence; NULL: its index */
+  int64_t n_seq;
+  int64_t max_q;            /* no sequence has more queries (queries beyond it are not computed) */
+  int64_t n_tokens, n_q_heads, n_kv_heads, head_dim; /* n_q_heads a multiple of n_kv_heads; head_dim 1 .. 256 */
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  int64_t kv_slot_stride, kv_head_stride, kv_row_stride;
+  int64_t n_slots, kv_rows;
+  int64_t window;           /* >= 1 */
+  int64_t n_sink;           /* >= 0: first positions that stay visible */
+  int32_t ring;             /* 0: position p is cache row p. 1: rows n_sink .. kv_rows - 1 are a ring of
+                               R = kv_rows - n_sink rows, R >= window + max_q - 1: position p >= n_sink is row
+                               n_sink + (p - n_sink) % R */
+  float scale;              /* of the scores */
+  int32_t dtype;            /* of q, k, v and out */
+} armai_window_attention_args;
+/* The i-th of a sequence's n queries is at position p = kv_len - n + i and
+ * sees the keys j <= p with j > p - window or j < n_sink; out = softmax(scale
+ * q k^T) v over them (query head h with key / value head h / (n_q_heads /
+ * n_kv_heads)), scores, softmax and sums in f32. A query that sees no key
+ * (p < 0, kv_len <= 0, a slot outside 0 .. n_slots - 1) gets zeros. Cache rows
+ * that no query of the sequence sees may hold anything; the values (not the
+ * keys) of a row that only some queries of a call see must be finite. Rows of
+ * out behind the last sequence are left as they are. */
+ARMAI_API int armai_dev_window_attention(const armai_window_attention_args* args, void* stream);
+/* Host form, f32: q [B,Hq,Sq,D], k / v [B,Hkv,Sk,D] as armai_flash_attention_f32
+ * (but with query i at position Sk - Sq + i) -> out [B,Hq,Sq,D]. */
+ARMAI_API int armai_window_attention_f32(const float* q, size_t q_len, const float* k, size_t k_len,
+                                         const float* v, size_t v_len, double scale, size_t b, size_t hq,
+                                         size_t hkv, size_t sq, size_t sk, size_t d, size_t window,
+                                         size_t n_sink, float* out);
+
+/* ------------------------------------------------------------------ */
 /* k-quant building blocks, exposed for bit-exact parity tests.           */
 /* ------------------------------------------------------------------ */
 /* Q8_K quantisation of x[m, k] (candle BlockQ8K::from_float): writes
