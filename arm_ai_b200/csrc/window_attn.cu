@@ -176,6 +176,15 @@ int ws_dim(const WaParams& p, cudaStream_t s) {
 
 }  // namespace
 
+bool wa_vectors(const WaParams& p, int dtype) {
+  const int64_t es = dtype_size(dtype);
+  const auto ok = [&](int64_t stride) { return stride * es % 16 == 0; };
+  return (reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
+          reinterpret_cast<uintptr_t>(p.out)) % 16 == 0 &&
+         ok(p.q_token) && ok(p.q_head) && ok(p.o_token) && ok(p.o_head) && ok(p.kv_slot) && ok(p.kv_head) &&
+         ok(p.kv_row);
+}
+
 int wa_simt_launch(const WaParams& p, int dtype, cudaStream_t s) {
   if (dtype == ARMAI_F32) return ws_dim<float>(p, s);
   if (dtype == ARMAI_F16) return ws_dim<__half>(p, s);
@@ -244,5 +253,9 @@ extern "C" int armai_dev_window_attention(const armai_window_attention_args* a, 
   p.n_sink = (int)sink;
   p.ring = a->ring ? (int)(a->kv_rows - sink) : 0;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  return wa_simt_launch(p, a->dtype, (cudaStream_t)stream);
+  const cudaStream_t s = (cudaStream_t)stream;
+  // Few query rows per key / value head: bound by the keys, split over the device.
+  if (wa_vectors(p, a->dtype) && wa_split_fits(p, a->dtype) && (int64_t)p.max_q * p.group <= 64)
+    return wa_split_launch(p, a->dtype, s);
+  return wa_simt_launch(p, a->dtype, s);
 }

@@ -102,6 +102,11 @@ __device__ __forceinline__ bool wa_sees(const WaParams& p, int qpos, int kpos) {
   return kpos <= qpos && (qpos - kpos < p.window || kpos < p.n_sink);
 }
 
+// Every pointer and stride a whole number of 16-byte vectors.
+bool wa_vectors(const WaParams& p, int dtype);
+
 int wa_simt_launch(const WaParams& p, int dtype, cudaStream_t s);
+bool wa_split_fits(const WaParams& p, int dtype);  // of aligned tensors (wa_vectors)
+int wa_split_launch(const WaParams& p, int dtype, cudaStream_t s);
 
 }  // namespace armai

@@ -1,0 +1,650 @@
+// window_attn_split.cu — window attention of few queries per sequence (single
+// tokens, short chunks): the visible keys are split over the warps of a
+// thread-block cluster and the parts joined through distributed shared memory.
+//
+// Bound by the bytes of the visible keys and values. A warp takes tiles of 16
+// keys in turn with the cluster's other warps and keeps its own running
+// maximum, sum and output, so no warp waits for another until the end. Its
+// tiles arrive by asynchronous 16-byte copies into a three-deep ring in which
+// every lane reads back only what it copied itself (no barrier, no bank
+// conflict): the order of the values within a row is free in both products, as
+// long as q and k (or p and v) agree, so each lane copies the 16-byte chunks
+// that hold its own operands.
+//   16-bit types: m16n8k16 tensor instructions, 16 rows = (token, query head)
+//   pairs of one key / value head, so a key is read once for all of them.
+//   f32: products on the CUDA cores, 8 lanes per key.
+// The cluster's parts are joined in rank order: results do not depend on
+// timing, no workspace, one launch.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "llama_kernels.cuh"
+#include "window_attn.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace armai {
+namespace {
+
+constexpr int SP_WARPS = 4, SP_THREADS = 32 * SP_WARPS;
+constexpr int SP_STAGES = 3;
+constexpr int SP_MAX_SPLIT = 16;
+// The running maximum is raised (and the output rescaled) only when a score
+// exceeds it by more than this many powers of two: the weights stay below 2^8
+// and their sum far inside f32, and most tiles need no exchange between lanes.
+constexpr float SP_SLACK = 8.f;
+
+__device__ __forceinline__ void cp16(void* dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ float sp_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                                        uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Tile t of KT keys of the runs: its first cache row, first position and keys.
+struct SpTile {
+  int row, pos, n;
+};
+template <int KT>
+__device__ __forceinline__ SpTile sp_tile(const WaRuns& r, int t) {
+  const int c0 = (r.len[0] + KT - 1) / KT, c1 = (r.len[1] + KT - 1) / KT;
+  const int s = t < c0 ? 0 : t < c0 + c1 ? 1 : 2;
+  const int o = (s == 0 ? t : s == 1 ? t - c0 : t - c0 - c1) * KT;
+  SpTile x;
+  x.row = (s == 0 ? r.row[0] : s == 1 ? r.row[1] : r.row[2]) + o;
+  x.pos = (s == 0 ? r.pos[0] : s == 1 ? r.pos[1] : r.pos[2]) + o;
+  x.n = min(KT, (s == 0 ? r.len[0] : s == 1 ? r.len[1] : r.len[2]) - o);
+  return x;
+}
+template <int KT>
+__device__ __forceinline__ int sp_tiles(const WaRuns& r) {
+  return (r.len[0] + KT - 1) / KT + (r.len[1] + KT - 1) / KT + (r.len[2] + KT - 1) / KT;
+}
+
+// What a CTA works on: rows f0 .. f0 + nr - 1 of the (token, query head of
+// the group) pairs of one sequence and key / value head.
+struct SpBlock {
+  WaSeq sq;
+  int kvh, f0, nr;
+  WaRuns runs;
+};
+template <int R>
+__device__ __forceinline__ bool sp_block(const WaParams& p, SpBlock& b) {
+  const int n_kv = p.n_q_heads / p.group;
+  b.kvh = blockIdx.y % n_kv;
+  b.f0 = (blockIdx.y / n_kv) * R;
+  b.sq = wa_seq(p, blockIdx.z);
+  b.nr = min(R, b.sq.n * p.group - b.f0);
+  if (b.nr <= 0) return false;  // the same for the whole cluster
+  b.runs = wa_runs(p, b.sq.pos0 + b.f0 / p.group, b.sq.pos0 + (b.f0 + b.nr - 1) / p.group);
+  return true;
+}
+
+// Joins the warps' parts ([warp][R] maxima and sums, [warp][R][DT] outputs in
+// shared memory, outputs unnormalised) within the CTA, then over the cluster,
+// and writes the rows. Every rank writes a share of the values.
+template <typename T, int R, int DT>
+__device__ __forceinline__ void sp_join(const WaParams& p, const SpBlock& b, float* part, float* wm, float* wl) {
+  // part: [SP_WARPS][R][DT], wm / wl: [SP_WARPS][R]; the CTA's own result replaces warp 0's
+  const int tid = threadIdx.x;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)gridDim.x, rank = (int)blockIdx.x;
+  __syncthreads();
+  for (int e = tid; e < b.nr * (DT / 4); e += SP_THREADS) {
+    const int r = e / (DT / 4), d = (e % (DT / 4)) * 4;
+    float m = wm[r];
+#pragma unroll
+    for (int w = 1; w < SP_WARPS; w++) m = fmaxf(m, wm[w * R + r]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; w++) {
+      const float f = sp_exp2(wm[w * R + r] - base);
+      const float4 v = *reinterpret_cast<const float4*>(part + (w * R + r) * DT + d);
+      acc.x += f * v.x;
+      acc.y += f * v.y;
+      acc.z += f * v.z;
+      acc.w += f * v.w;
+    }
+    *reinterpret_cast<float4*>(part + r * DT + d) = acc;
+  }
+  __syncthreads();
+  if (tid < b.nr) {
+    float m = wm[tid], l = 0.f;
+#pragma unroll
+    for (int w = 1; w < SP_WARPS; w++) m = fmaxf(m, wm[w * R + tid]);
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; w++) l += sp_exp2(wm[w * R + tid] - base) * wl[w * R + tid];
+    wm[tid] = m;
+    wl[tid] = l;
+  }
+  if (ranks > 1) cluster.sync(); else __syncthreads();
+  for (int e = rank * SP_THREADS + tid; e < b.nr * (DT / 4); e += ranks * SP_THREADS) {
+    const int r = e / (DT / 4), d = (e % (DT / 4)) * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    if (ranks == 1) {
+      acc = *reinterpret_cast<const float4*>(part + r * DT + d);
+      l = wl[r];
+    } else {
+      float m = -INFINITY;
+#pragma unroll 4
+      for (int k = 0; k < ranks; k++) m = fmaxf(m, *cluster.map_shared_rank(wm + r, k));
+      const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+      for (int k = 0; k < ranks; k++) {
+        const float f = sp_exp2(*cluster.map_shared_rank(wm + r, k) - base);
+        l += f * *cluster.map_shared_rank(wl + r, k);
+        const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part + r * DT + d, k));
+        acc.x += f * v.x;
+        acc.y += f * v.y;
+        acc.z += f * v.z;
+        acc.w += f * v.w;
+      }
+    }
+    if (d < p.head_dim) {
+      const float inv = l == 0.f ? 0.f : 1.0f / l;  // an empty row: 0 * 0; NaN kept
+      const int f = b.f0 + r;
+      T* o = static_cast<T*>(p.out) + (int64_t)(b.sq.q0 + f / p.group) * p.o_token +
+             (int64_t)(b.kvh * p.group + f % p.group) * p.o_head + d;
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(o) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      } else {
+        *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+      }
+    }
+  }
+  if (ranks > 1) cluster.sync();  // the others still read this CTA's part
+}
+
+// ---------------------------------------------------------------------------
+// 16-bit types. DT: head width, padded to 64, 128 or 256 (chunks beyond
+// head_dim are zero-filled). Lane (g = lane / 4, c = lane % 4).
+//   S = Q K^T: step s = 2 i + h of 16 takes the d = 8 (c + 4 i) + 4 h .. + 3
+//   of lane c, for q and k alike.
+//   O = P V: lane holds, for the tile's keys 2c, 2c+1, 2c+8, 2c+9, the
+//   d = 64 b + 8 g .. + 7; product (b, e) has d = 64 b + 8 n + e as column n,
+//   so a lane's outputs are the 16 values from 64 b + 16 c on.
+// ---------------------------------------------------------------------------
+constexpr int SP_ROWS = 16, SP_KT = 16;
+
+template <typename T, int DT>
+constexpr size_t sp_smem() {
+  const size_t ring = (size_t)SP_WARPS * SP_STAGES * 2 * SP_KT * DT * 2;
+  const size_t join = (size_t)SP_WARPS * SP_ROWS * (DT + 2) * 4;
+  return ring > join ? ring : join;
+}
+
+template <typename T, int DT>
+__global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
+  constexpr int KC = DT / 32, VB = DT / 64;       // k chunks per key and lane; 64-wide blocks of v
+  constexpr int CH = 2 * KC + 4 * VB;             // 16-byte chunks per lane and stage
+  extern __shared__ __align__(16) uint8_t sm[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+  SpBlock b;
+  if (!sp_block<SP_ROWS>(p, b)) return;
+  const int chunks = p.head_dim >> 3;             // valid 16-byte chunks of a row
+  const int64_t kv_off = (int64_t)b.sq.slot * p.kv_slot + (int64_t)b.kvh * p.kv_head;
+  const T* kb = static_cast<const T*>(p.k) + kv_off;
+  const T* vb = static_cast<const T*>(p.v) + kv_off;
+  uint4* ring = reinterpret_cast<uint4*>(sm) + warp * (SP_STAGES * CH * 32) + lane;
+  const int step = (int)gridDim.x * SP_WARPS, first = (int)blockIdx.x * SP_WARPS + warp;
+  const int nt = sp_tiles<SP_KT>(b.runs);
+
+  auto load = [&](int t, int slot) {
+    if (t < nt) {
+      const SpTile x = sp_tile<SP_KT>(b.runs, t);
+      uint4* dst = ring + slot * CH * 32;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int key = g + 8 * j;
+        const T* src = kb + (int64_t)(x.row + (key < x.n ? key : 0)) * p.kv_row;
+#pragma unroll
+        for (int i = 0; i < KC; i++) {
+          const bool ok = key < x.n && c + 4 * i < chunks;
+          cp16(dst + (j * KC + i) * 32, src + (ok ? 8 * (c + 4 * i) : 0), ok);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int key = 2 * c + (j & 1) + 8 * (j >> 1);
+        const T* src = vb + (int64_t)(x.row + (key < x.n ? key : 0)) * p.kv_row;
+#pragma unroll
+        for (int i = 0; i < VB; i++) {
+          const bool ok = key < x.n && 8 * i + g < chunks;
+          cp16(dst + (2 * KC + j * VB + i) * 32, src + (ok ? 64 * i + 8 * g : 0), ok);
+        }
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < SP_STAGES; s++) load(first + s * step, s);
+
+  // q rows g and g + 8; rows beyond the block are zero
+  uint32_t qa[KC][2][4];
+  int qpos[2];
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    const int r = g + 8 * j, f = b.f0 + (r < b.nr ? r : 0);
+    qpos[j] = b.sq.pos0 + f / p.group;
+    const T* src = static_cast<const T*>(p.q) + (int64_t)(b.sq.q0 + f / p.group) * p.q_token +
+                   (int64_t)(b.kvh * p.group + f % p.group) * p.q_head;
+#pragma unroll
+    for (int i = 0; i < KC; i++) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (r < b.nr && c + 4 * i < chunks) v = *reinterpret_cast<const uint4*>(src + 8 * (c + 4 * i));
+      qa[i][0][j] = v.x;
+      qa[i][0][2 + j] = v.y;
+      qa[i][1][j] = v.z;
+      qa[i][1][2 + j] = v.w;
+    }
+  }
+  const int qmin = b.sq.pos0 + b.f0 / p.group, qmax = b.sq.pos0 + (b.f0 + b.nr - 1) / p.group;
+
+  float o[VB][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < VB; i++)
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) o[i][e][k] = 0.f;
+
+  int slot = 0;
+#pragma unroll 1
+  for (int t = first; t < nt; t += step) {
+    const SpTile x = sp_tile<SP_KT>(b.runs, t);
+    cp_wait<SP_STAGES - 1>();
+    const uint4* src = ring + slot * CH * 32;
+    float s[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) s[j][k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KC; i++) {
+        const uint4 v = src[(j * KC + i) * 32];
+        mma16816<T>(s[j], qa[i][0], v.x, v.y);
+        mma16816<T>(s[j], qa[i][1], v.z, v.w);
+      }
+    }
+    // s[j][0, 1]: row g, keys 8 j + 2 c, + 1; s[j][2, 3]: row g + 8
+    const bool full = x.n == SP_KT && x.pos + SP_KT - 1 <= qmin &&
+                      (qmax - x.pos < p.window || x.pos + SP_KT - 1 < p.n_sink);
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        s[j][k] *= p.scale_log2;
+        const int key = 8 * j + 2 * c + (k & 1);
+        if (!full && (key >= x.n || !wa_sees(p, qpos[k >> 1], x.pos + key))) s[j][k] = -INFINITY;
+        top[k >> 1] = fmaxf(top[k >> 1], s[j][k]);
+      }
+    if (__any_sync(0xffffffffu, top[0] > m[0] + SP_SLACK || top[1] > m[1] + SP_SLACK)) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        float y = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 1));
+        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+        const float nm = fmaxf(m[j], y);
+        const float f = nm == -INFINITY ? 1.f : sp_exp2(m[j] - nm);
+        m[j] = nm;
+        l[j] *= f;
+#pragma unroll
+        for (int i = 0; i < VB; i++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            o[i][e][2 * j] *= f;
+            o[i][e][2 * j + 1] *= f;
+          }
+      }
+    }
+    uint32_t pa[4];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const float base = m[j] == -INFINITY ? 0.f : m[j];
+      const float p0 = sp_exp2(s[0][2 * j] - base), p1 = sp_exp2(s[0][2 * j + 1] - base);
+      const float p2 = sp_exp2(s[1][2 * j] - base), p3 = sp_exp2(s[1][2 * j + 1] - base);
+      l[j] += (p0 + p1) + (p2 + p3);
+      pa[j] = pack2<T>(p0, p1);      // rounded to T for the product: half a step of each weight
+      pa[2 + j] = pack2<T>(p2, p3);
+    }
+#pragma unroll
+    for (int i = 0; i < VB; i++) {
+      const uint4 v0 = src[(2 * KC + i) * 32], v1 = src[(2 * KC + VB + i) * 32];
+      const uint4 v2 = src[(2 * KC + 2 * VB + i) * 32], v3 = src[(2 * KC + 3 * VB + i) * 32];
+      const uint32_t a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
+      const uint32_t a2[4] = {v2.x, v2.y, v2.z, v2.w}, a3[4] = {v3.x, v3.y, v3.z, v3.w};
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        mma16816<T>(o[i][2 * e], pa, __byte_perm(a0[e], a1[e], 0x5410), __byte_perm(a2[e], a3[e], 0x5410));
+        mma16816<T>(o[i][2 * e + 1], pa, __byte_perm(a0[e], a1[e], 0x7632), __byte_perm(a2[e], a3[e], 0x7632));
+      }
+    }
+    load(t + SP_STAGES * step, slot);  // this lane has read what the slot held
+    slot = slot + 1 == SP_STAGES ? 0 : slot + 1;
+  }
+  cp_wait<0>();
+  __syncthreads();  // the ring becomes the join area
+  float* part = reinterpret_cast<float*>(sm);
+  float* wm = part + SP_WARPS * SP_ROWS * DT;
+  float* wl = wm + SP_WARPS * SP_ROWS;
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
+    l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
+    const int r = g + 8 * j;
+    if (c == 0) {
+      wm[warp * SP_ROWS + r] = m[j];
+      wl[warp * SP_ROWS + r] = l[j];
+    }
+#pragma unroll
+    for (int i = 0; i < VB; i++)
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+          *reinterpret_cast<float4*>(part + (warp * SP_ROWS + r) * DT + 64 * i + 16 * c + 8 * n + e) =
+              make_float4(o[i][e][2 * j + n], o[i][e + 1][2 * j + n], o[i][e + 2][2 * j + n], o[i][e + 3][2 * j + n]);
+  }
+  sp_join<T, SP_ROWS, DT>(p, b, part, wm, wl);
+}
+
+// ---------------------------------------------------------------------------
+// f32: R rows (1, 2, 4 or 8), 8 lanes per key, lane x of them the chunks
+// x + 8 i of 4 values; 4 keys at once, 8 per stage. The R partial dots are
+// exchanged so that a lane ends with one row's whole score (R = 8: 7 shuffles
+// for 8 rows), makes that row's weight, and hands it back to the 8 lanes.
+// ---------------------------------------------------------------------------
+constexpr int SF_KT = 8;
+
+template <int CH>
+constexpr size_t sf_smem(int rows) {
+  const size_t ring = (size_t)SP_WARPS * SP_STAGES * 2 * SF_KT * CH * 32 * 4;
+  const size_t join = (size_t)SP_WARPS * rows * (CH * 32 + 2) * 4;
+  return ring > join ? ring : join;
+}
+
+template <int R, int CH>
+__global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
+  constexpr int DT = 32 * CH;
+  constexpr int SH = R == 8 ? 0 : R == 4 ? 1 : R == 2 ? 2 : 3;  // lanes per row of the 8: 2^SH
+  extern __shared__ __align__(16) uint8_t sm[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kg = lane >> 3, x8 = lane & 7;
+  SpBlock b;
+  if (!sp_block<R>(p, b)) return;
+  const int chunks = p.head_dim >> 2;
+  const int64_t kv_off = (int64_t)b.sq.slot * p.kv_slot + (int64_t)b.kvh * p.kv_head;
+  const float* kb = static_cast<const float*>(p.k) + kv_off;
+  const float* vb = static_cast<const float*>(p.v) + kv_off;
+  float4* ring = reinterpret_cast<float4*>(sm) + warp * (SP_STAGES * 4 * CH * 32) + lane;
+  const int step = (int)gridDim.x * SP_WARPS, first = (int)blockIdx.x * SP_WARPS + warp;
+  const int nt = sp_tiles<SF_KT>(b.runs);
+
+  auto load = [&](int t, int slot) {
+    if (t < nt) {
+      const SpTile x = sp_tile<SF_KT>(b.runs, t);
+      float4* dst = ring + slot * 4 * CH * 32;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int key = kg + 4 * j;
+        const int64_t off = (int64_t)(x.row + (key < x.n ? key : 0)) * p.kv_row;
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+          const bool ok = key < x.n && x8 + 8 * i < chunks;
+          cp16(dst + (j * CH + i) * 32, kb + off + (ok ? 4 * (x8 + 8 * i) : 0), ok);
+          cp16(dst + ((2 + j) * CH + i) * 32, vb + off + (ok ? 4 * (x8 + 8 * i) : 0), ok);
+        }
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < SP_STAGES; s++) load(first + s * step, s);
+
+  float4 q[R][CH], o[R][CH];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const int f = b.f0 + (r < b.nr ? r : 0);
+    const float* src = static_cast<const float*>(p.q) + (int64_t)(b.sq.q0 + f / p.group) * p.q_token +
+                       (int64_t)(b.kvh * p.group + f % p.group) * p.q_head;
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      o[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      q[r][i] = o[r][i];
+      if (r < b.nr && x8 + 8 * i < chunks) {
+        const float4 v = *reinterpret_cast<const float4*>(src + 4 * (x8 + 8 * i));
+        q[r][i] = make_float4(v.x * p.scale_log2, v.y * p.scale_log2, v.z * p.scale_log2, v.w * p.scale_log2);
+      }
+    }
+  }
+  const int mine = x8 >> SH;  // the row whose scores this lane ends with
+  const int qpos = b.sq.pos0 + (b.f0 + min(mine, b.nr - 1)) / p.group;
+  float m = -INFINITY, l = 0.f;
+
+  int slot = 0;
+#pragma unroll 1
+  for (int t = first; t < nt; t += step) {
+    const SpTile x = sp_tile<SF_KT>(b.runs, t);
+    cp_wait<SP_STAGES - 1>();
+    const float4* src = ring + slot * 4 * CH * 32;
+    float s[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      float d[R];
+#pragma unroll
+      for (int r = 0; r < R; r++) d[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < CH; i++) {
+        const float4 k = src[(j * CH + i) * 32];
+#pragma unroll
+        for (int r = 0; r < R; r++)
+          d[r] += q[r][i].x * k.x + q[r][i].y * k.y + q[r][i].z * k.z + q[r][i].w * k.w;
+      }
+      int nr = R;
+#pragma unroll
+      for (int w = 4; w >= 1; w >>= 1) {
+        if (nr > 1) {
+          nr >>= 1;
+#pragma unroll
+          for (int r = 0; r < R / 2; r++)
+            if (r < nr) {
+              const bool up = (lane & w) != 0;
+              const float send = up ? d[r] : d[r + nr], keep = up ? d[r + nr] : d[r];
+              d[r] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+            }
+        } else {
+          d[0] += __shfl_xor_sync(0xffffffffu, d[0], w);
+        }
+      }
+      const int key = kg + 4 * j;
+      s[j] = key < x.n && wa_sees(p, qpos, x.pos + key) ? d[0] : -INFINITY;
+    }
+    const float top = fmaxf(s[0], s[1]);
+    if (__any_sync(0xffffffffu, top > m + SP_SLACK)) {
+      float y = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+      y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+      const float nm = fmaxf(m, y);
+      const float f = nm == -INFINITY ? 1.f : exp2f(m - nm);
+      m = nm;
+      l *= f;
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const float fr = __shfl_sync(0xffffffffu, f, (lane & 24) | (r << SH));
+#pragma unroll
+        for (int i = 0; i < CH; i++)
+          o[r][i] = make_float4(o[r][i].x * fr, o[r][i].y * fr, o[r][i].z * fr, o[r][i].w * fr);
+      }
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const float e = exp2f(s[j] - base);
+      l += e;
+      float w[R];
+#pragma unroll
+      for (int r = 0; r < R; r++) w[r] = __shfl_sync(0xffffffffu, e, (lane & 24) | (r << SH));
+#pragma unroll
+      for (int i = 0; i < CH; i++) {
+        const float4 v = src[((2 + j) * CH + i) * 32];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          o[r][i].x += w[r] * v.x;
+          o[r][i].y += w[r] * v.y;
+          o[r][i].z += w[r] * v.z;
+          o[r][i].w += w[r] * v.w;
+        }
+      }
+    }
+    load(t + SP_STAGES * step, slot);
+    slot = slot + 1 == SP_STAGES ? 0 : slot + 1;
+  }
+  cp_wait<0>();
+  __syncthreads();
+  // the warp's four key groups added up (they share the row's maximum)
+  l += __shfl_xor_sync(0xffffffffu, l, 8);
+  l += __shfl_xor_sync(0xffffffffu, l, 16);
+  float* part = reinterpret_cast<float*>(sm);
+  float* wm = part + SP_WARPS * R * DT;
+  float* wl = wm + SP_WARPS * R;
+  if (kg == 0 && (x8 & ((1 << SH) - 1)) == 0) {
+    wm[warp * R + mine] = m;
+    wl[warp * R + mine] = l;
+  }
+#pragma unroll
+  for (int r = 0; r < R; r++)
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      float4 v = o[r][i];
+#pragma unroll
+      for (int w = 8; w <= 16; w <<= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, w);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, w);
+        v.z += __shfl_xor_sync(0xffffffffu, v.z, w);
+        v.w += __shfl_xor_sync(0xffffffffu, v.w, w);
+      }
+      if (kg == 0) *reinterpret_cast<float4*>(part + (warp * R + r) * DT + 4 * (x8 + 8 * i)) = v;
+    }
+  sp_join<float, R, DT>(p, b, part, wm, wl);
+}
+
+// Splits of one sequence and head: enough CTAs for two per SM (each keeps
+// about 100 KB of copies in flight, so that is past what the memory needs),
+// but no warp without a tile.
+int sp_split(int64_t blocks, int64_t keys, int kt) {
+  const int64_t room = 2 * (int64_t)sm_count();
+  int n = 1;
+  while (n < SP_MAX_SPLIT && blocks * n * 2 <= room && (int64_t)n * 2 * SP_WARPS * kt <= keys) n *= 2;
+  return n;
+}
+
+template <typename K>
+int sp_launch(K kernel, size_t smem, const WaParams& p, int rows, int kt, cudaStream_t s) {
+  const int64_t pairs = (int64_t)p.max_q * p.group, rb = (pairs + rows - 1) / rows;
+  const int64_t blocks = rb * (p.n_q_heads / p.group);
+  const int64_t span = std::min<int64_t>(p.max_q, (rows + p.group - 1) / p.group + 1);
+  const int64_t keys = std::min<int64_t>(p.kv_rows, (int64_t)p.window + p.n_sink + span);
+  const int split = sp_split(blocks * p.n_seq, keys, kt);
+  ARMAI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (split > 8) ARMAI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)split, (unsigned)blocks, (unsigned)p.n_seq);
+  cfg.blockDim = dim3(SP_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  ARMAI_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+  return ARMAI_OK;
+}
+
+template <typename T>
+int sp_half(const WaParams& p, cudaStream_t s) {
+  if (p.head_dim <= 64) return sp_launch(k_wa_split<T, 64>, sp_smem<T, 64>(), p, SP_ROWS, SP_KT, s);
+  if (p.head_dim <= 128) return sp_launch(k_wa_split<T, 128>, sp_smem<T, 128>(), p, SP_ROWS, SP_KT, s);
+  return sp_launch(k_wa_split<T, 256>, sp_smem<T, 256>(), p, SP_ROWS, SP_KT, s);
+}
+
+template <int R, int CH>
+int sp_f32(const WaParams& p, cudaStream_t s) {
+  return sp_launch(k_wa_split_f32<R, CH>, sf_smem<CH>(R), p, R, SF_KT, s);
+}
+// Rows per CTA as many as there are, up to eight; four at the widths where
+// eight rows of q and of the output would not fit the registers.
+template <int CH>
+int sp_f32_rows(const WaParams& p, cudaStream_t s) {
+  const int64_t pairs = (int64_t)p.max_q * p.group;
+  if (pairs <= 1) return sp_f32<1, CH>(p, s);
+  if (pairs <= 2) return sp_f32<2, CH>(p, s);
+  if constexpr (CH <= 2) {
+    if (pairs > 4) return sp_f32<8, CH>(p, s);
+  }
+  return sp_f32<4, CH>(p, s);
+}
+
+}  // namespace
+
+// Head widths of whole 16-byte vectors, and heads that fit the grid.
+bool wa_split_fits(const WaParams& p, int dtype) {
+  const int es = dtype_size(dtype), v = 16 / es;
+  return p.head_dim % v == 0 && (dtype != ARMAI_F32 || p.head_dim <= 128) &&
+         ((int64_t)p.max_q * p.group + 3) / 4 * (p.n_q_heads / p.group) <= 65535;
+}
+
+int wa_split_launch(const WaParams& p, int dtype, cudaStream_t s) {
+  if (dtype == ARMAI_F16) return sp_half<__half>(p, s);
+  if (dtype == ARMAI_BF16) return sp_half<__nv_bfloat16>(p, s);
+  switch ((p.head_dim + 31) / 32) {
+    case 1: return sp_f32_rows<1>(p, s);
+    case 2: return sp_f32_rows<2>(p, s);
+    case 3: return sp_f32_rows<3>(p, s);
+    default: return sp_f32_rows<4>(p, s);
+  }
+}
+
+}  // namespace armai
