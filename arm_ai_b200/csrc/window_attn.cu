@@ -255,7 +255,11 @@ extern "C" int armai_dev_window_attention(const armai_window_attention_args* a, 
   p.scale_log2 = a->scale * 1.4426950408889634f;
   const cudaStream_t s = (cudaStream_t)stream;
   // Few query rows per key / value head: bound by the keys, split over the device.
-  if (wa_vectors(p, a->dtype) && wa_split_fits(p, a->dtype) && (int64_t)p.max_q * p.group <= 64)
-    return wa_split_launch(p, a->dtype, s);
+  if (wa_vectors(p, a->dtype)) {
+    if (wa_split_fits(p, a->dtype) && (int64_t)p.max_q * p.group <= 64) return wa_split_launch(p, a->dtype, s);
+    bool fits = false;
+    ARMAI_TRY(wa_tc_launch(p, a->dtype, s, &fits));
+    if (fits) return ARMAI_OK;
+  }
   return wa_simt_launch(p, a->dtype, s);
 }

@@ -102,11 +102,34 @@ __device__ __forceinline__ bool wa_sees(const WaParams& p, int qpos, int kpos) {
   return kpos <= qpos && (qpos - kpos < p.window || kpos < p.n_sink);
 }
 
+// Tile t of KT keys of the runs: its first cache row, first position and keys.
+struct WaTile {
+  int row, pos, n;
+};
+template <int KT>
+__device__ __forceinline__ WaTile wa_tile(const WaRuns& r, int t) {
+  const int c0 = (r.len[0] + KT - 1) / KT, c1 = (r.len[1] + KT - 1) / KT;
+  const int s = t < c0 ? 0 : t < c0 + c1 ? 1 : 2;
+  const int o = (s == 0 ? t : s == 1 ? t - c0 : t - c0 - c1) * KT;
+  WaTile x;
+  x.row = (s == 0 ? r.row[0] : s == 1 ? r.row[1] : r.row[2]) + o;
+  x.pos = (s == 0 ? r.pos[0] : s == 1 ? r.pos[1] : r.pos[2]) + o;
+  x.n = min(KT, (s == 0 ? r.len[0] : s == 1 ? r.len[1] : r.len[2]) - o);
+  return x;
+}
+template <int KT>
+__device__ __forceinline__ int wa_tiles(const WaRuns& r) {
+  return (r.len[0] + KT - 1) / KT + (r.len[1] + KT - 1) / KT + (r.len[2] + KT - 1) / KT;
+}
+
 // Every pointer and stride a whole number of 16-byte vectors.
 bool wa_vectors(const WaParams& p, int dtype);
 
 int wa_simt_launch(const WaParams& p, int dtype, cudaStream_t s);
 bool wa_split_fits(const WaParams& p, int dtype);  // of aligned tensors (wa_vectors)
 int wa_split_launch(const WaParams& p, int dtype, cudaStream_t s);
+// Of aligned tensors; *fits false (and nothing launched): not this form's types,
+// widths, scale or strides.
+int wa_tc_launch(const WaParams& p, int dtype, cudaStream_t s, bool* fits);
 
 }  // namespace armai

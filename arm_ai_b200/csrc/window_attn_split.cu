@@ -80,26 +80,6 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uin
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Tile t of KT keys of the runs: its first cache row, first position and keys.
-struct SpTile {
-  int row, pos, n;
-};
-template <int KT>
-__device__ __forceinline__ SpTile sp_tile(const WaRuns& r, int t) {
-  const int c0 = (r.len[0] + KT - 1) / KT, c1 = (r.len[1] + KT - 1) / KT;
-  const int s = t < c0 ? 0 : t < c0 + c1 ? 1 : 2;
-  const int o = (s == 0 ? t : s == 1 ? t - c0 : t - c0 - c1) * KT;
-  SpTile x;
-  x.row = (s == 0 ? r.row[0] : s == 1 ? r.row[1] : r.row[2]) + o;
-  x.pos = (s == 0 ? r.pos[0] : s == 1 ? r.pos[1] : r.pos[2]) + o;
-  x.n = min(KT, (s == 0 ? r.len[0] : s == 1 ? r.len[1] : r.len[2]) - o);
-  return x;
-}
-template <int KT>
-__device__ __forceinline__ int sp_tiles(const WaRuns& r) {
-  return (r.len[0] + KT - 1) / KT + (r.len[1] + KT - 1) / KT + (r.len[2] + KT - 1) / KT;
-}
-
 // What a CTA works on: rows f0 .. f0 + nr - 1 of the (token, query head of
 // the group) pairs of one sequence and key / value head.
 struct SpBlock {
@@ -229,11 +209,11 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
   const T* vb = static_cast<const T*>(p.v) + kv_off;
   uint4* ring = reinterpret_cast<uint4*>(sm) + warp * (SP_STAGES * CH * 32) + lane;
   const int step = (int)gridDim.x * SP_WARPS, first = (int)blockIdx.x * SP_WARPS + warp;
-  const int nt = sp_tiles<SP_KT>(b.runs);
+  const int nt = wa_tiles<SP_KT>(b.runs);
 
   auto load = [&](int t, int slot) {
     if (t < nt) {
-      const SpTile x = sp_tile<SP_KT>(b.runs, t);
+      const WaTile x = wa_tile<SP_KT>(b.runs, t);
       uint4* dst = ring + slot * CH * 32;
 #pragma unroll
       for (int j = 0; j < 2; j++) {
@@ -293,7 +273,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
   int slot = 0;
 #pragma unroll 1
   for (int t = first; t < nt; t += step) {
-    const SpTile x = sp_tile<SP_KT>(b.runs, t);
+    const WaTile x = wa_tile<SP_KT>(b.runs, t);
     cp_wait<SP_STAGES - 1>();
     const uint4* src = ring + slot * CH * 32;
     float s[2][4];
@@ -419,11 +399,11 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
   const float* vb = static_cast<const float*>(p.v) + kv_off;
   float4* ring = reinterpret_cast<float4*>(sm) + warp * (SP_STAGES * 4 * CH * 32) + lane;
   const int step = (int)gridDim.x * SP_WARPS, first = (int)blockIdx.x * SP_WARPS + warp;
-  const int nt = sp_tiles<SF_KT>(b.runs);
+  const int nt = wa_tiles<SF_KT>(b.runs);
 
   auto load = [&](int t, int slot) {
     if (t < nt) {
-      const SpTile x = sp_tile<SF_KT>(b.runs, t);
+      const WaTile x = wa_tile<SF_KT>(b.runs, t);
       float4* dst = ring + slot * 4 * CH * 32;
 #pragma unroll
       for (int j = 0; j < 2; j++) {
@@ -465,7 +445,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
   int slot = 0;
 #pragma unroll 1
   for (int t = first; t < nt; t += step) {
-    const SpTile x = sp_tile<SF_KT>(b.runs, t);
+    const WaTile x = wa_tile<SF_KT>(b.runs, t);
     cp_wait<SP_STAGES - 1>();
     const float4* src = ring + slot * 4 * CH * 32;
     float s[2];

@@ -1,0 +1,476 @@
+// window_attn_tc.cu — window attention of many queries on the 5th-generation
+// tensor cores (f16 and bf16, head width 64 or 128).
+//
+//   S = Q K^T, P = exp2(scale S - m), O += P V, over the visible key tiles
+//
+// A CTA has two tiles of 128 query rows of one key / value head; a row is a
+// (token, query head) pair, the heads of a power-of-two part of the group
+// inside the token, so that grouped heads share the keys they read and a tile
+// spans few tokens: little of a window's edge tiles is masked away. One thread
+// streams 128-key tiles of K and V by TMA straight from the cache into a ring;
+// one thread issues the MMAs: S of each query tile into its 128 columns of
+// tensor memory, then O += P V with P (16-bit, written back over S) as the A
+// operand from tensor memory and V as the transposed (N-major) B operand from
+// the rows as they lie in the cache. Four warps per query tile, one thread
+// per row, do the softmax: no exchange between threads. While one tile's
+// softmax runs, the tensor cores work on the other's products.
+//
+// The row's maximum is raised, and its output in tensor memory rescaled, only
+// when a score exceeds it by more than 2^8: then weights stay below 2^8, sums
+// far inside f32, and most tiles need no pass over the output.
+//
+// Rounding: scores, weights and sums f32; the weights rounded once to the
+// tensors' type for P V (half a step each), the output once at the end.
+// Every wait is bounded; rows whose wait gave up are written as NaN.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+#include <type_traits>
+
+#include "tcgen05.cuh"
+#include "window_attn.cuh"
+
+namespace armai {
+namespace {
+
+constexpr int WT_KT = 128;                     // keys per tile
+constexpr int WT_ROWS = 128;                   // query rows per tile, two tiles per CTA
+constexpr int WT_LOAD = 8, WT_MMA = 9;         // warps 0-3, 4-7: softmax of tile 0, 1
+constexpr int WT_THREADS = 320;
+constexpr float WT_SLACK = 8.f;
+
+template <int HD>
+struct WtLayout {
+  static constexpr uint32_t TILE = 128u * HD * 2u;       // one operand tile: HD / 64 blocks of 128 rows x 128 B
+  static constexpr int SLOTS = HD == 128 ? 5 : 8;        // K and V tiles in turn
+  static constexpr uint32_t BAR = (2 + SLOTS) * TILE;
+  static constexpr uint32_t SMEM = 1024 + BAR + 256;
+};
+
+// tcgen05.ld / st of 32 columns of this warp's 32 lanes; the caller waits.
+__device__ __forceinline__ void wt_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// Waits for the loads; the values pass through it, so that no use of them is
+// moved ahead of it.
+__device__ __forceinline__ void wt_wait_ld(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void wt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wt_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ float wt_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t wt_pack(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t wt_pack<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t wt_pack<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// N-major operand (rows are K, N contiguous), 128-byte swizzle: blocks of 64
+// N values `lead` bytes apart, 8-row groups 1024 B apart.
+__device__ __forceinline__ uint64_t wt_desc_n(uint32_t saddr, uint32_t lead) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(lead >> 4) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
+  return d;
+}
+
+__device__ __forceinline__ void wt_tma3(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void wt_tma4(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// The CTA's work, the same for every thread: its tokens, each query tile's
+// positions, the runs and their tiles.
+struct WtWork {
+  WaSeq sq;
+  WaRuns runs;
+  int vh, kvh, i0, nt;
+  int qlo[2], qhi[2];  // positions of a query tile's first and last token; qhi < qlo: no token
+
+  // whether any row of query tile h sees a key of the tile
+  __device__ __forceinline__ bool needs(const WaParams& p, int h, const WaTile& x) const {
+    const int lo = h ? qlo[1] : qlo[0], hi = h ? qhi[1] : qhi[0];
+    return lo <= hi && x.pos <= hi && (lo - (x.pos + x.n - 1) < p.window || x.pos < p.n_sink);
+  }
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(WT_THREADS, 1)
+    k_wa_tc(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+            const __grid_constant__ CUtensorMap mv, const WaParams p, int pack) {
+  using L = WtLayout<HD>;
+  extern __shared__ uint8_t wt_raw[];
+  const uint32_t raw = smem_u32(wt_raw);
+  uint8_t* smem = wt_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint8_t* qs = smem;                  // two query tiles
+  uint8_t* ring = smem + 2 * L::TILE;  // SLOTS tiles: K of a key tile, then V
+  uint64_t* qfull = reinterpret_cast<uint64_t*>(smem + L::BAR);
+  uint64_t* full = qfull + 1;          // [SLOTS]
+  uint64_t* empty = full + L::SLOTS;   // [SLOTS]
+  uint64_t* sfull = empty + L::SLOTS;  // [2] S of query tile h written
+  uint64_t* pready = sfull + 2;        // [2] P of query tile h in place
+  uint64_t* pvdone = pready + 2;       // [2] P V of query tile h added
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(pvdone + 2);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  WtWork w;
+  w.sq = wa_seq(p, blockIdx.z);
+  const int tokens = WT_ROWS / pack;   // per query tile
+  w.i0 = (int)(gridDim.x - 1 - blockIdx.x) * 2 * tokens;  // the longest causal rows first
+  if (w.i0 >= w.sq.n) return;
+  w.vh = blockIdx.y;
+  w.kvh = w.vh * pack / p.group;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    w.qlo[h] = w.sq.pos0 + w.i0 + h * tokens;
+    w.qhi[h] = w.sq.pos0 + min(w.sq.n, w.i0 + (h + 1) * tokens) - 1;
+  }
+  w.runs = wa_runs(p, w.qlo[0], max(w.qhi[0], w.qhi[1]));
+  w.nt = wa_tiles<WT_KT>(w.runs);
+
+  if (tid == 0) {
+    mbar_init(qfull, 1);
+    for (int i = 0; i < L::SLOTS; i++) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int h = 0; h < 2; h++) {
+      mbar_init(&sfull[h], 1);
+      mbar_init(&pready[h], 4);
+      mbar_init(&pvdone[h], 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 0) tmem_alloc(tslot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;  // S 0: columns 0-127, S 1: 128-255, O 0: 256 .., O 1: 384 ..
+
+  if (warp == WT_LOAD) {
+    if (lane == 0) {
+      mbar_arrive_tx(qfull, 2 * L::TILE);
+      for (int h = 0; h < 2; h++)
+        for (int kb = 0; kb < HD / 64; kb++)
+          wt_tma3(qs + h * L::TILE + kb * 16384, &mq, 64 * kb, w.vh * pack, w.sq.q0 + w.i0 + h * tokens, qfull);
+      int issued = 0;
+      bool ok = true;
+      for (int j = 0; j < 2 * w.nt && ok; j++) {
+        const int s = j % L::SLOTS;
+        if (j >= L::SLOTS) ok = qg_wait(&empty[s], (uint32_t)((j / L::SLOTS - 1) & 1), p.err);
+        if (!ok) break;
+        const WaTile x = wa_tile<WT_KT>(w.runs, j >> 1);
+        mbar_arrive_tx(&full[s], L::TILE);
+        for (int kb = 0; kb < HD / 64; kb++)
+          wt_tma4(ring + s * L::TILE + kb * 16384, (j & 1) ? &mv : &mk, 64 * kb, x.row, w.kvh, w.sq.slot, &full[s]);
+        issued = j + 1;
+      }
+      // every requested box has landed before the CTA may end
+      qg_wait(qfull, 0, p.err);
+      for (int j = issued > L::SLOTS ? issued - L::SLOTS : 0; j < issued; j++)
+        qg_wait(&full[j % L::SLOTS], (uint32_t)((j / L::SLOTS) & 1), p.err);
+    }
+  } else if (warp == WT_MMA) {
+    constexpr uint32_t TY = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t BASE = (1u << 4) | (TY << 7) | (TY << 10) | ((uint32_t)(WT_ROWS >> 4) << 24);
+    int done[2] = {0, 0};  // products P V issued per query tile
+    bool ok = qg_wait_warp(qfull, 0, p.err);
+    auto qk = [&](int h, const WaTile& x, int s) {
+      if (!ok || !w.needs(p, h, x)) return;
+      const int n = h ? done[1] : done[0];
+      // its columns held P of the tile before
+      if (n > 0) ok = qg_wait_warp(&pvdone[h], (uint32_t)((n - 1) & 1), p.err);
+      if (!ok) return;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t qa = smem_u32(qs + h * L::TILE), ka = smem_u32(ring + s * L::TILE);
+        const uint32_t idesc = BASE | ((uint32_t)((x.n + 15) >> 4) << 18);  // N = the tile's keys, in steps of 16
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; kk++) {
+          const uint32_t off = (uint32_t)(kk >> 2) * 16384u + 32u * (uint32_t)(kk & 3);
+          tc_mma_ss(tmem + 128u * (uint32_t)h, qg_smem_desc(qa + off), qg_smem_desc(ka + off), idesc, kk > 0);
+        }
+        qg_commit(&sfull[h]);
+      }
+      __syncwarp();
+    };
+    auto pv = [&](int h, const WaTile& x, int s) {
+      if (!ok || !w.needs(p, h, x)) return;
+      const int n = h ? done[1] : done[0];
+      ok = qg_wait_warp(&pready[h], (uint32_t)(n & 1), p.err);
+      if (!ok) return;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t va = smem_u32(ring + s * L::TILE), o = tmem + 256u + 128u * (uint32_t)h;
+        const uint32_t idesc = BASE | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
+        const int steps = (x.n + 15) >> 4;
+        for (int kk = 0; kk < steps; kk++)
+          qg_mma_ts(o, tmem + 128u * (uint32_t)h + 8u * (uint32_t)kk, wt_desc_n(va + 2048u * (uint32_t)kk, 16384u),
+                    idesc, (n > 0 || kk > 0) ? 1u : 0u);
+        qg_commit(&pvdone[h]);
+      }
+      __syncwarp();
+      if (h) done[1]++; else done[0]++;
+    };
+    auto arrived = [&](int j) {  // operand tile j of the ring
+      if (ok) ok = qg_wait_warp(&full[j % L::SLOTS], (uint32_t)((j / L::SLOTS) & 1), p.err);
+      if (ok) tc_fence_after();
+    };
+    auto release = [&](int j) {
+      if (ok && lane == 0) qg_commit(&empty[j % L::SLOTS]);
+      __syncwarp();
+    };
+    WaTile x = wa_tile<WT_KT>(w.runs, 0);
+    if (w.nt > 0) {
+      arrived(0);
+      qk(0, x, 0);
+      qk(1, x, 0);
+      release(0);
+    }
+    for (int t = 0; t < w.nt && ok; t++) {
+      const int vs = (2 * t + 1) % L::SLOTS, ks = (2 * t + 2) % L::SLOTS;
+      const bool more = t + 1 < w.nt;
+      const WaTile y = wa_tile<WT_KT>(w.runs, more ? t + 1 : t);
+      arrived(2 * t + 1);
+      if (ok && (x.n & 15)) {
+        // the last product of 16 keys also reads rows behind the tile's: zero
+        // them (their weights are zero, but the rows may hold anything)
+        const int r0 = x.n, rows = 16 - (x.n & 15);
+        for (int e = lane; e < rows * (HD / 8); e += 32)
+          *reinterpret_cast<uint4*>(ring + vs * L::TILE + (e & 7) * 16 + (r0 + (e >> 3) % rows) * 128 +
+                                    ((e >> 3) / rows) * 16384) = make_uint4(0u, 0u, 0u, 0u);
+        fence_async_smem();
+        __syncwarp();
+      }
+      pv(0, x, vs);
+      if (more) {
+        arrived(2 * t + 2);
+        qk(0, y, ks);
+      }
+      pv(1, x, vs);
+      release(2 * t + 1);
+      if (more) {
+        qk(1, y, ks);
+        release(2 * t + 2);
+      }
+      x = y;
+    }
+  } else {
+    // ---- softmax: thread = query row ----
+    const int h = warp >> 2, row = tid & 127;
+    const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t ts = tmem + lane_base + 128u * (uint32_t)h, to = ts + 256u;
+    const int tok = w.i0 + h * tokens + row / pack, head = w.vh * pack + row % pack;
+    const int qpos = w.sq.pos0 + tok;
+    const float sl = p.scale_log2;
+    float m = -INFINITY, l = 0.f;
+    int n = 0;
+    bool ok = true;
+    for (int t = 0; t < w.nt; t++) {
+      const WaTile x = wa_tile<WT_KT>(w.runs, t);
+      if (!w.needs(p, h, x)) continue;
+      ok = qg_wait_warp(&sfull[h], (uint32_t)(n & 1), p.err);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[128];
+#pragma unroll
+      for (int c = 0; c < 4; c++) wt_ld32(ts + 32u * c, s + 32 * c);
+#pragma unroll
+      for (int c = 0; c < 4; c++) wt_wait_ld(s + 32 * c);
+      // columns first .. last are seen, and those before `sink`
+      const int last = min(x.n - 1, qpos - x.pos), first = qpos - x.pos - p.window + 1, sink = p.n_sink - x.pos;
+      const bool all = last == WT_KT - 1 && (first <= 0 || sink >= WT_KT);
+      if (!__all_sync(0xffffffffu, all)) {
+#pragma unroll
+        for (int c = 0; c < 128; c++)
+          if (c > last || (c < first && c >= sink)) s[c] = 0xff800000u;  // -inf
+      }
+      float a[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++) a[c] = __uint_as_float(s[c]);
+#pragma unroll
+      for (int c = 4; c < 128; c += 4)
+#pragma unroll
+        for (int k = 0; k < 4; k++) a[k] = fmaxf(a[k], __uint_as_float(s[c + k]));
+      const float top = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * sl;
+      if (__any_sync(0xffffffffu, top > m + WT_SLACK)) {
+        const float nm = fmaxf(m, top);
+        const float f = nm == -INFINITY ? 1.f : wt_exp2(m - nm);
+        m = nm;
+        l *= f;
+        if (n > 0) {
+          ok = qg_wait_warp(&pvdone[h], (uint32_t)((n - 1) & 1), p.err);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t o[32];
+            wt_ld32(to + c, o);
+            wt_wait_ld(o);
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            wt_st32(to + c, o);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 128; c += 4) {
+        float e[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          e[k] = wt_exp2(fmaf(__uint_as_float(s[c + k]), sl, -base));
+          sum[k] += e[k];
+        }
+        s[c >> 1] = wt_pack<T>(e[0], e[1]);
+        s[(c >> 1) + 1] = wt_pack<T>(e[2], e[3]);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      wt_st32(ts, s);
+      wt_st32(ts + 32u, s + 32);
+      wt_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(&pready[h]);
+      n++;
+    }
+    if (ok && n > 0) ok = qg_wait_warp(&pvdone[h], (uint32_t)((n - 1) & 1), p.err);
+    tc_fence_after();
+    const float inv = !ok ? __int_as_float(0x7fc00000) : l == 0.f ? 0.f : 1.0f / l;
+    T* out = static_cast<T*>(p.out) + (int64_t)(w.sq.q0 + tok) * p.o_token + (int64_t)head * p.o_head;
+#pragma unroll 1
+    for (int c = 0; c < HD; c += 32) {
+      uint32_t o[32];
+      wt_ld32(to + c, o);
+      wt_wait_ld(o);
+      if (tok < w.sq.n) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          uint32_t v[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++)  // no key seen: the columns were never written
+            v[k] = ok && (n == 0 || l == 0.f) ? 0u
+                                              : wt_pack<T>(__uint_as_float(o[e + 2 * k]) * inv,
+                                                           __uint_as_float(o[e + 2 * k + 1]) * inv);
+          *reinterpret_cast<uint4*>(out + c + e) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 wt_encoder() {
+  static std::once_flag once;
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  std::call_once(once, [] {
+    cudaDriverEntryPointQueryResult q;
+    void* f = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  return fn;
+}
+
+bool wt_map(CUtensorMap* map, int dtype, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+            const cuuint32_t* box) {
+  const auto enc = wt_encoder();
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  return enc &&
+         enc(map, dtype == ARMAI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank,
+             const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+__device__ uint32_t g_wt_err;
+
+template <typename T, int HD>
+int wt_launch(const WaParams& in, int dtype, cudaStream_t s, bool* fits) {
+  WaParams p = in;
+  const int n_kv = p.n_q_heads / p.group;
+  int pack = 1;  // heads per token in a tile: the power of two in the group
+  while (pack < 128 && p.group % (2 * pack) == 0) pack *= 2;
+  CUtensorMap mq, mk, mv;
+  const cuuint64_t qd[3] = {(cuuint64_t)HD, (cuuint64_t)p.n_q_heads, (cuuint64_t)p.n_tokens};
+  const cuuint64_t qst[2] = {(cuuint64_t)p.q_head * 2, (cuuint64_t)p.q_token * 2};
+  const cuuint32_t qb[3] = {64, (cuuint32_t)pack, (cuuint32_t)(WT_ROWS / pack)};
+  const cuuint64_t kd[4] = {(cuuint64_t)HD, (cuuint64_t)p.kv_rows, (cuuint64_t)n_kv, (cuuint64_t)p.n_slots};
+  const cuuint64_t kst[3] = {(cuuint64_t)p.kv_row * 2, (cuuint64_t)p.kv_head * 2, (cuuint64_t)p.kv_slot * 2};
+  const cuuint32_t kb[4] = {64, WT_KT, 1, 1};
+  *fits = wt_map(&mq, dtype, 3, p.q, qd, qst, qb) && wt_map(&mk, dtype, 4, p.k, kd, kst, kb) &&
+          wt_map(&mv, dtype, 4, p.v, kd, kst, kb);
+  if (!*fits) return ARMAI_OK;
+  ARMAI_CUDA(cudaGetSymbolAddress((void**)&p.err, g_wt_err));
+  ARMAI_CUDA(cudaFuncSetAttribute(k_wa_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WtLayout<HD>::SMEM));
+  const int tokens = 2 * WT_ROWS / pack;
+  const dim3 grid((unsigned)((p.max_q + tokens - 1) / tokens), (unsigned)(p.n_q_heads / pack), (unsigned)p.n_seq);
+  k_wa_tc<T, HD><<<grid, WT_THREADS, WtLayout<HD>::SMEM, s>>>(mq, mk, mv, p, pack);
+  ARMAI_CUDA(cudaGetLastError());
+  return ARMAI_OK;
+}
+
+}  // namespace
+
+int wa_tc_launch(const WaParams& p, int dtype, cudaStream_t s, bool* fits) {
+  *fits = dtype != ARMAI_F32 && (p.head_dim == 64 || p.head_dim == 128) && p.scale_log2 > 0.f;
+  if (!*fits) return ARMAI_OK;
+  if (dtype == ARMAI_F16) return p.head_dim == 64 ? wt_launch<__half, 64>(p, dtype, s, fits) : wt_launch<__half, 128>(p, dtype, s, fits);
+  return p.head_dim == 64 ? wt_launch<__nv_bfloat16, 64>(p, dtype, s, fits) : wt_launch<__nv_bfloat16, 128>(p, dtype, s, fits);
+}
+
+}  // namespace armai
