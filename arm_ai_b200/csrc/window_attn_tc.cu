@@ -37,7 +37,11 @@ namespace {
 constexpr int WT_KT = 128;                     // keys per tile
 constexpr int WT_ROWS = 128;                   // query rows per tile, two tiles per CTA
 constexpr int WT_LOAD = 8, WT_MMA = 9;         // warps 0-3, 4-7: softmax of tile 0, 1
-constexpr int WT_THREADS = 320;
+constexpr int WT_THREADS = 384;                // warps 10, 11 only complete the warp group
+// Registers: 384 x 168 at launch; the loading group gives up what the softmax
+// threads (128 scores each) need: 256 x 216 + 128 x 72 = 384 x 168.
+constexpr int WT_REGS = 168, WT_REGS_SOFTMAX = 216, WT_REGS_LOAD = 72;
+static_assert(256 * WT_REGS_SOFTMAX + 128 * WT_REGS_LOAD <= WT_THREADS * WT_REGS, "register split");
 constexpr float WT_SLACK = 8.f;
 
 template <int HD>
@@ -86,6 +90,31 @@ __device__ __forceinline__ float wt_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two f32 operations per instruction.
+__device__ __forceinline__ uint64_t wt_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void wt_unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t wt_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t wt_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float wt_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 template <typename T>
@@ -194,115 +223,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tslot;  // S 0: columns 0-127, S 1: 128-255, O 0: 256 .., O 1: 384 ..
 
-  if (warp == WT_LOAD) {
-    if (lane == 0) {
-      mbar_arrive_tx(qfull, 2 * L::TILE);
-      for (int h = 0; h < 2; h++)
-        for (int kb = 0; kb < HD / 64; kb++)
-          wt_tma3(qs + h * L::TILE + kb * 16384, &mq, 64 * kb, w.vh * pack, w.sq.q0 + w.i0 + h * tokens, qfull);
-      int issued = 0;
-      bool ok = true;
-      for (int j = 0; j < 2 * w.nt && ok; j++) {
-        const int s = j % L::SLOTS;
-        if (j >= L::SLOTS) ok = qg_wait(&empty[s], (uint32_t)((j / L::SLOTS - 1) & 1), p.err);
-        if (!ok) break;
-        const WaTile x = wa_tile<WT_KT>(w.runs, j >> 1);
-        mbar_arrive_tx(&full[s], L::TILE);
-        for (int kb = 0; kb < HD / 64; kb++)
-          wt_tma4(ring + s * L::TILE + kb * 16384, (j & 1) ? &mv : &mk, 64 * kb, x.row, w.kvh, w.sq.slot, &full[s]);
-        issued = j + 1;
-      }
-      // every requested box has landed before the CTA may end
-      qg_wait(qfull, 0, p.err);
-      for (int j = issued > L::SLOTS ? issued - L::SLOTS : 0; j < issued; j++)
-        qg_wait(&full[j % L::SLOTS], (uint32_t)((j / L::SLOTS) & 1), p.err);
-    }
-  } else if (warp == WT_MMA) {
-    constexpr uint32_t TY = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    constexpr uint32_t BASE = (1u << 4) | (TY << 7) | (TY << 10) | ((uint32_t)(WT_ROWS >> 4) << 24);
-    int done[2] = {0, 0};  // products P V issued per query tile
-    bool ok = qg_wait_warp(qfull, 0, p.err);
-    auto qk = [&](int h, const WaTile& x, int s) {
-      if (!ok || !w.needs(p, h, x)) return;
-      const int n = h ? done[1] : done[0];
-      // its columns held P of the tile before
-      if (n > 0) ok = qg_wait_warp(&pvdone[h], (uint32_t)((n - 1) & 1), p.err);
-      if (!ok) return;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t qa = smem_u32(qs + h * L::TILE), ka = smem_u32(ring + s * L::TILE);
-        const uint32_t idesc = BASE | ((uint32_t)((x.n + 15) >> 4) << 18);  // N = the tile's keys, in steps of 16
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; kk++) {
-          const uint32_t off = (uint32_t)(kk >> 2) * 16384u + 32u * (uint32_t)(kk & 3);
-          tc_mma_ss(tmem + 128u * (uint32_t)h, qg_smem_desc(qa + off), qg_smem_desc(ka + off), idesc, kk > 0);
-        }
-        qg_commit(&sfull[h]);
-      }
-      __syncwarp();
-    };
-    auto pv = [&](int h, const WaTile& x, int s) {
-      if (!ok || !w.needs(p, h, x)) return;
-      const int n = h ? done[1] : done[0];
-      ok = qg_wait_warp(&pready[h], (uint32_t)(n & 1), p.err);
-      if (!ok) return;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t va = smem_u32(ring + s * L::TILE), o = tmem + 256u + 128u * (uint32_t)h;
-        const uint32_t idesc = BASE | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
-        const int steps = (x.n + 15) >> 4;
-        for (int kk = 0; kk < steps; kk++)
-          qg_mma_ts(o, tmem + 128u * (uint32_t)h + 8u * (uint32_t)kk, wt_desc_n(va + 2048u * (uint32_t)kk, 16384u),
-                    idesc, (n > 0 || kk > 0) ? 1u : 0u);
-        qg_commit(&pvdone[h]);
-      }
-      __syncwarp();
-      if (h) done[1]++; else done[0]++;
-    };
-    auto arrived = [&](int j) {  // operand tile j of the ring
-      if (ok) ok = qg_wait_warp(&full[j % L::SLOTS], (uint32_t)((j / L::SLOTS) & 1), p.err);
-      if (ok) tc_fence_after();
-    };
-    auto release = [&](int j) {
-      if (ok && lane == 0) qg_commit(&empty[j % L::SLOTS]);
-      __syncwarp();
-    };
-    WaTile x = wa_tile<WT_KT>(w.runs, 0);
-    if (w.nt > 0) {
-      arrived(0);
-      qk(0, x, 0);
-      qk(1, x, 0);
-      release(0);
-    }
-    for (int t = 0; t < w.nt && ok; t++) {
-      const int vs = (2 * t + 1) % L::SLOTS, ks = (2 * t + 2) % L::SLOTS;
-      const bool more = t + 1 < w.nt;
-      const WaTile y = wa_tile<WT_KT>(w.runs, more ? t + 1 : t);
-      arrived(2 * t + 1);
-      if (ok && (x.n & 15)) {
-        // the last product of 16 keys also reads rows behind the tile's: zero
-        // them (their weights are zero, but the rows may hold anything)
-        const int r0 = x.n, rows = 16 - (x.n & 15);
-        for (int e = lane; e < rows * (HD / 8); e += 32)
-          *reinterpret_cast<uint4*>(ring + vs * L::TILE + (e & 7) * 16 + (r0 + (e >> 3) % rows) * 128 +
-                                    ((e >> 3) / rows) * 16384) = make_uint4(0u, 0u, 0u, 0u);
-        fence_async_smem();
-        __syncwarp();
-      }
-      pv(0, x, vs);
-      if (more) {
-        arrived(2 * t + 2);
-        qk(0, y, ks);
-      }
-      pv(1, x, vs);
-      release(2 * t + 1);
-      if (more) {
-        qk(1, y, ks);
-        release(2 * t + 2);
-      }
-      x = y;
-    }
-  } else {
+  if (warp < WT_LOAD) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(WT_REGS_SOFTMAX));
     // ---- softmax: thread = query row ----
     const int h = warp >> 2, row = tid & 127;
     const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
@@ -336,9 +258,11 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
 #pragma unroll
       for (int c = 0; c < 4; c++) a[c] = __uint_as_float(s[c]);
 #pragma unroll
-      for (int c = 4; c < 128; c += 4)
+      for (int c = 4; c + 8 <= 128; c += 8)
 #pragma unroll
-        for (int k = 0; k < 4; k++) a[k] = fmaxf(a[k], __uint_as_float(s[c + k]));
+        for (int k = 0; k < 4; k++) a[k] = wt_max3(a[k], __uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1]));
+#pragma unroll
+      for (int k = 0; k < 4; k++) a[k] = fmaxf(a[k], __uint_as_float(s[124 + k]));
       const float top = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * sl;
       if (__any_sync(0xffffffffu, top > m + WT_SLACK)) {
         const float nm = fmaxf(m, top);
@@ -361,19 +285,25 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         }
       }
       const float base = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t sl2 = wt_pair(sl, sl), nb2 = wt_pair(-base, -base);
+      uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < 128; c += 4) {
-        float e[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          e[k] = wt_exp2(fmaf(__uint_as_float(s[c + k]), sl, -base));
-          sum[k] += e[k];
+        for (int k = 0; k < 2; k++) {
+          float e0, e1;
+          wt_unpair(wt_fma2(wt_pair(__uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1])), sl2, nb2), e0, e1);
+          e0 = wt_exp2(e0);
+          e1 = wt_exp2(e1);
+          sum[k] = wt_add2(sum[k], wt_pair(e0, e1));
+          s[(c >> 1) + k] = wt_pack<T>(e0, e1);
         }
-        s[c >> 1] = wt_pack<T>(e[0], e[1]);
-        s[(c >> 1) + 1] = wt_pack<T>(e[2], e[3]);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      {
+        float e0, e1;
+        wt_unpair(wt_add2(sum[0], sum[1]), e0, e1);
+        l += e0 + e1;
+      }
       wt_st32(ts, s);
       wt_st32(ts + 32u, s + 32);
       wt_wait_st();
@@ -402,6 +332,117 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
                                                            __uint_as_float(o[e + 2 * k + 1]) * inv);
           *reinterpret_cast<uint4*>(out + c + e) = make_uint4(v[0], v[1], v[2], v[3]);
         }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WT_REGS_LOAD));
+    if (warp == WT_LOAD) {
+      if (lane == 0) {
+        mbar_arrive_tx(qfull, 2 * L::TILE);
+        for (int h = 0; h < 2; h++)
+          for (int kb = 0; kb < HD / 64; kb++)
+            wt_tma3(qs + h * L::TILE + kb * 16384, &mq, 64 * kb, w.vh * pack, w.sq.q0 + w.i0 + h * tokens, qfull);
+        int issued = 0;
+        bool ok = true;
+        for (int j = 0; j < 2 * w.nt && ok; j++) {
+          const int s = j % L::SLOTS;
+          if (j >= L::SLOTS) ok = qg_wait(&empty[s], (uint32_t)((j / L::SLOTS - 1) & 1), p.err);
+          if (!ok) break;
+          const WaTile x = wa_tile<WT_KT>(w.runs, j >> 1);
+          mbar_arrive_tx(&full[s], L::TILE);
+          for (int kb = 0; kb < HD / 64; kb++)
+            wt_tma4(ring + s * L::TILE + kb * 16384, (j & 1) ? &mv : &mk, 64 * kb, x.row, w.kvh, w.sq.slot, &full[s]);
+          issued = j + 1;
+        }
+        // every requested box has landed before the CTA may end
+        qg_wait(qfull, 0, p.err);
+        for (int j = issued > L::SLOTS ? issued - L::SLOTS : 0; j < issued; j++)
+          qg_wait(&full[j % L::SLOTS], (uint32_t)((j / L::SLOTS) & 1), p.err);
+      }
+    } else if (warp == WT_MMA) {
+      constexpr uint32_t TY = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      constexpr uint32_t BASE = (1u << 4) | (TY << 7) | (TY << 10) | ((uint32_t)(WT_ROWS >> 4) << 24);
+      int done[2] = {0, 0};  // products P V issued per query tile
+      bool ok = qg_wait_warp(qfull, 0, p.err);
+      auto qk = [&](int h, const WaTile& x, int s) {
+        if (!ok || !w.needs(p, h, x)) return;
+        const int n = h ? done[1] : done[0];
+        // its columns held P of the tile before
+        if (n > 0) ok = qg_wait_warp(&pvdone[h], (uint32_t)((n - 1) & 1), p.err);
+        if (!ok) return;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t qa = smem_u32(qs + h * L::TILE), ka = smem_u32(ring + s * L::TILE);
+          const uint32_t idesc = BASE | ((uint32_t)((x.n + 15) >> 4) << 18);  // N = the tile's keys, in steps of 16
+  #pragma unroll
+          for (int kk = 0; kk < HD / 16; kk++) {
+            const uint32_t off = (uint32_t)(kk >> 2) * 16384u + 32u * (uint32_t)(kk & 3);
+            tc_mma_ss(tmem + 128u * (uint32_t)h, qg_smem_desc(qa + off), qg_smem_desc(ka + off), idesc, kk > 0);
+          }
+          qg_commit(&sfull[h]);
+        }
+        __syncwarp();
+      };
+      auto pv = [&](int h, const WaTile& x, int s) {
+        if (!ok || !w.needs(p, h, x)) return;
+        const int n = h ? done[1] : done[0];
+        ok = qg_wait_warp(&pready[h], (uint32_t)(n & 1), p.err);
+        if (!ok) return;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t va = smem_u32(ring + s * L::TILE), o = tmem + 256u + 128u * (uint32_t)h;
+          const uint32_t idesc = BASE | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
+          const int steps = (x.n + 15) >> 4;
+          for (int kk = 0; kk < steps; kk++)
+            qg_mma_ts(o, tmem + 128u * (uint32_t)h + 8u * (uint32_t)kk, wt_desc_n(va + 2048u * (uint32_t)kk, 16384u),
+                      idesc, (n > 0 || kk > 0) ? 1u : 0u);
+          qg_commit(&pvdone[h]);
+        }
+        __syncwarp();
+        if (h) done[1]++; else done[0]++;
+      };
+      auto arrived = [&](int j) {  // operand tile j of the ring
+        if (ok) ok = qg_wait_warp(&full[j % L::SLOTS], (uint32_t)((j / L::SLOTS) & 1), p.err);
+        if (ok) tc_fence_after();
+      };
+      auto release = [&](int j) {
+        if (ok && lane == 0) qg_commit(&empty[j % L::SLOTS]);
+        __syncwarp();
+      };
+      WaTile x = wa_tile<WT_KT>(w.runs, 0);
+      if (w.nt > 0) {
+        arrived(0);
+        qk(0, x, 0);
+        qk(1, x, 0);
+        release(0);
+      }
+      for (int t = 0; t < w.nt && ok; t++) {
+        const int vs = (2 * t + 1) % L::SLOTS, ks = (2 * t + 2) % L::SLOTS;
+        const bool more = t + 1 < w.nt;
+        const WaTile y = wa_tile<WT_KT>(w.runs, more ? t + 1 : t);
+        arrived(2 * t + 1);
+        if (ok && (x.n & 15)) {
+          // the last product of 16 keys also reads rows behind the tile's: zero
+          // them (their weights are zero, but the rows may hold anything)
+          const int r0 = x.n, rows = 16 - (x.n & 15);
+          for (int e = lane; e < rows * (HD / 8); e += 32)
+            *reinterpret_cast<uint4*>(ring + vs * L::TILE + (e & 7) * 16 + (r0 + (e >> 3) % rows) * 128 +
+                                      ((e >> 3) / rows) * 16384) = make_uint4(0u, 0u, 0u, 0u);
+          fence_async_smem();
+          __syncwarp();
+        }
+        pv(0, x, vs);
+        if (more) {
+          arrived(2 * t + 2);
+          qk(0, y, ks);
+        }
+        pv(1, x, vs);
+        release(2 * t + 1);
+        if (more) {
+          qk(1, y, ks);
+          release(2 * t + 2);
+        }
+        x = y;
       }
     }
   }
@@ -456,6 +497,14 @@ int wt_launch(const WaParams& in, int dtype, cudaStream_t s, bool* fits) {
           wt_map(&mv, dtype, 4, p.v, kd, kst, kb);
   if (!*fits) return ARMAI_OK;
   ARMAI_CUDA(cudaGetSymbolAddress((void**)&p.err, g_wt_err));
+  // the register split waits for registers that a smaller launch would not have
+  static thread_local int regs = 0;
+  if (!regs) {
+    cudaFuncAttributes fa;
+    ARMAI_CUDA(cudaFuncGetAttributes(&fa, k_wa_tc<T, HD>));
+    regs = fa.numRegs;
+  }
+  if (regs != WT_REGS) return fail(ARMAI_E_INVALID, "window_attn: the tensor-core kernel was built with " + std::to_string(regs) + " registers");
   ARMAI_CUDA(cudaFuncSetAttribute(k_wa_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WtLayout<HD>::SMEM));
   const int tokens = 2 * WT_ROWS / pack;
   const dim3 grid((unsigned)((p.max_q + tokens - 1) / tokens), (unsigned)(p.n_q_heads / pack), (unsigned)p.n_seq);
