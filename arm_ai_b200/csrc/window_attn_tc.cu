@@ -36,8 +36,8 @@ namespace {
 
 constexpr int WT_KT = 128;                     // keys per tile
 constexpr int WT_ROWS = 128;                   // query rows per tile, two tiles per CTA
-constexpr int WT_LOAD = 8, WT_MMA = 9;         // warps 0-3, 4-7: softmax of tile 0, 1
-constexpr int WT_THREADS = 384;                // warps 10, 11 only complete the warp group
+constexpr int WT_LOAD = 8, WT_MMA = 9, WT_CLEAN = 10;  // warps 0-3, 4-7: softmax of tile 0, 1
+constexpr int WT_THREADS = 384;                // warp 11 only completes the warp group
 // Registers: 384 x 168 at launch; the loading group gives up what the softmax
 // threads (128 scores each) need: 256 x 216 + 128 x 72 = 384 x 168.
 constexpr int WT_REGS = 168, WT_REGS_SOFTMAX = 216, WT_REGS_LOAD = 72;
@@ -130,16 +130,24 @@ __device__ __forceinline__ uint32_t wt_pack<__nv_bfloat16>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// N-major operand (rows are K, N contiguous), 128-byte swizzle: blocks of 64
-// N values `lead` bytes apart, 8-row groups 1024 B apart.
-__device__ __forceinline__ uint64_t wt_desc_n(uint32_t saddr, uint32_t lead) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-  d |= (uint64_t)(lead >> 4) << 16;
-  d |= (uint64_t)(1024u >> 4) << 32;
-  d |= (uint64_t)1u << 46;
-  d |= (uint64_t)2u << 61;
-  return d;
+// The row's weights exp2(scale s - base) over its scores, as pairs of T in
+// s[0 .. 63]; returns their f32 sum (of the unrounded values).
+template <typename T>
+__device__ __forceinline__ float wt_weights(uint32_t (&s)[128], float sl, float base) {
+  const uint64_t sl2 = wt_pair(sl, sl), nb2 = wt_pair(-base, -base);
+  uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+  for (int c = 0; c < 64; c++) {
+    float e0, e1;
+    wt_unpair(wt_fma2(wt_pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sl2, nb2), e0, e1);
+    e0 = wt_exp2(e0);
+    e1 = wt_exp2(e1);
+    sum[c & 1] = wt_add2(sum[c & 1], wt_pair(e0, e1));
+    s[c] = wt_pack<T>(e0, e1);
+  }
+  float e0, e1;
+  wt_unpair(wt_add2(sum[0], sum[1]), e0, e1);
+  return e0 + e1;
 }
 
 __device__ __forceinline__ void wt_tma3(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
@@ -170,6 +178,65 @@ struct WtWork {
   }
 };
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool wt_elect() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e != 0;
+}
+
+// The key tiles one after another.
+struct WtIter {
+  WaTile x;
+  int run, left;
+  __device__ __forceinline__ void enter(const WaRuns& r) {
+    x.row = run == 0 ? r.row[0] : run == 1 ? r.row[1] : r.row[2];
+    x.pos = run == 0 ? r.pos[0] : run == 1 ? r.pos[1] : r.pos[2];
+    left = run == 0 ? r.len[0] : run == 1 ? r.len[1] : r.len[2];
+    x.n = min(left, WT_KT);
+  }
+  __device__ __forceinline__ explicit WtIter(const WaRuns& r) : run(0) { enter(r); }
+  __device__ __forceinline__ void next(const WaRuns& r) {
+    x.row += WT_KT;
+    x.pos += WT_KT;
+    left -= WT_KT;
+    x.n = min(left, WT_KT);
+    if (left <= 0) {
+      run++;
+      enter(r);
+    }
+  }
+};
+
+// Place in a ring of N slots: the slot and how often it has been used before.
+template <int N>
+struct WtSlot {
+  int s = 0;
+  uint32_t turn = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == N) {
+      s = 0;
+      turn++;
+    }
+  }
+};
+
+// The parts of an operand descriptor that a kernel's tiles share, and the
+// descriptor at an address.
+constexpr uint32_t WT_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);  // 8-row groups 1024 B apart, 128-B swizzle
+__device__ __forceinline__ uint64_t wt_desc(uint32_t lo) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(WT_DESC_HI));
+  return d;
+}
+__device__ __forceinline__ uint32_t wt_desc_lo(uint32_t saddr, uint32_t lead) {
+  return ((saddr >> 4) & 0x3FFFu) | (lead >> 4) << 16;
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(WT_THREADS, 1)
     k_wa_tc(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
@@ -186,9 +253,11 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   uint64_t* sfull = empty + L::SLOTS;  // [2] S of query tile h written
   uint64_t* pready = sfull + 2;        // [2] P of query tile h in place
   uint64_t* pvdone = pready + 2;       // [2] P V of query tile h added
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(pvdone + 2);
+  uint64_t* vclean = pvdone + 2;       // [3] rows behind a short tile of V zeroed (a run has one at most)
+  uint64_t* vgo = vclean + 3;          // [3] that tile has landed
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(vgo + 3);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   WtWork w;
   w.sq = wa_seq(p, blockIdx.z);
   const int tokens = WT_ROWS / pack;   // per query tile
@@ -206,6 +275,10 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
 
   if (tid == 0) {
     mbar_init(qfull, 1);
+    for (int i = 0; i < 3; i++) {
+      mbar_init(&vclean[i], 1);
+      mbar_init(&vgo[i], 1);
+    }
     for (int i = 0; i < L::SLOTS; i++) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -221,7 +294,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tslot;  // S 0: columns 0-127, S 1: 128-255, O 0: 256 .., O 1: 384 ..
+  // the whole of tensor memory, so from column 0 on: S 0 in 0-127, S 1 in 128-255, O 0 from 256, O 1 from 384
+  constexpr uint32_t tmem = 0;
 
   if (warp < WT_LOAD) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(WT_REGS_SOFTMAX));
@@ -235,8 +309,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     float m = -INFINITY, l = 0.f;
     int n = 0;
     bool ok = true;
-    for (int t = 0; t < w.nt; t++) {
-      const WaTile x = wa_tile<WT_KT>(w.runs, t);
+    WtIter it(w.runs);
+    for (int t = 0; t < w.nt; t++, it.next(w.runs)) {
+      const WaTile x = it.x;
       if (!w.needs(p, h, x)) continue;
       ok = qg_wait_warp(&sfull[h], (uint32_t)(n & 1), p.err);
       if (!ok) break;
@@ -285,25 +360,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         }
       }
       const float base = m == -INFINITY ? 0.f : m;
-      const uint64_t sl2 = wt_pair(sl, sl), nb2 = wt_pair(-base, -base);
-      uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-      for (int c = 0; c < 128; c += 4) {
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-          float e0, e1;
-          wt_unpair(wt_fma2(wt_pair(__uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1])), sl2, nb2), e0, e1);
-          e0 = wt_exp2(e0);
-          e1 = wt_exp2(e1);
-          sum[k] = wt_add2(sum[k], wt_pair(e0, e1));
-          s[(c >> 1) + k] = wt_pack<T>(e0, e1);
-        }
-      }
-      {
-        float e0, e1;
-        wt_unpair(wt_add2(sum[0], sum[1]), e0, e1);
-        l += e0 + e1;
-      }
+      l += wt_weights<T>(s, sl, base);
       wt_st32(ts, s);
       wt_st32(ts + 32u, s + 32);
       wt_wait_st();
@@ -314,7 +371,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     }
     if (ok && n > 0) ok = qg_wait_warp(&pvdone[h], (uint32_t)((n - 1) & 1), p.err);
     tc_fence_after();
-    const float inv = !ok ? __int_as_float(0x7fc00000) : l == 0.f ? 0.f : 1.0f / l;
+    const bool none = n == 0 || l == 0.f;  // no key seen
+    const float inv = ok ? 1.0f / l : __int_as_float(0x7fc00000);
     T* out = static_cast<T*>(p.out) + (int64_t)(w.sq.q0 + tok) * p.o_token + (int64_t)head * p.o_head;
 #pragma unroll 1
     for (int c = 0; c < HD; c += 32) {
@@ -326,10 +384,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         for (int e = 0; e < 32; e += 8) {
           uint32_t v[4];
 #pragma unroll
-          for (int k = 0; k < 4; k++)  // no key seen: the columns were never written
-            v[k] = ok && (n == 0 || l == 0.f) ? 0u
-                                              : wt_pack<T>(__uint_as_float(o[e + 2 * k]) * inv,
-                                                           __uint_as_float(o[e + 2 * k + 1]) * inv);
+          for (int k = 0; k < 4; k++)
+            v[k] = ok && none ? 0u
+                              : wt_pack<T>(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
           *reinterpret_cast<uint4*>(out + c + e) = make_uint4(v[0], v[1], v[2], v[3]);
         }
       }
@@ -342,17 +399,20 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         for (int h = 0; h < 2; h++)
           for (int kb = 0; kb < HD / 64; kb++)
             wt_tma3(qs + h * L::TILE + kb * 16384, &mq, 64 * kb, w.vh * pack, w.sq.q0 + w.i0 + h * tokens, qfull);
+        WtIter it(w.runs);
+        WtSlot<L::SLOTS> slot;
         int issued = 0;
         bool ok = true;
-        for (int j = 0; j < 2 * w.nt && ok; j++) {
-          const int s = j % L::SLOTS;
-          if (j >= L::SLOTS) ok = qg_wait(&empty[s], (uint32_t)((j / L::SLOTS - 1) & 1), p.err);
+        for (int j = 0; j < 2 * w.nt; j++) {
+          if (slot.turn) ok = qg_wait(&empty[slot.s], (slot.turn - 1) & 1, p.err);
           if (!ok) break;
-          const WaTile x = wa_tile<WT_KT>(w.runs, j >> 1);
-          mbar_arrive_tx(&full[s], L::TILE);
+          mbar_arrive_tx(&full[slot.s], L::TILE);
           for (int kb = 0; kb < HD / 64; kb++)
-            wt_tma4(ring + s * L::TILE + kb * 16384, (j & 1) ? &mv : &mk, 64 * kb, x.row, w.kvh, w.sq.slot, &full[s]);
+            wt_tma4(ring + slot.s * L::TILE + kb * 16384, (j & 1) ? &mv : &mk, 64 * kb, it.x.row, w.kvh, w.sq.slot,
+                    &full[slot.s]);
+          slot.next();
           issued = j + 1;
+          if (j & 1) it.next(w.runs);
         }
         // every requested box has landed before the CTA may end
         qg_wait(qfull, 0, p.err);
@@ -360,24 +420,28 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
           qg_wait(&full[j % L::SLOTS], (uint32_t)((j / L::SLOTS) & 1), p.err);
       }
     } else if (warp == WT_MMA) {
-      constexpr uint32_t TY = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      // The whole warp walks the loop, so that the operands' descriptors stay in
+      // uniform registers; one elected lane issues.
+      constexpr uint32_t TY = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       constexpr uint32_t BASE = (1u << 4) | (TY << 7) | (TY << 10) | ((uint32_t)(WT_ROWS >> 4) << 24);
-      int done[2] = {0, 0};  // products P V issued per query tile
+      constexpr uint32_t PV = BASE | (1u << 16) | ((uint32_t)(HD >> 3) << 17);  // B transposed
+      const uint32_t qlo = wt_desc_lo(smem_u32(qs), 16), rlo = wt_desc_lo(smem_u32(ring), 16);
+      uint32_t done[2] = {0u, 0u};  // products P V issued per query tile
       bool ok = qg_wait_warp(qfull, 0, p.err);
       auto qk = [&](int h, const WaTile& x, int s) {
         if (!ok || !w.needs(p, h, x)) return;
-        const int n = h ? done[1] : done[0];
+        const uint32_t n = h ? done[1] : done[0];
         // its columns held P of the tile before
-        if (n > 0) ok = qg_wait_warp(&pvdone[h], (uint32_t)((n - 1) & 1), p.err);
+        if (n > 0) ok = qg_wait_warp(&pvdone[h], (n - 1) & 1, p.err);
         if (!ok) return;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t qa = smem_u32(qs + h * L::TILE), ka = smem_u32(ring + s * L::TILE);
-          const uint32_t idesc = BASE | ((uint32_t)((x.n + 15) >> 4) << 18);  // N = the tile's keys, in steps of 16
-  #pragma unroll
+        const uint32_t idesc = BASE | ((uint32_t)((x.n + 15) >> 4) << 18);  // N: the tile's keys, in steps of 16
+        const uint32_t qa = qlo + (uint32_t)h * (L::TILE >> 4), ka = rlo + (uint32_t)s * (L::TILE >> 4);
+        if (wt_elect()) {
+#pragma unroll
           for (int kk = 0; kk < HD / 16; kk++) {
-            const uint32_t off = (uint32_t)(kk >> 2) * 16384u + 32u * (uint32_t)(kk & 3);
-            tc_mma_ss(tmem + 128u * (uint32_t)h, qg_smem_desc(qa + off), qg_smem_desc(ka + off), idesc, kk > 0);
+            const uint32_t off = (uint32_t)(kk >> 2) * 1024u + 2u * (uint32_t)(kk & 3);
+            tc_mma_ss(tmem + 128u * (uint32_t)h, wt_desc(qa + off), wt_desc(ka + off), idesc, kk > 0);
           }
           qg_commit(&sfull[h]);
         }
@@ -385,64 +449,85 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       };
       auto pv = [&](int h, const WaTile& x, int s) {
         if (!ok || !w.needs(p, h, x)) return;
-        const int n = h ? done[1] : done[0];
-        ok = qg_wait_warp(&pready[h], (uint32_t)(n & 1), p.err);
+        const uint32_t n = h ? done[1] : done[0];
+        ok = qg_wait_warp(&pready[h], n & 1, p.err);
         if (!ok) return;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t va = smem_u32(ring + s * L::TILE), o = tmem + 256u + 128u * (uint32_t)h;
-          const uint32_t idesc = BASE | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
-          const int steps = (x.n + 15) >> 4;
-          for (int kk = 0; kk < steps; kk++)
-            qg_mma_ts(o, tmem + 128u * (uint32_t)h + 8u * (uint32_t)kk, wt_desc_n(va + 2048u * (uint32_t)kk, 16384u),
-                      idesc, (n > 0 || kk > 0) ? 1u : 0u);
+        // 64-wide blocks of the row 16 KB apart
+        const uint32_t va = rlo + (uint32_t)s * (L::TILE >> 4) + ((16384u - 16u) >> 4 << 16);
+        const uint32_t o = tmem + 256u + 128u * (uint32_t)h, pa = tmem + 128u * (uint32_t)h;
+        if (wt_elect()) {
+          if (x.n > WT_KT - 16) {
+#pragma unroll
+            for (int kk = 0; kk < WT_KT / 16; kk++)
+              qg_mma_ts(o, pa + 8u * kk, wt_desc(va + 128u * kk), PV, kk > 0 ? 1u : n > 0);
+          } else {
+            for (int kk = 0; 16 * kk < x.n; kk++)
+              qg_mma_ts(o, pa + 8u * kk, wt_desc(va + 128u * kk), PV, kk > 0 ? 1u : n > 0);
+          }
           qg_commit(&pvdone[h]);
         }
         __syncwarp();
-        if (h) done[1]++; else done[0]++;
+        if (h) done[1] = n + 1; else done[0] = n + 1;
       };
-      auto arrived = [&](int j) {  // operand tile j of the ring
-        if (ok) ok = qg_wait_warp(&full[j % L::SLOTS], (uint32_t)((j / L::SLOTS) & 1), p.err);
-        if (ok) tc_fence_after();
-      };
-      auto release = [&](int j) {
-        if (ok && lane == 0) qg_commit(&empty[j % L::SLOTS]);
+      auto release = [&](int s) {
+        if (ok && wt_elect()) qg_commit(&empty[s]);
         __syncwarp();
       };
-      WaTile x = wa_tile<WT_KT>(w.runs, 0);
+      WtIter it(w.runs);
+      WtSlot<L::SLOTS> slot;
+      uint32_t cleaned = 0;
+      if (w.nt > 0 && ok) ok = qg_wait_warp(&full[0], 0, p.err);
       if (w.nt > 0) {
-        arrived(0);
-        qk(0, x, 0);
-        qk(1, x, 0);
+        qk(0, it.x, 0);
+        qk(1, it.x, 0);
         release(0);
       }
       for (int t = 0; t < w.nt && ok; t++) {
-        const int vs = (2 * t + 1) % L::SLOTS, ks = (2 * t + 2) % L::SLOTS;
-        const bool more = t + 1 < w.nt;
-        const WaTile y = wa_tile<WT_KT>(w.runs, more ? t + 1 : t);
-        arrived(2 * t + 1);
+        const WaTile x = it.x;
+        slot.next();
+        const WtSlot<L::SLOTS> v = slot;
+        slot.next();
+        it.next(w.runs);
+        ok = qg_wait_warp(&full[v.s], v.turn & 1, p.err);
         if (ok && (x.n & 15)) {
-          // the last product of 16 keys also reads rows behind the tile's: zero
-          // them (their weights are zero, but the rows may hold anything)
-          const int r0 = x.n, rows = 16 - (x.n & 15);
+          if (lane == 0) mbar_arrive1(&vgo[cleaned]);
+          ok = qg_wait_warp(&vclean[cleaned++], 0, p.err);
+        }
+        pv(0, x, v.s);
+        const bool more = t + 1 < w.nt;
+        if (more && ok) {
+          ok = qg_wait_warp(&full[slot.s], slot.turn & 1, p.err);
+          qk(0, it.x, slot.s);
+        }
+        pv(1, x, v.s);
+        release(v.s);
+        if (more) {
+          qk(1, it.x, slot.s);
+          release(slot.s);
+        }
+      }
+    } else if (warp == WT_CLEAN) {
+      // the last product of 16 keys of a short tile also reads rows behind the
+      // tile's: zero them (their weights are zero, but the rows may hold anything)
+      WtIter it(w.runs);
+      WtSlot<L::SLOTS> slot;
+      int cleaned = 0;
+      for (int t = 0; t < w.nt; t++) {
+        slot.next();
+        if (it.x.n & 15) {
+          if (!qg_wait_warp(&vgo[cleaned], 0, p.err)) break;
+          const int rows = 16 - (it.x.n & 15);
           for (int e = lane; e < rows * (HD / 8); e += 32)
-            *reinterpret_cast<uint4*>(ring + vs * L::TILE + (e & 7) * 16 + (r0 + (e >> 3) % rows) * 128 +
+            *reinterpret_cast<uint4*>(ring + slot.s * L::TILE + (e & 7) * 16 + (it.x.n + (e >> 3) % rows) * 128 +
                                       ((e >> 3) / rows) * 16384) = make_uint4(0u, 0u, 0u, 0u);
           fence_async_smem();
           __syncwarp();
+          if (lane == 0) mbar_arrive1(&vclean[cleaned]);
+          cleaned++;
         }
-        pv(0, x, vs);
-        if (more) {
-          arrived(2 * t + 2);
-          qk(0, y, ks);
-        }
-        pv(1, x, vs);
-        release(2 * t + 1);
-        if (more) {
-          qk(1, y, ks);
-          release(2 * t + 2);
-        }
-        x = y;
+        slot.next();
+        it.next(w.runs);
       }
     }
   }
