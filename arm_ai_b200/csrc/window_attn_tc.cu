@@ -39,8 +39,8 @@ constexpr int WT_ROWS = 128;                   // query rows per tile, two tiles
 constexpr int WT_LOAD = 8, WT_MMA = 9, WT_CLEAN = 10;  // warps 0-3, 4-7: softmax of tile 0, 1
 constexpr int WT_THREADS = 384;                // warp 11 only completes the warp group
 // Registers: 384 x 168 at launch; the loading group gives up what the softmax
-// threads (128 scores each) need: 256 x 216 + 128 x 72 = 384 x 168.
-constexpr int WT_REGS = 168, WT_REGS_SOFTMAX = 216, WT_REGS_LOAD = 72;
+// threads (128 scores each) need: 256 x 208 + 128 x 88 = 384 x 168.
+constexpr int WT_REGS = 168, WT_REGS_SOFTMAX = 208, WT_REGS_LOAD = 88;
 static_assert(256 * WT_REGS_SOFTMAX + 128 * WT_REGS_LOAD <= WT_THREADS * WT_REGS, "register split");
 constexpr float WT_SLACK = 8.f;
 
@@ -130,24 +130,21 @@ __device__ __forceinline__ uint32_t wt_pack<__nv_bfloat16>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The row's weights exp2(scale s - base) over its scores, as pairs of T in
-// s[0 .. 63]; returns their f32 sum (of the unrounded values).
+// The weights exp2(scale s - base) of 64 scores s[0 .. 63], as pairs of T in
+// w[0 .. 31]; adds them (unrounded) to the two f32 pairs of sum. w may be the
+// start of s or lie before it.
 template <typename T>
-__device__ __forceinline__ float wt_weights(uint32_t (&s)[128], float sl, float base) {
-  const uint64_t sl2 = wt_pair(sl, sl), nb2 = wt_pair(-base, -base);
-  uint64_t sum[2] = {0ull, 0ull};
+__device__ __forceinline__ void wt_weights(const uint32_t* s, uint32_t* w, uint64_t sl2, uint64_t nb2,
+                                           uint64_t (&sum)[2]) {
 #pragma unroll
-  for (int c = 0; c < 64; c++) {
+  for (int c = 0; c < 32; c++) {
     float e0, e1;
     wt_unpair(wt_fma2(wt_pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sl2, nb2), e0, e1);
     e0 = wt_exp2(e0);
     e1 = wt_exp2(e1);
     sum[c & 1] = wt_add2(sum[c & 1], wt_pair(e0, e1));
-    s[c] = wt_pack<T>(e0, e1);
+    w[c] = wt_pack<T>(e0, e1);
   }
-  float e0, e1;
-  wt_unpair(wt_add2(sum[0], sum[1]), e0, e1);
-  return e0 + e1;
 }
 
 __device__ __forceinline__ void wt_tma3(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
@@ -177,6 +174,24 @@ struct WtWork {
     return lo <= hi && x.pos <= hi && (lo - (x.pos + x.n - 1) < p.window || x.pos < p.n_sink);
   }
 };
+
+// Waits of a converged warp: one look, and the bounded loop only where that
+// was not enough. After a wait that gave up (ok false) no further one waits,
+// so the role runs to its end.
+__device__ __forceinline__ bool wt_wait_slow(uint64_t* bar, uint32_t parity, bool ok, uint32_t* err) {
+  return ok && qg_wait_warp(bar, parity, err);
+}
+__device__ __forceinline__ void wt_wait(uint64_t* bar, uint32_t parity, bool& ok, uint32_t* err) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  if (!__all_sync(0xffffffffu, done)) ok = wt_wait_slow(bar, parity, ok, err);
+}
 
 // One lane of a converged warp.
 __device__ __forceinline__ bool wt_elect() {
@@ -255,7 +270,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   uint64_t* pvdone = pready + 2;       // [2] P V of query tile h added
   uint64_t* vclean = pvdone + 2;       // [3] rows behind a short tile of V zeroed (a run has one at most)
   uint64_t* vgo = vclean + 3;          // [3] that tile has landed
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(vgo + 3);
+  uint64_t* fin = vgo + 3;             // every product done
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 1);
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   WtWork w;
@@ -275,6 +291,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
 
   if (tid == 0) {
     mbar_init(qfull, 1);
+    mbar_init(fin, 1);
     for (int i = 0; i < 3; i++) {
       mbar_init(&vclean[i], 1);
       mbar_init(&vgo[i], 1);
@@ -313,8 +330,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     for (int t = 0; t < w.nt; t++, it.next(w.runs)) {
       const WaTile x = it.x;
       if (!w.needs(p, h, x)) continue;
-      ok = qg_wait_warp(&sfull[h], (uint32_t)(n & 1), p.err);
-      if (!ok) break;
+      wt_wait(&sfull[h], (uint32_t)(n & 1), ok, p.err);
       tc_fence_after();
       uint32_t s[128];
 #pragma unroll
@@ -345,8 +361,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         m = nm;
         l *= f;
         if (n > 0) {
-          ok = qg_wait_warp(&pvdone[h], (uint32_t)((n - 1) & 1), p.err);
-          if (!ok) break;
+          wt_wait(&pvdone[h], (uint32_t)((n - 1) & 1), ok, p.err);
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
@@ -360,16 +375,23 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         }
       }
       const float base = m == -INFINITY ? 0.f : m;
-      l += wt_weights<T>(s, sl, base);
-      wt_st32(ts, s);
-      wt_st32(ts + 32u, s + 32);
+      const uint64_t sl2 = wt_pair(sl, sl), nb2 = wt_pair(-base, -base);
+      uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        wt_weights<T>(s + 64 * half, s + 32 * half, sl2, nb2, sum);
+        wt_st32(ts + 32u * half, s + 32 * half);
+      }
       wt_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive1(&pready[h]);
+      float s0, s1;
+      wt_unpair(wt_add2(sum[0], sum[1]), s0, s1);
+      l += s0 + s1;
       n++;
     }
-    if (ok && n > 0) ok = qg_wait_warp(&pvdone[h], (uint32_t)((n - 1) & 1), p.err);
+    if (n > 0) wt_wait(&pvdone[h], (uint32_t)((n - 1) & 1), ok, p.err);
     tc_fence_after();
     const bool none = n == 0 || l == 0.f;  // no key seen
     const float inv = ok ? 1.0f / l : __int_as_float(0x7fc00000);
@@ -426,14 +448,17 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       constexpr uint32_t BASE = (1u << 4) | (TY << 7) | (TY << 10) | ((uint32_t)(WT_ROWS >> 4) << 24);
       constexpr uint32_t PV = BASE | (1u << 16) | ((uint32_t)(HD >> 3) << 17);  // B transposed
       const uint32_t qlo = wt_desc_lo(smem_u32(qs), 16), rlo = wt_desc_lo(smem_u32(ring), 16);
-      uint32_t done[2] = {0u, 0u};  // products P V issued per query tile
-      bool ok = qg_wait_warp(qfull, 0, p.err);
+      bool ok = true;
+      wt_wait(qfull, 0, ok, p.err);
+      WtIter it(w.runs);
+      WtSlot<L::SLOTS> slot;
+      uint32_t cleaned = 0;
+      // bit h: query tile h takes part in the key tile; has had a product P V; the parity of their number
+      uint32_t need = 0, begun = 0, par = 0;
+      // S of query tile h with the K tile in slot s
       auto qk = [&](int h, const WaTile& x, int s) {
-        if (!ok || !w.needs(p, h, x)) return;
-        const uint32_t n = h ? done[1] : done[0];
         // its columns held P of the tile before
-        if (n > 0) ok = qg_wait_warp(&pvdone[h], (n - 1) & 1, p.err);
-        if (!ok) return;
+        if (begun >> h & 1) wt_wait(&pvdone[h], (par >> h & 1) ^ 1, ok, p.err);
         tc_fence_after();
         const uint32_t idesc = BASE | ((uint32_t)((x.n + 15) >> 4) << 18);  // N: the tile's keys, in steps of 16
         const uint32_t qa = qlo + (uint32_t)h * (L::TILE >> 4), ka = rlo + (uint32_t)s * (L::TILE >> 4);
@@ -447,66 +472,66 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         }
         __syncwarp();
       };
-      auto pv = [&](int h, const WaTile& x, int s) {
-        if (!ok || !w.needs(p, h, x)) return;
-        const uint32_t n = h ? done[1] : done[0];
-        ok = qg_wait_warp(&pready[h], n & 1, p.err);
-        if (!ok) return;
-        tc_fence_after();
-        // 64-wide blocks of the row 16 KB apart
-        const uint32_t va = rlo + (uint32_t)s * (L::TILE >> 4) + ((16384u - 16u) >> 4 << 16);
-        const uint32_t o = tmem + 256u + 128u * (uint32_t)h, pa = tmem + 128u * (uint32_t)h;
-        if (wt_elect()) {
-          if (x.n > WT_KT - 16) {
-#pragma unroll
-            for (int kk = 0; kk < WT_KT / 16; kk++)
-              qg_mma_ts(o, pa + 8u * kk, wt_desc(va + 128u * kk), PV, kk > 0 ? 1u : n > 0);
-          } else {
-            for (int kk = 0; 16 * kk < x.n; kk++)
-              qg_mma_ts(o, pa + 8u * kk, wt_desc(va + 128u * kk), PV, kk > 0 ? 1u : n > 0);
-          }
-          qg_commit(&pvdone[h]);
-        }
-        __syncwarp();
-        if (h) done[1] = n + 1; else done[0] = n + 1;
-      };
-      auto release = [&](int s) {
-        if (ok && wt_elect()) qg_commit(&empty[s]);
-        __syncwarp();
-      };
-      WtIter it(w.runs);
-      WtSlot<L::SLOTS> slot;
-      uint32_t cleaned = 0;
-      if (w.nt > 0 && ok) ok = qg_wait_warp(&full[0], 0, p.err);
       if (w.nt > 0) {
-        qk(0, it.x, 0);
-        qk(1, it.x, 0);
-        release(0);
+        need = w.needs(p, 0, it.x) | w.needs(p, 1, it.x) << 1;
+        wt_wait(&full[0], 0, ok, p.err);
+#pragma unroll 1
+        for (int h = 0; h < 2; h++)
+          if (need >> h & 1) qk(h, it.x, 0);
+        if (wt_elect()) qg_commit(&empty[0]);
+        __syncwarp();
       }
-      for (int t = 0; t < w.nt && ok; t++) {
+      // Every step of this loop lies on the path between a weight and the next
+      // score, and its code is refetched each time (the softmax's fills the
+      // instruction caches): one copy for both query tiles, few branches.
+#pragma unroll 1
+      for (int t = 0; t < w.nt; t++) {
         const WaTile x = it.x;
         slot.next();
         const WtSlot<L::SLOTS> v = slot;
         slot.next();
         it.next(w.runs);
-        ok = qg_wait_warp(&full[v.s], v.turn & 1, p.err);
-        if (ok && (x.n & 15)) {
-          if (lane == 0) mbar_arrive1(&vgo[cleaned]);
-          ok = qg_wait_warp(&vclean[cleaned++], 0, p.err);
-        }
-        pv(0, x, v.s);
         const bool more = t + 1 < w.nt;
-        if (more && ok) {
-          ok = qg_wait_warp(&full[slot.s], slot.turn & 1, p.err);
-          qk(0, it.x, slot.s);
+        const uint32_t next = more ? w.needs(p, 0, it.x) | w.needs(p, 1, it.x) << 1 : 0;
+        wt_wait(&full[v.s], v.turn & 1, ok, p.err);
+        if (more) wt_wait(&full[slot.s], slot.turn & 1, ok, p.err);
+        if (x.n & 15) {
+          if (lane == 0) mbar_arrive1(&vgo[cleaned]);
+          wt_wait(&vclean[cleaned++], 0, ok, p.err);
         }
-        pv(1, x, v.s);
-        release(v.s);
-        if (more) {
-          qk(1, it.x, slot.s);
-          release(slot.s);
+        // 64-wide blocks of the row 16 KB apart
+        const uint32_t va = rlo + (uint32_t)v.s * (L::TILE >> 4) + ((16384u - 16u) >> 4 << 16);
+#pragma unroll 1
+        for (int h = 0; h < 2; h++) {
+          if (need >> h & 1) {
+            const uint32_t o = tmem + 256u + 128u * (uint32_t)h, pa = tmem + 128u * (uint32_t)h;
+            wt_wait(&pready[h], par >> h & 1, ok, p.err);
+            tc_fence_after();
+            if (wt_elect()) {
+#pragma unroll
+              for (int kk = 0; kk < WT_KT / 16; kk++)
+                if (16 * kk < x.n)
+                  qg_mma_ts(o, pa + 8u * kk, wt_desc(va + 128u * kk), PV, kk > 0 ? 1u : begun >> h & 1);
+              qg_commit(&pvdone[h]);
+            }
+            __syncwarp();
+            begun |= 1u << h;
+            par ^= 1u << h;
+          }
+          if (next >> h & 1) qk(h, it.x, slot.s);
         }
+        if (wt_elect()) {
+          qg_commit(&empty[v.s]);
+          if (more) qg_commit(&empty[slot.s]);
+        }
+        __syncwarp();
+        need = next;
       }
+      // no product is in flight when tensor memory is given back, failed waits or not
+      if (wt_elect()) qg_commit(fin);
+      __syncwarp();
+      ok = true;
+      wt_wait(fin, 0, ok, p.err);
     } else if (warp == WT_CLEAN) {
       // the last product of 16 keys of a short tile also reads rows behind the
       // tile's: zero them (their weights are zero, but the rows may hold anything)
