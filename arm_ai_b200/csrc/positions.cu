@@ -7,22 +7,29 @@
 //   norm (before the rotation): x * 1/sqrt(mean(x^2) + eps) * gamma
 //
 // Bound by memory: every value is read once and written once, with a handful
-// of operations between. A CTA takes the heads of one token: its first
-// threads make the token's cos / sin table in shared memory (one f64
-// reduction and one sincospi per pair, instead of one per pair and head)
-// while the heads' loads are in flight; each head then is a power-of-two
-// group of lanes with one 16-byte vector each, so the norm's sum is a few
-// shuffles and the partner of a half-layout pair one more.
+// of operations between. A warp has one token: it makes the token's cosines
+// and sines once (instead of once per head), and a lane keeps its own, and its
+// gains, in registers for all heads. A power-of-two group of lanes holds a
+// head; a lane has both members of its pairs (two 16-byte vectors), so the
+// rotation needs no exchange and the norm's sum a few shuffles per head.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "dev_call.cuh"
 
 namespace armai {
 namespace {
 
-constexpr int ROT_THREADS = 256;
+constexpr int ROT_THREADS = 128;
 constexpr int ROT_MAX_DIM = 256;
+constexpr int ROT_WARPS = ROT_THREADS / 32;
+// Items in flight per warp, and CTAs per SM: 80 warps' worth of 1 KB items per
+// SM. 16381 tokens of 32 + 8 + 8 heads of 128, bf16: 84.9 us = 4.74 TB/s (6 or 8
+// stages 86; 6 or 8 CTAs 92 to 107; two heads per lane in registers and no ring
+// 132; a table shared by the CTA's tokens 262).
+constexpr int ROT_STAGES = 4;
+constexpr int ROT_CTAS = 5;
 
 struct RotTensor {
   const void* src;
@@ -42,15 +49,21 @@ struct RotParams {
   float eps, mscale;
 };
 
-// cos and sin of pos * f, times m. The product is exact in f64 (24 + 29
-// bits; a position beyond 2^29 rounds it to 2^-53), reduced to half turns
-// there, and only the remainder rounded to f32: 2^-24 of at most one half
-// turn, 2e-7 absolute, at any position.
-__device__ __forceinline__ float2 rot_angle(int64_t pos, float f, float m) {
-  double t = (double)pos * (double)f * 0.15915494309189533577;  // turns
-  t -= rint(t);
+// Turns per position of frequency f, as a 64-bit fraction of a turn. Times a
+// position it wraps modulo one turn by itself (negative positions too), with
+// an error of 2^-53 of the angle and 2^-64 turns per position: the f64 product
+// reduced exactly, without f64 work per position.
+__device__ __forceinline__ uint64_t rot_turns(float f) {
+  double t = (double)f * 0.15915494309189533577;
+  t -= floor(t);
+  return __double2ull_rz(t * 18446744073709551616.0);
+}
+// cos and sin of the angle, times m. The remainder, below half a turn, is
+// rounded to f32: 2e-7 absolute, at any position.
+__device__ __forceinline__ float2 rot_angle(int64_t pos, uint64_t turns, float m) {
+  const int32_t r = (int32_t)(((uint64_t)pos * turns) >> 32);  // signed, in 2^-32 turns
   float s, c;
-  sincospif((float)(2.0 * t), &s, &c);
+  sincospif((float)r * 4.656612873077392578125e-10f, &s, &c);  // half turns: 2^-31
   return make_float2(c * m, s * m);
 }
 
@@ -74,6 +87,11 @@ __device__ __forceinline__ int rot_locate(const RotParams& p, int h, int& head) 
   return i;
 }
 
+__device__ __forceinline__ void rot_copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+
 // Destination row of a token in tensor i, or -1.
 __device__ __forceinline__ int64_t rot_row(const RotParams& p, int i, int64_t token) {
   if (i == 0 || !p.kv_rows) return i == 0 || token < p.n_rows ? token : -1;
@@ -81,92 +99,164 @@ __device__ __forceinline__ int64_t rot_row(const RotParams& p, int i, int64_t to
   return r >= 0 && r < p.n_rows ? r : -1;
 }
 
-// Vector form: head_dim a multiple of the 16-byte vector, every head's start
-// 16-byte aligned, pairs of the half layout a whole number of vectors apart.
-// A group of HL lanes (power of two, at least head_dim / VEC) holds a head;
-// a warp has 32 / HL heads at once and U such passes in flight.
-template <typename T, typename KV, int U>
-__global__ void __launch_bounds__(ROT_THREADS) k_rotate_vec(const RotParams p, int hl, int layout) {
+// Vector form: every head's start and the second vectors 16-byte aligned.
+// Lane l of a head's HL lanes (power of two) has the VEC pairs from l * VEC on:
+//   half layout: the vectors at l * VEC and rot / 2 + l * VEC; the lanes behind
+//   rot / 2 have two vectors each of what is not rotated
+//   interleaved: the two vectors at 2 l * VEC
+// A warp goes through a stream of items, one item being 32 / HL heads of a
+// tensor of one token: all items of the tokens w, w + warps, ... (splits 1), or
+// one item (splits: the items of a token). The stream's loads run ROT_STAGES
+// items ahead, as asynchronous copies into a ring in which a lane reads back
+// only what it copied itself: enough bytes in flight for the memory, whatever
+// the registers hold.
+template <typename T, typename KV, bool IL>
+__global__ void __launch_bounds__(ROT_THREADS) k_rotate_vec(const RotParams p, int hl, int64_t n_tokens, int items,
+                                                            int splits) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  __shared__ float2 cs[ROT_MAX_DIM / 2];
-  const int64_t token = blockIdx.x;
+  __shared__ float2 table[ROT_WARPS][ROT_MAX_DIM / 2];
+  __shared__ uint4 ring_[ROT_WARPS][ROT_STAGES][2][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per_warp = 32 / hl, sub = lane / hl, l = lane % hl, d0 = l * VEC;
-  const int per_pass = per_warp * (ROT_THREADS / 32);
-  const int h0 = blockIdx.y * per_pass * U + warp * per_warp + sub;
-  Vec<T, VEC> raw[U];
-  int which[U], head[U];
-#pragma unroll
-  for (int u = 0; u < U; u++) {
-    const int h = h0 + u * per_pass;
-    which[u] = -1;
-    if (h < p.heads && d0 < p.dim) {
-      which[u] = rot_locate(p, h, head[u]);
-      const RotTensor& t = p.t[which[u]];
-      raw[u] = *reinterpret_cast<const Vec<T, VEC>*>(static_cast<const T*>(t.src) + token * t.src_token +
-                                                     head[u] * t.src_head + d0);
+  const int64_t unit = (int64_t)blockIdx.x * ROT_WARPS + warp;
+  int64_t token = unit / splits;
+  if (token >= n_tokens) return;
+  const int64_t step = (int64_t)gridDim.x * ROT_WARPS;  // tokens between a warp's tokens (splits 1)
+  const int half = p.rot >> 1, hpw = 32 / hl, sub = lane / hl, l = lane % hl, p0 = l * VEC;
+  const int da = IL ? 2 * p0 : p0 < half ? p0 : p.rot + 2 * (p0 - half);
+  const int db = IL || p0 >= half ? da + VEC : p0 + half;
+  const bool mine = 2 * p0 < p.dim;
+  const int n0 = (p.t[0].heads + hpw - 1) / hpw, n1 = (p.t[1].heads + hpw - 1) / hpw;  // items of q, of k
+
+  // the tensor of an item of a token, and this lane's head in it
+  auto place = [&](int g, int& h) {
+    const int i = g < n0 ? 0 : g < n0 + n1 ? 1 : 2;
+    h = (g - (i == 0 ? 0 : i == 1 ? n0 : n0 + n1)) * hpw + sub;
+    return i;
+  };
+  uint4(*ring)[2][32] = ring_[warp];
+  int64_t ahead = token;  // the loads' place in the stream
+  int ahead_g = splits > 1 ? (int)(unit % splits) : 0, put = 0;
+  const int end_g = splits > 1 ? ahead_g + 1 : items;
+  auto load = [&]() {
+    if (ahead < n_tokens) {
+      int h;
+      const RotTensor& t = p.t[place(ahead_g, h)];
+      if (mine && h < t.heads) {
+        const T* src = static_cast<const T*>(t.src) + ahead * t.src_token + h * t.src_head;
+        rot_copy16(&ring[put][0][lane], src + da);
+        rot_copy16(&ring[put][1][lane], src + db);
+      }
+      if (++ahead_g == end_g) {
+        ahead_g = 0;
+        ahead = splits > 1 ? n_tokens : ahead + step;
+      }
     }
-  }
-  const int half = p.rot >> 1;
-  if ((int)threadIdx.x < half) cs[threadIdx.x] = rot_angle(p.positions[token], p.inv_freq[threadIdx.x], p.mscale);
-  __syncthreads();
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    put = put + 1 == ROT_STAGES ? 0 : put + 1;
+  };
+  int g = ahead_g, get = 0;
 #pragma unroll
-  for (int u = 0; u < U; u++) {
-    float x[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; e++) x[e] = which[u] >= 0 ? to_f32(raw[u].v[e]) : 0.f;
-    const float* gamma = which[u] >= 0 ? p.t[which[u]].gamma : nullptr;
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < VEC; e++) ss += x[e] * x[e];
-    for (int o = hl >> 1; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (gamma) {
-      const float inv = 1.0f / sqrtf(ss / (float)p.dim + p.eps);
-#pragma unroll
-      for (int e = 0; e < VEC; e++) x[e] = x[e] * inv * gamma[d0 + e];
+  for (int i = 0; i < ROT_STAGES; i++) load();
+
+  float2* cs = table[warp];
+  float c[VEC], s[VEC], ga[VEC], gb[VEC];
+  for (; token < n_tokens; token = splits > 1 ? n_tokens : token + step, g = 0) {
+    __syncwarp();
+    if (half) {
+      const int64_t pos = p.positions[token];
+      for (int i = lane; i < half; i += 32) cs[i] = rot_angle(pos, rot_turns(p.inv_freq[i]), p.mscale);
     }
-    if (layout == ARMAI_ROPE_INTERLEAVED) {
-      if (which[u] < 2) {
+    __syncwarp();
 #pragma unroll
-        for (int e = 0; e < VEC; e += 2) {
-          if (d0 + e < p.rot) {
-            const float2 c = cs[(d0 + e) >> 1];
-            const float a = x[e], b = x[e + 1];
-            x[e] = a * c.x - b * c.y;
-            x[e + 1] = a * c.y + b * c.x;
+    for (int e = 0; e < VEC; e++) {
+      const float2 v = p0 + e < half ? cs[p0 + e] : make_float2(1.f, 0.f);
+      c[e] = v.x;
+      s[e] = v.y;
+    }
+    int64_t row = token;
+    int have = -1;  // the tensor whose gains and row these are
+    for (; g < end_g; g++) {
+      int h;
+      const int i = place(g, h);
+      const RotTensor& t = p.t[i];
+      if (i != have) {
+        if (t.gamma && mine) {
+#pragma unroll
+          for (int e = 0; e < VEC; e += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(t.gamma + (IL ? da + 2 * e : da + e));
+            const float4 y = *reinterpret_cast<const float4*>(t.gamma + (IL ? da + 2 * e + 4 : db + e));
+            if (IL) {
+              ga[e] = x.x, gb[e] = x.y, ga[e + 1] = x.z, gb[e + 1] = x.w;
+              ga[e + 2] = y.x, gb[e + 2] = y.y, ga[e + 3] = y.z, gb[e + 3] = y.w;
+            } else {
+              ga[e] = x.x, ga[e + 1] = x.y, ga[e + 2] = x.z, ga[e + 3] = x.w;
+              gb[e] = y.x, gb[e + 1] = y.y, gb[e + 2] = y.z, gb[e + 3] = y.w;
+            }
+          }
+        }
+        row = rot_row(p, i, token);
+        have = i;
+      }
+      const bool on = mine && h < t.heads;
+      asm volatile("cp.async.wait_group %0;" ::"n"(ROT_STAGES - 1) : "memory");
+      const Vec<T, VEC> ra = *reinterpret_cast<const Vec<T, VEC>*>(&ring[get][0][lane]);
+      const Vec<T, VEC> rb = *reinterpret_cast<const Vec<T, VEC>*>(&ring[get][1][lane]);
+      get = get + 1 == ROT_STAGES ? 0 : get + 1;
+      float a[VEC], b[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        // interleaved: values 2e and 2e + 1 of the 2 VEC
+        a[e] = to_f32(!IL ? ra.v[e] : 2 * e < VEC ? ra.v[(2 * e) % VEC] : rb.v[(2 * e) % VEC]);
+        b[e] = to_f32(!IL ? rb.v[e] : 2 * e < VEC ? ra.v[(2 * e + 1) % VEC] : rb.v[(2 * e + 1) % VEC]);
+      }
+      load();  // this lane has read what the slot held
+      if (t.gamma) {
+        float ss = 0.f;
+        if (on) {
+#pragma unroll
+          for (int e = 0; e < VEC; e++) ss += a[e] * a[e] + b[e] * b[e];
+        }
+        for (int o = hl >> 1; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = 1.0f / sqrtf(ss / (float)p.dim + p.eps);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          a[e] *= inv * ga[e];
+          b[e] *= inv * gb[e];
+        }
+      }
+      if (i < 2) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          if (p0 + e < half) {
+            const float x = a[e], y = b[e];
+            a[e] = x * c[e] - y * s[e];
+            b[e] = x * s[e] + y * c[e];
           }
         }
       }
-    } else {
-      // the partner vector: half / VEC lanes up (first half) or down
-      const bool low = d0 < half;
-      const int other = d0 < p.rot ? lane + (low ? half : -half) / VEC : lane;
+      if (!on || row < 0) continue;
+      const int64_t off = row * t.dst_token + h * t.dst_head;
+      auto store = [&](auto* base) {
+        using O = std::remove_reference_t<decltype(*base)>;
+        Vec<O, VEC> oa, ob;
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
-        const float y = __shfl_sync(0xffffffffu, x[e], other);
-        if (which[u] < 2 && d0 < p.rot) {
-          const float2 c = cs[low ? d0 + e : d0 + e - half];
-          x[e] = low ? x[e] * c.x - y * c.y : y * c.y + x[e] * c.x;
+        for (int e = 0; e < VEC; e++) {
+          if (IL) {
+            Vec<O, VEC>& o = 2 * e < VEC ? oa : ob;
+            o.v[(2 * e) % VEC] = from_f32<O>(a[e]);
+            o.v[(2 * e + 1) % VEC] = from_f32<O>(b[e]);
+          } else {
+            oa.v[e] = from_f32<O>(a[e]);
+            ob.v[e] = from_f32<O>(b[e]);
+          }
         }
-      }
-    }
-    if (which[u] < 0) continue;
-    const RotTensor& t = p.t[which[u]];
-    const int64_t row = rot_row(p, which[u], token);
-    if (row < 0) continue;
-    const int64_t off = row * t.dst_token + head[u] * t.dst_head + d0;
-    if (which[u] == 0) {
-      Vec<T, VEC> o;
-#pragma unroll
-      for (int e = 0; e < VEC; e++) o.v[e] = from_f32<T>(x[e]);
-      *reinterpret_cast<Vec<T, VEC>*>(static_cast<T*>(t.dst) + off) = o;
-    } else {
-      Vec<KV, VEC> o;
-#pragma unroll
-      for (int e = 0; e < VEC; e++) o.v[e] = from_f32<KV>(x[e]);
-      *reinterpret_cast<Vec<KV, VEC>*>(static_cast<KV*>(t.dst) + off) = o;
+        *reinterpret_cast<Vec<O, VEC>*>(base + off + da) = oa;
+        *reinterpret_cast<Vec<O, VEC>*>(base + off + db) = ob;
+      };
+      if (i == 0) store(static_cast<T*>(t.dst)); else store(static_cast<KV*>(t.dst));
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Any head_dim, alignment and pairing: a warp per head, one value per lane
@@ -178,7 +268,8 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotate_any(const RotParams p, i
   const int64_t token = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int half = p.rot >> 1;
-  if ((int)threadIdx.x < half) cs[threadIdx.x] = rot_angle(p.positions[token], p.inv_freq[threadIdx.x], p.mscale);
+  for (int i = threadIdx.x; i < half; i += ROT_THREADS)
+    cs[i] = rot_angle(p.positions[token], rot_turns(p.inv_freq[i]), p.mscale);
   __syncthreads();
   for (int h = blockIdx.y * (ROT_THREADS / 32) + warp; h < p.heads; h += gridDim.y * (ROT_THREADS / 32)) {
     int head;
@@ -226,7 +317,8 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotate_any(const RotParams p, i
 
 bool aligned16(const RotTensor& t, int es, int des) {
   if (!t.heads) return true;
-  return reinterpret_cast<uintptr_t>(t.src) % 16 == 0 && (t.src_token * es) % 16 == 0 && (t.src_head * es) % 16 == 0 &&
+  return reinterpret_cast<uintptr_t>(t.gamma) % 16 == 0 &&
+         reinterpret_cast<uintptr_t>(t.src) % 16 == 0 && (t.src_token * es) % 16 == 0 && (t.src_head * es) % 16 == 0 &&
          // a destination vector is 16 bytes of the source type, so 8 where the cache is narrower
          reinterpret_cast<uintptr_t>(t.dst) % (16 * des / es) == 0 && (t.dst_token * des) % (16 * des / es) == 0 &&
          (t.dst_head * des) % (16 * des / es) == 0;
@@ -235,28 +327,31 @@ bool aligned16(const RotTensor& t, int es, int des) {
 template <typename T, typename KV>
 int rotate_launch(const RotParams& p, int64_t n_tokens, int layout, cudaStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  bool vec = p.dim % VEC == 0 && p.dim / VEC <= 32 &&
-             (layout == ARMAI_ROPE_INTERLEAVED || (p.rot >> 1) % VEC == 0);
+  const int half = p.rot >> 1;
+  bool vec = p.dim % (2 * VEC) == 0 &&
+             (layout == ARMAI_ROPE_INTERLEAVED || (half % VEC == 0 && (p.dim - p.rot) % (2 * VEC) == 0));
   for (int i = 0; i < 3; i++) vec = vec && aligned16(p.t[i], sizeof(T), i ? sizeof(KV) : sizeof(T));
   if (!vec) {
-    const dim3 grid((unsigned)n_tokens, (unsigned)std::min<int64_t>((p.heads + 7) / 8, n_tokens < 64 ? 64 : 1));
+    const dim3 grid((unsigned)n_tokens, (unsigned)std::min<int64_t>((p.heads + 3) / 4, n_tokens < 64 ? 64 : 1));
     k_rotate_any<T, KV><<<grid, ROT_THREADS, 0, s>>>(p, layout);
     ARMAI_CUDA(cudaGetLastError());
     return ARMAI_OK;
   }
   int hl = 1;
-  while (hl < p.dim / VEC) hl <<= 1;
-  const int per_pass = (32 / hl) * (ROT_THREADS / 32);
-  const int passes = (p.heads + per_pass - 1) / per_pass;
-  // Few tokens: one pass per CTA, the heads spread over the SMs (latency).
-  // Many: four passes per CTA, so that four loads per thread are in flight
-  // and the token's angles are made once.
-  if (n_tokens * passes <= 8 * (int64_t)sm_count()) {
-    k_rotate_vec<T, KV, 1><<<dim3((unsigned)n_tokens, (unsigned)passes), ROT_THREADS, 0, s>>>(p, hl, layout);
-  } else {
-    k_rotate_vec<T, KV, 4><<<dim3((unsigned)n_tokens, (unsigned)((passes + 3) / 4)), ROT_THREADS, 0, s>>>(p, hl,
-                                                                                                       layout);
-  }
+  while (hl * 2 * VEC < p.dim) hl <<= 1;
+  const int hpw = 32 / hl;
+  int64_t items = 0;
+  for (int i = 0; i < 3; i++) items += (p.t[i].heads + hpw - 1) / hpw;
+  // Few tokens: every item has a warp of its own (latency). Many: the warps
+  // that fit the device at once share the tokens.
+  const bool few = n_tokens * items <= 16 * (int64_t)sm_count();
+  const int splits = few ? (int)items : 1;
+  const int64_t ctas = std::min<int64_t>((n_tokens * splits + ROT_WARPS - 1) / ROT_WARPS,
+                                         few ? INT32_MAX : ROT_CTAS * (int64_t)sm_count());
+  if (layout == ARMAI_ROPE_INTERLEAVED)
+    k_rotate_vec<T, KV, true><<<(unsigned)ctas, ROT_THREADS, 0, s>>>(p, hl, n_tokens, (int)items, splits);
+  else
+    k_rotate_vec<T, KV, false><<<(unsigned)ctas, ROT_THREADS, 0, s>>>(p, hl, n_tokens, (int)items, splits);
   ARMAI_CUDA(cudaGetLastError());
   return ARMAI_OK;
 }
