@@ -5,11 +5,10 @@
 // Bound by the bytes of the visible keys and values. A warp takes tiles of 16
 // keys in turn with the cluster's other warps and keeps its own running
 // maximum, sum and output, so no warp waits for another until the end. Its
-// tiles arrive by asynchronous 16-byte copies into a three-deep ring in which
-// every lane reads back only what it copied itself (no barrier, no bank
-// conflict): the order of the values within a row is free in both products, as
-// long as q and k (or p and v) agree, so each lane copies the 16-byte chunks
-// that hold its own operands.
+// tiles arrive by asynchronous 16-byte copies, whole lines at a time, into a
+// two-deep ring of its own. The order of the values within a row is free in
+// both products, as long as q and k (or p and v) agree, so each lane's operands
+// are whole 16-byte chunks.
 //   16-bit types: m16n8k16 tensor instructions, 16 rows = (token, query head)
 //   pairs of one key / value head, so a key is read once for all of them.
 //   f32: products on the CUDA cores, 8 lanes per key.
@@ -28,16 +27,18 @@ namespace armai {
 namespace {
 
 constexpr int SP_WARPS = 4, SP_THREADS = 32 * SP_WARPS;
-constexpr int SP_STAGES = 3;
+constexpr int SP_STAGES = 2;
 constexpr int SP_MAX_SPLIT = 16;
 // The running maximum is raised (and the output rescaled) only when a score
 // exceeds it by more than this many powers of two: the weights stay below 2^8
 // and their sum far inside f32, and most tiles need no exchange between lanes.
 constexpr float SP_SLACK = 8.f;
 
-__device__ __forceinline__ void cp16(void* dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0)
-               : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -98,6 +99,34 @@ __device__ __forceinline__ bool sp_block(const WaParams& p, SpBlock& b) {
   b.runs = wa_runs(p, b.sq.pos0 + b.f0 / p.group, b.sq.pos0 + (b.f0 + b.nr - 1) / p.group);
   return true;
 }
+
+// A warp's tiles, every step-th of KT keys through the runs.
+template <int KT>
+struct SpCursor {
+  int run, off, row, pos, len;  // the run, the tile's place in it, and the run's own
+  __device__ __forceinline__ void enter(const WaRuns& r) {
+    row = run == 0 ? r.row[0] : run == 1 ? r.row[1] : r.row[2];
+    pos = run == 0 ? r.pos[0] : run == 1 ? r.pos[1] : r.pos[2];
+    len = run == 0 ? r.len[0] : run == 1 ? r.len[1] : r.len[2];
+  }
+  __device__ __forceinline__ SpCursor(const WaRuns& r, int tile) : run(0) {
+    enter(r);
+    off = 0;
+    advance(r, tile);
+  }
+  __device__ __forceinline__ void advance(const WaRuns& r, int tiles) {
+    off += tiles * KT;
+    while (off >= len && run < 3) {  // into the next run: its tiles start where this one's ended
+      off -= (len + KT - 1) / KT * KT;
+      run++;
+      if (run < 3) enter(r);
+    }
+  }
+  __device__ __forceinline__ bool valid() const { return run < 3; }
+  __device__ __forceinline__ int first_row() const { return row + off; }
+  __device__ __forceinline__ int first_pos() const { return pos + off; }
+  __device__ __forceinline__ int keys() const { return min(KT, len - off); }
+};
 
 // Joins the warps' parts ([warp][R] maxima and sums, [warp][R][DT] outputs in
 // shared memory, outputs unnormalised) within the CTA, then over the cluster,
@@ -188,6 +217,11 @@ __device__ __forceinline__ void sp_join(const WaParams& p, const SpBlock& b, flo
 // ---------------------------------------------------------------------------
 constexpr int SP_ROWS = 16, SP_KT = 16;
 
+// The eight lanes of one shared-memory access read, of K, four chunks of two
+// consecutive keys; of V, two chunks of four keys two apart.
+__device__ __forceinline__ int sp_swz_k(int key) { return (key & 1) << 2; }
+__device__ __forceinline__ int sp_swz_v(int key) { return key & 6; }
+
 template <typename T, int DT>
 constexpr size_t sp_smem() {
   const size_t ring = (size_t)SP_WARPS * SP_STAGES * 2 * SP_KT * DT * 2;
@@ -198,52 +232,63 @@ constexpr size_t sp_smem() {
 template <typename T, int DT>
 __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
   constexpr int KC = DT / 32, VB = DT / 64;       // k chunks per key and lane; 64-wide blocks of v
-  constexpr int CH = 2 * KC + 4 * VB;             // 16-byte chunks per lane and stage
+  constexpr uint32_t TILE = SP_KT * DT * 2;       // a tile of K or V
   extern __shared__ __align__(16) uint8_t sm[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   SpBlock b;
   if (!sp_block<SP_ROWS>(p, b)) return;
   const int chunks = p.head_dim >> 3;             // valid 16-byte chunks of a row
+  const bool whole = p.head_dim == DT;
+  // copies: 16-byte chunk cc of key ck + RPC i, consecutive lanes consecutive
+  // chunks (requests of whole lines: half lines cost a third of the bandwidth);
+  // chunk x of a row lies at x ^ swizzle of the key, so that the reads below
+  // are free of bank conflicts
+  constexpr int RC = DT / 8, RPC = 32 / RC;       // chunks per row, rows per copy instruction
+  const int ck = lane / RC, cc = lane % RC;
   const int64_t kv_off = (int64_t)b.sq.slot * p.kv_slot + (int64_t)b.kvh * p.kv_head;
-  const T* kb = static_cast<const T*>(p.k) + kv_off;
-  const T* vb = static_cast<const T*>(p.v) + kv_off;
-  uint4* ring = reinterpret_cast<uint4*>(sm) + warp * (SP_STAGES * CH * 32) + lane;
+  const int64_t row = p.kv_row, tile_stride = (int64_t)gridDim.x * SP_WARPS * SP_KT * row;
+  const T* kb = static_cast<const T*>(p.k) + kv_off + ck * row + 8 * cc;
+  const T* vb = static_cast<const T*>(p.v) + kv_off + ck * row + 8 * cc;
+  const uint8_t* ring = sm + warp * (SP_STAGES * 2 * TILE);
+  const uint32_t ring32 = smem_u32(ring);
   const int step = (int)gridDim.x * SP_WARPS, first = (int)blockIdx.x * SP_WARPS + warp;
-  const int nt = wa_tiles<SP_KT>(b.runs);
 
-  auto load = [&](int t, int slot) {
-    if (t < nt) {
-      const WaTile x = wa_tile<SP_KT>(b.runs, t);
-      uint4* dst = ring + slot * CH * 32;
+  SpCursor<SP_KT> cur(b.runs, first), ahead = cur;
+  int64_t at = (int64_t)ahead.first_row() * row;  // of the loads' tile, in values from kb and vb
+  auto load = [&](uint32_t dst) {
+    if (ahead.valid()) {
+      const int n = ahead.keys();
+      const T* k = kb + at;
+      const T* v = vb + at;
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const int key = g + 8 * j;
-        const T* src = kb + (int64_t)(x.row + (key < x.n ? key : 0)) * p.kv_row;
-#pragma unroll
-        for (int i = 0; i < KC; i++) {
-          const bool ok = key < x.n && c + 4 * i < chunks;
-          cp16(dst + (j * KC + i) * 32, src + (ok ? 8 * (c + 4 * i) : 0), ok);
+      for (int i = 0; i < SP_KT / RPC; i++) {
+        const int key = ck + RPC * i;
+        const uint32_t dk = dst + key * (RC * 16) + ((cc ^ sp_swz_k(key)) << 4);
+        const uint32_t dv = dst + TILE + key * (RC * 16) + ((cc ^ sp_swz_v(key)) << 4);
+        if (whole && n == SP_KT) {
+          cp16(dk, k + RPC * i * row);
+          cp16(dv, v + RPC * i * row);
+        } else {  // keys behind a short tile's end and chunks behind the head are zero
+          const bool ok = key < n && cc < chunks;
+          cp16_or_zero(dk, ok ? k + RPC * i * row : static_cast<const T*>(p.k), ok);
+          cp16_or_zero(dv, ok ? v + RPC * i * row : static_cast<const T*>(p.v), ok);
         }
       }
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int key = 2 * c + (j & 1) + 8 * (j >> 1);
-        const T* src = vb + (int64_t)(x.row + (key < x.n ? key : 0)) * p.kv_row;
-#pragma unroll
-        for (int i = 0; i < VB; i++) {
-          const bool ok = key < x.n && 8 * i + g < chunks;
-          cp16(dst + (2 * KC + j * VB + i) * 32, src + (ok ? 64 * i + 8 * g : 0), ok);
-        }
-      }
+      const int run = ahead.run;
+      ahead.advance(b.runs, step);
+      at = ahead.run == run ? at + tile_stride : (int64_t)ahead.first_row() * row;
     }
     cp_commit();
   };
 #pragma unroll
-  for (int s = 0; s < SP_STAGES; s++) load(first + s * step, s);
+  for (int s = 0; s < SP_STAGES; s++) load(ring32 + s * 2 * TILE);
 
-  // q rows g and g + 8; rows beyond the block are zero
+  // q rows g and g + 8; rows beyond the block are zero. A negative scale turns
+  // q's signs instead, so that larger products always mean larger scores.
   uint32_t qa[KC][2][4];
   int qpos[2];
+  const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+  const float sl = fabsf(p.scale_log2);
 #pragma unroll
   for (int j = 0; j < 2; j++) {
     const int r = g + 8 * j, f = b.f0 + (r < b.nr ? r : 0);
@@ -254,10 +299,10 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
     for (int i = 0; i < KC; i++) {
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
       if (r < b.nr && c + 4 * i < chunks) v = *reinterpret_cast<const uint4*>(src + 8 * (c + 4 * i));
-      qa[i][0][j] = v.x;
-      qa[i][0][2 + j] = v.y;
-      qa[i][1][j] = v.z;
-      qa[i][1][2 + j] = v.w;
+      qa[i][0][j] = v.x ^ flip;
+      qa[i][0][2 + j] = v.y ^ flip;
+      qa[i][1][j] = v.z ^ flip;
+      qa[i][1][2 + j] = v.w ^ flip;
     }
   }
   const int qmin = b.sq.pos0 + b.f0 / p.group, qmax = b.sq.pos0 + (b.f0 + b.nr - 1) / p.group;
@@ -270,37 +315,49 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
 #pragma unroll
       for (int k = 0; k < 4; k++) o[i][e][k] = 0.f;
 
+  // the lane's operands in a tile: K chunk c + 4 i of keys g and g + 8; V chunk
+  // g + 8 i of keys 2c, 2c + 1, 2c + 8, 2c + 9 (one swizzle for the four)
+  const uint32_t flipped = 64u * (g & 1);  // odd keys: the chunks of even and odd i change places
+  const uint32_t kread[2] = {g * (RC * 16) + 16 * c + flipped, g * (RC * 16) + 16 * c - flipped};
+  const uint32_t vread = TILE + 2 * c * (RC * 16) + ((g ^ sp_swz_v(2 * c)) << 4);
   int slot = 0;
 #pragma unroll 1
-  for (int t = first; t < nt; t += step) {
-    const WaTile x = wa_tile<SP_KT>(b.runs, t);
+  while (cur.valid()) {
+    const uint8_t* src = ring + slot * 2 * TILE;
     cp_wait<SP_STAGES - 1>();
-    const uint4* src = ring + slot * CH * 32;
-    float s[2][4];
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-#pragma unroll
-      for (int k = 0; k < 4; k++) s[j][k] = 0.f;
-#pragma unroll
-      for (int i = 0; i < KC; i++) {
-        const uint4 v = src[(j * KC + i) * 32];
-        mma16816<T>(s[j], qa[i][0], v.x, v.y);
-        mma16816<T>(s[j], qa[i][1], v.z, v.w);
-      }
-    }
-    // s[j][0, 1]: row g, keys 8 j + 2 c, + 1; s[j][2, 3]: row g + 8
-    const bool full = x.n == SP_KT && x.pos + SP_KT - 1 <= qmin &&
-                      (qmax - x.pos < p.window || x.pos + SP_KT - 1 < p.n_sink);
-    float top[2] = {-INFINITY, -INFINITY};
+    __syncwarp();
+    // s[j][0, 1]: row g, keys 8 j + 2 c, + 1; s[j][2, 3]: row g + 8. Two sums
+    // each, for shorter chains.
+    float s[2][4], s2[2][4];
 #pragma unroll
     for (int j = 0; j < 2; j++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        s[j][k] *= p.scale_log2;
-        const int key = 8 * j + 2 * c + (k & 1);
-        if (!full && (key >= x.n || !wa_sees(p, qpos[k >> 1], x.pos + key))) s[j][k] = -INFINITY;
-        top[k >> 1] = fmaxf(top[k >> 1], s[j][k]);
+      for (int k = 0; k < 4; k++) s[j][k] = s2[j][k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < KC; i++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const uint4 v = *reinterpret_cast<const uint4*>(src + kread[i & 1] + j * 8 * (RC * 16) + i * 64);
+        mma16816<T>(s[j], qa[i][0], v.x, v.y);
+        mma16816<T>(s2[j], qa[i][1], v.z, v.w);
       }
+    const int pos = cur.first_pos(), n = cur.keys();
+    cur.advance(b.runs, step);
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) s[j][k] += s2[j][k];
+    if (!(n == SP_KT && pos + SP_KT - 1 <= qmin && (qmax - pos < p.window || pos + SP_KT - 1 < p.n_sink))) {
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int key = 8 * j + 2 * c + (k & 1);
+          if (key >= n || !wa_sees(p, qpos[k >> 1], pos + key)) s[j][k] = -INFINITY;
+        }
+    }
+    const float top[2] = {fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])) * sl,
+                          fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])) * sl};
     if (__any_sync(0xffffffffu, top[0] > m[0] + SP_SLACK || top[1] > m[1] + SP_SLACK)) {
 #pragma unroll
       for (int j = 0; j < 2; j++) {
@@ -323,16 +380,17 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       const float base = m[j] == -INFINITY ? 0.f : m[j];
-      const float p0 = sp_exp2(s[0][2 * j] - base), p1 = sp_exp2(s[0][2 * j + 1] - base);
-      const float p2 = sp_exp2(s[1][2 * j] - base), p3 = sp_exp2(s[1][2 * j + 1] - base);
+      const float p0 = sp_exp2(fmaf(s[0][2 * j], sl, -base)), p1 = sp_exp2(fmaf(s[0][2 * j + 1], sl, -base));
+      const float p2 = sp_exp2(fmaf(s[1][2 * j], sl, -base)), p3 = sp_exp2(fmaf(s[1][2 * j + 1], sl, -base));
       l[j] += (p0 + p1) + (p2 + p3);
       pa[j] = pack2<T>(p0, p1);      // rounded to T for the product: half a step of each weight
       pa[2 + j] = pack2<T>(p2, p3);
     }
 #pragma unroll
     for (int i = 0; i < VB; i++) {
-      const uint4 v0 = src[(2 * KC + i) * 32], v1 = src[(2 * KC + VB + i) * 32];
-      const uint4 v2 = src[(2 * KC + 2 * VB + i) * 32], v3 = src[(2 * KC + 3 * VB + i) * 32];
+      const uint8_t* vs = src + vread + i * 128;
+      const uint4 v0 = *reinterpret_cast<const uint4*>(vs), v1 = *reinterpret_cast<const uint4*>(vs + RC * 16);
+      const uint4 v2 = *reinterpret_cast<const uint4*>(vs + 8 * RC * 16), v3 = *reinterpret_cast<const uint4*>(vs + 9 * RC * 16);
       const uint32_t a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
       const uint32_t a2[4] = {v2.x, v2.y, v2.z, v2.w}, a3[4] = {v3.x, v3.y, v3.z, v3.w};
 #pragma unroll
@@ -341,7 +399,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
         mma16816<T>(o[i][2 * e + 1], pa, __byte_perm(a0[e], a1[e], 0x7632), __byte_perm(a2[e], a3[e], 0x7632));
       }
     }
-    load(t + SP_STAGES * step, slot);  // this lane has read what the slot held
+    __syncwarp();  // every lane has read what the slot held
+    load(ring32 + slot * 2 * TILE);
     slot = slot + 1 == SP_STAGES ? 0 : slot + 1;
   }
   cp_wait<0>();
@@ -412,8 +471,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
 #pragma unroll
         for (int i = 0; i < CH; i++) {
           const bool ok = key < x.n && x8 + 8 * i < chunks;
-          cp16(dst + (j * CH + i) * 32, kb + off + (ok ? 4 * (x8 + 8 * i) : 0), ok);
-          cp16(dst + ((2 + j) * CH + i) * 32, vb + off + (ok ? 4 * (x8 + 8 * i) : 0), ok);
+          cp16_or_zero(smem_u32(dst + (j * CH + i) * 32), kb + off + (ok ? 4 * (x8 + 8 * i) : 0), ok);
+          cp16_or_zero(smem_u32(dst + ((2 + j) * CH + i) * 32), vb + off + (ok ? 4 * (x8 + 8 * i) : 0), ok);
         }
       }
     }
@@ -548,11 +607,13 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
   sp_join<float, R, DT>(p, b, part, wm, wl);
 }
 
-// Splits of one sequence and head: enough CTAs for two per SM (each keeps
-// about 100 KB of copies in flight, so that is past what the memory needs),
-// but no warp without a tile.
+// Splits of one sequence and head: up to three CTAs per SM (what their rings
+// leave room for; 64 KB of copies in flight each), but no warp without a tile.
+// 32 streams of 4100 visible keys, 8 heads of 128, bf16: 83.0 us = 6.48 TB/s
+// (room for two CTAs with three stages each 86.9; four or eight times the
+// splits 88 to 100).
 int sp_split(int64_t blocks, int64_t keys, int kt) {
-  const int64_t room = 2 * (int64_t)sm_count();
+  const int64_t room = 3 * (int64_t)sm_count();
   int n = 1;
   while (n < SP_MAX_SPLIT && blocks * n * 2 <= room && (int64_t)n * 2 * SP_WARPS * kt <= keys) n *= 2;
   return n;
@@ -612,7 +673,7 @@ int sp_f32_rows(const WaParams& p, cudaStream_t s) {
 // Head widths of whole 16-byte vectors, and heads that fit the grid.
 bool wa_split_fits(const WaParams& p, int dtype) {
   const int es = dtype_size(dtype), v = 16 / es;
-  return p.head_dim % v == 0 && (dtype != ARMAI_F32 || p.head_dim <= 128) &&
+  return p.head_dim % v == 0 && p.scale_log2 != 0.f && p.scale_log2 == p.scale_log2 && (dtype != ARMAI_F32 || p.head_dim <= 128) &&
          ((int64_t)p.max_q * p.group + 3) / 4 * (p.n_q_heads / p.group) <= 65535;
 }
 
