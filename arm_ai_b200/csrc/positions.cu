@@ -24,10 +24,11 @@ namespace {
 constexpr int ROT_THREADS = 128;
 constexpr int ROT_MAX_DIM = 256;
 constexpr int ROT_WARPS = ROT_THREADS / 32;
-// Items in flight per warp, and CTAs per SM: 80 warps' worth of 1 KB items per
-// SM. 16381 tokens of 32 + 8 + 8 heads of 128, bf16: 84.9 us = 4.74 TB/s (6 or 8
-// stages 86; 6 or 8 CTAs 92 to 107; two heads per lane in registers and no ring
-// 132; a table shared by the CTA's tokens 262).
+// Items in flight per warp, and CTAs per SM: 20 warps with four items of 1 KB
+// each. 16381 tokens of 32 + 8 + 8 heads of 128, bf16: 71.8 us = 5.61 TB/s (with
+// addresses made anew for each item 85; six to eight CTAs or stages a tenth
+// more; two heads per lane in registers and no ring 132; the cosines and sines
+// of several tokens shared by a CTA 262).
 constexpr int ROT_STAGES = 4;
 constexpr int ROT_CTAS = 5;
 
@@ -102,7 +103,7 @@ __device__ __forceinline__ int64_t rot_row(const RotParams& p, int i, int64_t to
 // Vector form: every head's start and the second vectors 16-byte aligned.
 // Lane l of a head's HL lanes (power of two) has the VEC pairs from l * VEC on:
 //   half layout: the vectors at l * VEC and rot / 2 + l * VEC; the lanes behind
-//   rot / 2 have two vectors each of what is not rotated
+//   rot / 2 one of each half of what is not rotated
 //   interleaved: the two vectors at 2 l * VEC
 // A warp goes through a stream of items, one item being 32 / HL heads of a
 // tensor of one token: all items of the tokens w, w + warps, ... (splits 1), or
@@ -111,8 +112,8 @@ __device__ __forceinline__ int64_t rot_row(const RotParams& p, int i, int64_t to
 // only what it copied itself: enough bytes in flight for the memory, whatever
 // the registers hold.
 template <typename T, typename KV, bool IL>
-__global__ void __launch_bounds__(ROT_THREADS) k_rotate_vec(const RotParams p, int hl, int64_t n_tokens, int items,
-                                                            int splits) {
+__global__ void __launch_bounds__(ROT_THREADS) k_rotate_vec(const RotParams p, int hl, int64_t n_tokens, int splits,
+                                                            float inv_dim) {
   constexpr int VEC = 16 / (int)sizeof(T);
   __shared__ float2 table[ROT_WARPS][ROT_MAX_DIM / 2];
   __shared__ uint4 ring_[ROT_WARPS][ROT_STAGES][2][32];
@@ -122,45 +123,66 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotate_vec(const RotParams p, i
   if (token >= n_tokens) return;
   const int64_t step = (int64_t)gridDim.x * ROT_WARPS;  // tokens between a warp's tokens (splits 1)
   const int half = p.rot >> 1, hpw = 32 / hl, sub = lane / hl, l = lane % hl, p0 = l * VEC;
-  const int da = IL ? 2 * p0 : p0 < half ? p0 : p.rot + 2 * (p0 - half);
-  const int db = IL || p0 >= half ? da + VEC : p0 + half;
+  const int da = IL ? 2 * p0 : p0 < half ? p0 : half + p0;
+  const int db = IL ? da + VEC : p0 < half ? p0 + half : da + (p.dim - p.rot) / 2;
   const bool mine = 2 * p0 < p.dim;
-  const int n0 = (p.t[0].heads + hpw - 1) / hpw, n1 = (p.t[1].heads + hpw - 1) / hpw;  // items of q, of k
 
-  // the tensor of an item of a token, and this lane's head in it
-  auto place = [&](int g, int& h) {
-    const int i = g < n0 ? 0 : g < n0 + n1 ? 1 : 2;
-    h = (g - (i == 0 ? 0 : i == 1 ? n0 : n0 + n1)) * hpw + sub;
-    return i;
-  };
+  // splits: the one item, as tensor and first head
+  int only = 0, h0 = 0;
+  if (splits > 1) {
+    h0 = (int)(unit % splits) * hpw;
+    for (; only < 2; only++) {
+      const int padded = (p.t[only].heads + hpw - 1) / hpw * hpw;
+      if (h0 < padded) break;
+      h0 -= padded;
+    }
+  }
+  // the loads' place in the stream: token, tensor, this lane's head in the item, its address
   uint4(*ring)[2][32] = ring_[warp];
-  int64_t ahead = token;  // the loads' place in the stream
-  int ahead_g = splits > 1 ? (int)(unit % splits) : 0, put = 0;
-  const int end_g = splits > 1 ? ahead_g + 1 : items;
+  int64_t ahead = token, ahead_step = 0;
+  int ahead_i = only, ahead_h = h0 + sub, put = 0;
+  const T* ahead_src = nullptr;
+  auto enter = [&]() {  // the address, at a tensor's start; skips tensors without heads
+    while (ahead < n_tokens) {
+      const RotTensor& t = p.t[ahead_i];
+      if (ahead_h - sub < t.heads) {
+        ahead_src = static_cast<const T*>(t.src) + ahead * t.src_token + ahead_h * t.src_head;
+        ahead_step = hpw * t.src_head;
+        return;
+      }
+      ahead_h = sub;
+      if (++ahead_i == 3) {
+        ahead_i = 0;
+        ahead += step;
+      }
+      if (splits > 1) ahead = n_tokens;
+    }
+  };
+  enter();
   auto load = [&]() {
     if (ahead < n_tokens) {
-      int h;
-      const RotTensor& t = p.t[place(ahead_g, h)];
-      if (mine && h < t.heads) {
-        const T* src = static_cast<const T*>(t.src) + ahead * t.src_token + h * t.src_head;
-        rot_copy16(&ring[put][0][lane], src + da);
-        rot_copy16(&ring[put][1][lane], src + db);
+      const int heads = p.t[ahead_i].heads;
+      if (mine && ahead_h < heads) {
+        rot_copy16(&ring[put][0][lane], ahead_src + da);
+        rot_copy16(&ring[put][1][lane], ahead_src + db);
       }
-      if (++ahead_g == end_g) {
-        ahead_g = 0;
-        ahead = splits > 1 ? n_tokens : ahead + step;
-      }
+      ahead_h += hpw;
+      ahead_src += ahead_step;
+      if (splits > 1)
+        ahead = n_tokens;
+      else if (ahead_h - sub >= heads)
+        enter();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     put = put + 1 == ROT_STAGES ? 0 : put + 1;
   };
-  int g = ahead_g, get = 0;
 #pragma unroll
   for (int i = 0; i < ROT_STAGES; i++) load();
 
+  int get = 0;
   float2* cs = table[warp];
   float c[VEC], s[VEC], ga[VEC], gb[VEC];
-  for (; token < n_tokens; token = splits > 1 ? n_tokens : token + step, g = 0) {
+  for (; token < n_tokens; token += step) {
     __syncwarp();
     if (half) {
       const int64_t pos = p.positions[token];
@@ -173,88 +195,92 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotate_vec(const RotParams p, i
       c[e] = v.x;
       s[e] = v.y;
     }
-    int64_t row = token;
-    int have = -1;  // the tensor whose gains and row these are
-    for (; g < end_g; g++) {
-      int h;
-      const int i = place(g, h);
+    for (int i = only; i < 3; i++) {
       const RotTensor& t = p.t[i];
-      if (i != have) {
-        if (t.gamma && mine) {
+      const bool norm = t.gamma != nullptr;
+      if (norm && mine) {
 #pragma unroll
-          for (int e = 0; e < VEC; e += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(t.gamma + (IL ? da + 2 * e : da + e));
-            const float4 y = *reinterpret_cast<const float4*>(t.gamma + (IL ? da + 2 * e + 4 : db + e));
-            if (IL) {
-              ga[e] = x.x, gb[e] = x.y, ga[e + 1] = x.z, gb[e + 1] = x.w;
-              ga[e + 2] = y.x, gb[e + 2] = y.y, ga[e + 3] = y.z, gb[e + 3] = y.w;
-            } else {
-              ga[e] = x.x, ga[e + 1] = x.y, ga[e + 2] = x.z, ga[e + 3] = x.w;
-              gb[e] = y.x, gb[e + 1] = y.y, gb[e + 2] = y.z, gb[e + 3] = y.w;
-            }
-          }
-        }
-        row = rot_row(p, i, token);
-        have = i;
-      }
-      const bool on = mine && h < t.heads;
-      asm volatile("cp.async.wait_group %0;" ::"n"(ROT_STAGES - 1) : "memory");
-      const Vec<T, VEC> ra = *reinterpret_cast<const Vec<T, VEC>*>(&ring[get][0][lane]);
-      const Vec<T, VEC> rb = *reinterpret_cast<const Vec<T, VEC>*>(&ring[get][1][lane]);
-      get = get + 1 == ROT_STAGES ? 0 : get + 1;
-      float a[VEC], b[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; e++) {
-        // interleaved: values 2e and 2e + 1 of the 2 VEC
-        a[e] = to_f32(!IL ? ra.v[e] : 2 * e < VEC ? ra.v[(2 * e) % VEC] : rb.v[(2 * e) % VEC]);
-        b[e] = to_f32(!IL ? rb.v[e] : 2 * e < VEC ? ra.v[(2 * e + 1) % VEC] : rb.v[(2 * e + 1) % VEC]);
-      }
-      load();  // this lane has read what the slot held
-      if (t.gamma) {
-        float ss = 0.f;
-        if (on) {
-#pragma unroll
-          for (int e = 0; e < VEC; e++) ss += a[e] * a[e] + b[e] * b[e];
-        }
-        for (int o = hl >> 1; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = 1.0f / sqrtf(ss / (float)p.dim + p.eps);
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          a[e] *= inv * ga[e];
-          b[e] *= inv * gb[e];
-        }
-      }
-      if (i < 2) {
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          if (p0 + e < half) {
-            const float x = a[e], y = b[e];
-            a[e] = x * c[e] - y * s[e];
-            b[e] = x * s[e] + y * c[e];
-          }
-        }
-      }
-      if (!on || row < 0) continue;
-      const int64_t off = row * t.dst_token + h * t.dst_head;
-      auto store = [&](auto* base) {
-        using O = std::remove_reference_t<decltype(*base)>;
-        Vec<O, VEC> oa, ob;
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
+        for (int e = 0; e < VEC; e += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(t.gamma + (IL ? da + 2 * e : da + e));
+          const float4 y = *reinterpret_cast<const float4*>(t.gamma + (IL ? da + 2 * e + 4 : db + e));
           if (IL) {
-            Vec<O, VEC>& o = 2 * e < VEC ? oa : ob;
-            o.v[(2 * e) % VEC] = from_f32<O>(a[e]);
-            o.v[(2 * e + 1) % VEC] = from_f32<O>(b[e]);
+            ga[e] = x.x, gb[e] = x.y, ga[e + 1] = x.z, gb[e + 1] = x.w;
+            ga[e + 2] = y.x, gb[e + 2] = y.y, ga[e + 3] = y.z, gb[e + 3] = y.w;
           } else {
-            oa.v[e] = from_f32<O>(a[e]);
-            ob.v[e] = from_f32<O>(b[e]);
+            ga[e] = x.x, ga[e + 1] = x.y, ga[e + 2] = x.z, ga[e + 3] = x.w;
+            gb[e] = y.x, gb[e + 1] = y.y, gb[e + 2] = y.z, gb[e + 3] = y.w;
           }
         }
-        *reinterpret_cast<Vec<O, VEC>*>(base + off + da) = oa;
-        *reinterpret_cast<Vec<O, VEC>*>(base + off + db) = ob;
-      };
-      if (i == 0) store(static_cast<T*>(t.dst)); else store(static_cast<KV*>(t.dst));
+      }
+      const int64_t row = rot_row(p, i, token);
+      const int heads = t.heads;
+      int64_t off = row * t.dst_token + (h0 + sub) * t.dst_head;
+      const int64_t off_step = hpw * t.dst_head;
+#pragma unroll 1
+      for (int h = h0 + sub; h - sub < heads; h += hpw, off += off_step) {
+        const bool on = mine && h < heads;
+        asm volatile("cp.async.wait_group %0;" ::"n"(ROT_STAGES - 1) : "memory");
+        const Vec<T, VEC> ra = *reinterpret_cast<const Vec<T, VEC>*>(&ring[get][0][lane]);
+        const Vec<T, VEC> rb = *reinterpret_cast<const Vec<T, VEC>*>(&ring[get][1][lane]);
+        get = get + 1 == ROT_STAGES ? 0 : get + 1;
+        float a[VEC], b[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          // interleaved: values 2e and 2e + 1 of the 2 VEC
+          a[e] = to_f32(!IL ? ra.v[e] : 2 * e < VEC ? ra.v[(2 * e) % VEC] : rb.v[(2 * e) % VEC]);
+          b[e] = to_f32(!IL ? rb.v[e] : 2 * e < VEC ? ra.v[(2 * e + 1) % VEC] : rb.v[(2 * e + 1) % VEC]);
+        }
+        load();  // this lane has read what the slot held
+        if (norm) {
+          float ss = 0.f;
+          if (on) {
+#pragma unroll
+            for (int e = 0; e < VEC; e++) ss += a[e] * a[e] + b[e] * b[e];
+          }
+          for (int o = hl >> 1; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float inv = rsqrtf(ss * inv_dim + p.eps);
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            a[e] *= inv * ga[e];
+            b[e] *= inv * gb[e];
+          }
+        }
+        if (i < 2 && p0 < half) {
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            // where a lane's pairs end before its vectors, the others have cosine 1 and sine 0; a
+            // selection, not a product, keeps infinities of one out of the other
+            const float x = a[e], y = b[e];
+            const bool in = !IL || p0 + e < half;
+            a[e] = in ? x * c[e] - y * s[e] : x;
+            b[e] = in ? x * s[e] + y * c[e] : y;
+          }
+        }
+        if (on && row >= 0) {
+          auto store = [&](auto* base) {
+            using O = std::remove_reference_t<decltype(*base)>;
+            Vec<O, VEC> oa, ob;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+              if (IL) {
+                Vec<O, VEC>& o = 2 * e < VEC ? oa : ob;
+                o.v[(2 * e) % VEC] = from_f32<O>(a[e]);
+                o.v[(2 * e + 1) % VEC] = from_f32<O>(b[e]);
+              } else {
+                oa.v[e] = from_f32<O>(a[e]);
+                ob.v[e] = from_f32<O>(b[e]);
+              }
+            }
+            *reinterpret_cast<Vec<O, VEC>*>(base + off + da) = oa;
+            *reinterpret_cast<Vec<O, VEC>*>(base + off + db) = ob;
+          };
+          if (i == 0) store(static_cast<T*>(t.dst)); else store(static_cast<KV*>(t.dst));
+        }
+        if (splits > 1) break;
+      }
+      if (splits > 1) break;
     }
+    if (splits > 1) break;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -349,9 +375,9 @@ int rotate_launch(const RotParams& p, int64_t n_tokens, int layout, cudaStream_t
   const int64_t ctas = std::min<int64_t>((n_tokens * splits + ROT_WARPS - 1) / ROT_WARPS,
                                          few ? INT32_MAX : ROT_CTAS * (int64_t)sm_count());
   if (layout == ARMAI_ROPE_INTERLEAVED)
-    k_rotate_vec<T, KV, true><<<(unsigned)ctas, ROT_THREADS, 0, s>>>(p, hl, n_tokens, (int)items, splits);
+    k_rotate_vec<T, KV, true><<<(unsigned)ctas, ROT_THREADS, 0, s>>>(p, hl, n_tokens, splits, 1.0f / (float)p.dim);
   else
-    k_rotate_vec<T, KV, false><<<(unsigned)ctas, ROT_THREADS, 0, s>>>(p, hl, n_tokens, (int)items, splits);
+    k_rotate_vec<T, KV, false><<<(unsigned)ctas, ROT_THREADS, 0, s>>>(p, hl, n_tokens, splits, 1.0f / (float)p.dim);
   ARMAI_CUDA(cudaGetLastError());
   return ARMAI_OK;
 }
