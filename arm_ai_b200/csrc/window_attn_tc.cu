@@ -39,8 +39,8 @@ constexpr int WT_ROWS = 128;                   // query rows per tile, two tiles
 constexpr int WT_LOAD = 8, WT_MMA = 9, WT_CLEAN = 10;  // warps 0-3, 4-7: softmax of tile 0, 1
 constexpr int WT_THREADS = 384;                // warp 11 only completes the warp group
 // Registers: 384 x 168 at launch; the loading group gives up what the softmax
-// threads (128 scores each) need: 256 x 208 + 128 x 88 = 384 x 168.
-constexpr int WT_REGS = 168, WT_REGS_SOFTMAX = 208, WT_REGS_LOAD = 88;
+// threads (128 scores each) need: 256 x 200 + 128 x 104 = 384 x 168.
+constexpr int WT_REGS = 168, WT_REGS_SOFTMAX = 200, WT_REGS_LOAD = 104;
 static_assert(256 * WT_REGS_SOFTMAX + 128 * WT_REGS_LOAD <= WT_THREADS * WT_REGS, "register split");
 constexpr float WT_SLACK = 8.f;
 
@@ -49,7 +49,7 @@ struct WtLayout {
   static constexpr uint32_t TILE = 128u * HD * 2u;       // one operand tile: HD / 64 blocks of 128 rows x 128 B
   static constexpr int SLOTS = HD == 128 ? 5 : 8;        // K and V tiles in turn
   static constexpr uint32_t BAR = (2 + SLOTS) * TILE;
-  static constexpr uint32_t SMEM = 1024 + BAR + 256;
+  static constexpr uint32_t SMEM = 1024 + BAR + 512;
 };
 
 // tcgen05.ld / st of 32 columns of this warp's 32 lanes; the caller waits.
@@ -130,14 +130,14 @@ __device__ __forceinline__ uint32_t wt_pack<__nv_bfloat16>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The weights exp2(scale s - base) of 64 scores s[0 .. 63], as pairs of T in
-// w[0 .. 31]; adds them (unrounded) to the two f32 pairs of sum. w may be the
-// start of s or lie before it.
-template <typename T>
-__device__ __forceinline__ void wt_weights(const uint32_t* s, uint32_t* w, uint64_t sl2, uint64_t nb2,
-                                           uint64_t (&sum)[2]) {
+// The weights exp2(scale s - base) of N scores, as pairs of T in w[0 .. N/2 - 1]
+// (which may be the start of s); returns their f32 sum (of the unrounded values).
+template <typename T, int N>
+__device__ __forceinline__ float wt_weights(const uint32_t* s, uint32_t* w, float sl, float base) {
+  const uint64_t sl2 = wt_pair(sl, sl), nb2 = wt_pair(-base, -base);
+  uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-  for (int c = 0; c < 32; c++) {
+  for (int c = 0; c < N / 2; c++) {
     float e0, e1;
     wt_unpair(wt_fma2(wt_pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sl2, nb2), e0, e1);
     e0 = wt_exp2(e0);
@@ -145,6 +145,9 @@ __device__ __forceinline__ void wt_weights(const uint32_t* s, uint32_t* w, uint6
     sum[c & 1] = wt_add2(sum[c & 1], wt_pair(e0, e1));
     w[c] = wt_pack<T>(e0, e1);
   }
+  float e0, e1;
+  wt_unpair(wt_add2(sum[0], sum[1]), e0, e1);
+  return e0 + e1;
 }
 
 __device__ __forceinline__ void wt_tma3(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
@@ -164,7 +167,6 @@ __device__ __forceinline__ void wt_tma4(void* dst, const CUtensorMap* map, int x
 // positions, the runs and their tiles.
 struct WtWork {
   WaSeq sq;
-  WaRuns runs;
   int vh, kvh, i0, nt;
   int qlo[2], qhi[2];  // positions of a query tile's first and last token; qhi < qlo: no token
 
@@ -208,21 +210,23 @@ __device__ __forceinline__ bool wt_elect() {
 struct WtIter {
   WaTile x;
   int run, left;
-  __device__ __forceinline__ void enter(const WaRuns& r) {
-    x.row = run == 0 ? r.row[0] : run == 1 ? r.row[1] : r.row[2];
-    x.pos = run == 0 ? r.pos[0] : run == 1 ? r.pos[1] : r.pos[2];
-    left = run == 0 ? r.len[0] : run == 1 ? r.len[1] : r.len[2];
+  // runs: rows, positions and lengths of the three runs, in shared memory (the
+  // roles' loops have no registers to spare)
+  __device__ __forceinline__ void enter(const int* runs) {
+    x.row = runs[run];
+    x.pos = runs[3 + run];
+    left = runs[6 + run];
     x.n = min(left, WT_KT);
   }
-  __device__ __forceinline__ explicit WtIter(const WaRuns& r) : run(0) { enter(r); }
-  __device__ __forceinline__ void next(const WaRuns& r) {
+  __device__ __forceinline__ explicit WtIter(const int* runs) : run(0) { enter(runs); }
+  __device__ __forceinline__ void next(const int* runs) {
     x.row += WT_KT;
     x.pos += WT_KT;
     left -= WT_KT;
     x.n = min(left, WT_KT);
-    if (left <= 0) {
+    if (left <= 0 && run < 2) {
       run++;
-      enter(r);
+      enter(runs);
     }
   }
 };
@@ -271,7 +275,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   uint64_t* vclean = pvdone + 2;       // [3] rows behind a short tile of V zeroed (a run has one at most)
   uint64_t* vgo = vclean + 3;          // [3] that tile has landed
   uint64_t* fin = vgo + 3;             // every product done
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 1);
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 1);  // two words, then the runs (9)
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   WtWork w;
@@ -286,8 +290,19 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     w.qlo[h] = w.sq.pos0 + w.i0 + h * tokens;
     w.qhi[h] = w.sq.pos0 + min(w.sq.n, w.i0 + (h + 1) * tokens) - 1;
   }
-  w.runs = wa_runs(p, w.qlo[0], max(w.qhi[0], w.qhi[1]));
-  w.nt = wa_tiles<WT_KT>(w.runs);
+  int* runs = reinterpret_cast<int*>(fin + 2);
+  {
+    const WaRuns r = wa_runs(p, w.qlo[0], max(w.qhi[0], w.qhi[1]));
+    w.nt = wa_tiles<WT_KT>(r);
+    if (tid == 0) {
+#pragma unroll
+      for (int i = 0; i < 3; i++) {
+        runs[i] = r.row[i];
+        runs[3 + i] = r.pos[i];
+        runs[6 + i] = r.len[i];
+      }
+    }
+  }
 
   if (tid == 0) {
     mbar_init(qfull, 1);
@@ -326,69 +341,103 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     float m = -INFINITY, l = 0.f;
     int n = 0;
     bool ok = true;
-    WtIter it(w.runs);
-    for (int t = 0; t < w.nt; t++, it.next(w.runs)) {
+    WtIter it(runs);
+    for (int t = 0; t < w.nt; t++, it.next(runs)) {
       const WaTile x = it.x;
       if (!w.needs(p, h, x)) continue;
       wt_wait(&sfull[h], (uint32_t)(n & 1), ok, p.err);
       tc_fence_after();
-      uint32_t s[128];
-#pragma unroll
-      for (int c = 0; c < 4; c++) wt_ld32(ts + 32u * c, s + 32 * c);
-#pragma unroll
-      for (int c = 0; c < 4; c++) wt_wait_ld(s + 32 * c);
       // columns first .. last are seen, and those before `sink`
       const int last = min(x.n - 1, qpos - x.pos), first = qpos - x.pos - p.window + 1, sink = p.n_sink - x.pos;
       const bool all = last == WT_KT - 1 && (first <= 0 || sink >= WT_KT);
-      if (!__all_sync(0xffffffffu, all)) {
-#pragma unroll
-        for (int c = 0; c < 128; c++)
-          if (c > last || (c < first && c >= sink)) s[c] = 0xff800000u;  // -inf
-      }
-      float a[4];
-#pragma unroll
-      for (int c = 0; c < 4; c++) a[c] = __uint_as_float(s[c]);
-#pragma unroll
-      for (int c = 4; c + 8 <= 128; c += 8)
-#pragma unroll
-        for (int k = 0; k < 4; k++) a[k] = wt_max3(a[k], __uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1]));
-#pragma unroll
-      for (int k = 0; k < 4; k++) a[k] = fmaxf(a[k], __uint_as_float(s[124 + k]));
-      const float top = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * sl;
-      if (__any_sync(0xffffffffu, top > m + WT_SLACK)) {
-        const float nm = fmaxf(m, top);
-        const float f = nm == -INFINITY ? 1.f : wt_exp2(m - nm);
-        m = nm;
-        l *= f;
-        if (n > 0) {
-          wt_wait(&pvdone[h], (uint32_t)((n - 1) & 1), ok, p.err);
-          tc_fence_after();
+      float sum = 0.f;
+      // the maximum is raised to a larger score: the sum and the output so far follow
+      auto raise = [&](float top) {
+        if (__any_sync(0xffffffffu, top > m + WT_SLACK)) {
+          const float nm = fmaxf(m, top);
+          const float f = nm == -INFINITY ? 1.f : wt_exp2(m - nm);
+          m = nm;
+          l *= f;
+          if (n > 0) {
+            wt_wait(&pvdone[h], (uint32_t)((n - 1) & 1), ok, p.err);
+            tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t o[32];
-            wt_ld32(to + c, o);
-            wt_wait_ld(o);
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[32];
+              wt_ld32(to + c, o);
+              wt_wait_ld(o);
 #pragma unroll
-            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            wt_st32(to + c, o);
+              for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              wt_st32(to + c, o);
+            }
           }
         }
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      const uint64_t sl2 = wt_pair(sl, sl), nb2 = wt_pair(-base, -base);
-      uint64_t sum[2] = {0ull, 0ull};
+      };
+      if (__all_sync(0xffffffffu, all)) {
+        uint32_t s[128];
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        wt_weights<T>(s + 64 * half, s + 32 * half, sl2, nb2, sum);
-        wt_st32(ts + 32u * half, s + 32 * half);
+        for (int c = 0; c < 4; c++) wt_ld32(ts + 32u * c, s + 32 * c);
+#pragma unroll
+        for (int c = 0; c < 4; c++) wt_wait_ld(s + 32 * c);
+        float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 128; c += 8)
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            a[k] = wt_max3(a[k], __uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1]));
+        raise(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * sl);
+        sum = wt_weights<T, 128>(s, s, sl, m == -INFINITY ? 0.f : m);
+        wt_st32(ts, s);
+        wt_st32(ts + 32u, s + 32);
+      } else {
+        // an edge tile, 32 columns at a time and twice over (few instructions:
+        // seldom run, they are never in the instruction cache); P of a block
+        // overwrites scores that have been read
+        auto seen = [&](int c) {
+          const int le = last - c + 1, ge = first - c, si = sink - c;
+          const uint32_t ml = le >= 32 ? 0xffffffffu : le <= 0 ? 0u : (1u << le) - 1u;
+          const uint32_t mg = ge >= 32 ? 0u : ge <= 0 ? 0xffffffffu : 0xffffffffu << ge;
+          const uint32_t ms = si >= 32 ? 0xffffffffu : si <= 0 ? 0u : (1u << si) - 1u;
+          return ml & (mg | ms);
+        };
+        auto load = [&](int c, uint32_t mask, uint32_t (&r)[32]) {
+          wt_ld32(ts + c, r);
+          wt_wait_ld(r);
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if (!(mask >> e & 1)) r[e] = 0xff800000u;  // -inf
+        };
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < x.n; c += 32) {
+          const uint32_t mask = seen(c);
+          if (!__any_sync(0xffffffffu, mask)) continue;
+          uint32_t r[32];
+          load(c, mask, r);
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) top = wt_max3(top, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+        }
+        raise(top * sl);
+#pragma unroll 1
+        for (int c = 0; c < x.n; c += 32) {
+          const uint32_t mask = seen(c);
+          uint32_t w16[16];
+          if (__any_sync(0xffffffffu, mask)) {
+            uint32_t r[32];
+            load(c, mask, r);
+            sum += wt_weights<T, 32>(r, w16, sl, m == -INFINITY ? 0.f : m);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) w16[e] = 0u;
+          }
+          qg_tmem_st16(ts + (c >> 1), w16);
+        }
       }
+      l += sum;
       wt_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive1(&pready[h]);
-      float s0, s1;
-      wt_unpair(wt_add2(sum[0], sum[1]), s0, s1);
-      l += s0 + s1;
       n++;
     }
     if (n > 0) wt_wait(&pvdone[h], (uint32_t)((n - 1) & 1), ok, p.err);
@@ -421,7 +470,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         for (int h = 0; h < 2; h++)
           for (int kb = 0; kb < HD / 64; kb++)
             wt_tma3(qs + h * L::TILE + kb * 16384, &mq, 64 * kb, w.vh * pack, w.sq.q0 + w.i0 + h * tokens, qfull);
-        WtIter it(w.runs);
+        WtIter it(runs);
         WtSlot<L::SLOTS> slot;
         int issued = 0;
         bool ok = true;
@@ -434,7 +483,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
                     &full[slot.s]);
           slot.next();
           issued = j + 1;
-          if (j & 1) it.next(w.runs);
+          if (j & 1) it.next(runs);
         }
         // every requested box has landed before the CTA may end
         qg_wait(qfull, 0, p.err);
@@ -450,7 +499,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       const uint32_t qlo = wt_desc_lo(smem_u32(qs), 16), rlo = wt_desc_lo(smem_u32(ring), 16);
       bool ok = true;
       wt_wait(qfull, 0, ok, p.err);
-      WtIter it(w.runs);
+      WtIter it(runs);
       WtSlot<L::SLOTS> slot;
       uint32_t cleaned = 0;
       // bit h: query tile h takes part in the key tile; has had a product P V; the parity of their number
@@ -490,7 +539,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         slot.next();
         const WtSlot<L::SLOTS> v = slot;
         slot.next();
-        it.next(w.runs);
+        it.next(runs);
         const bool more = t + 1 < w.nt;
         const uint32_t next = more ? w.needs(p, 0, it.x) | w.needs(p, 1, it.x) << 1 : 0;
         wt_wait(&full[v.s], v.turn & 1, ok, p.err);
@@ -535,7 +584,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     } else if (warp == WT_CLEAN) {
       // the last product of 16 keys of a short tile also reads rows behind the
       // tile's: zero them (their weights are zero, but the rows may hold anything)
-      WtIter it(w.runs);
+      WtIter it(runs);
       WtSlot<L::SLOTS> slot;
       int cleaned = 0;
       for (int t = 0; t < w.nt; t++) {
@@ -552,7 +601,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
           cleaned++;
         }
         slot.next();
-        it.next(w.runs);
+        it.next(runs);
       }
     }
   }
