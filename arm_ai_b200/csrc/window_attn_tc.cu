@@ -11,9 +11,10 @@
 // one thread issues the MMAs: S of each query tile into its 128 columns of
 // tensor memory, then O += P V with P (16-bit, written back over S) as the A
 // operand from tensor memory and V as the transposed (N-major) B operand from
-// the rows as they lie in the cache. Four warps per query tile, one thread
-// per row, do the softmax: no exchange between threads. While one tile's
-// softmax runs, the tensor cores work on the other's products.
+// the rows as they lie in the cache. Four warps per query tile, a thread per
+// row, do its softmax; each query tile has two score buffers and an issuing
+// warp of its own, so that the tensor cores turn one buffer round (P V of a
+// key tile, S of the next but one) while the softmax works on the other.
 //
 // The row's maximum is raised, and its output in tensor memory rescaled, only
 // when a score exceeds it by more than 2^8: then weights stay below 2^8, sums
@@ -34,21 +35,21 @@
 namespace armai {
 namespace {
 
-constexpr int WT_KT = 128;                     // keys per tile
+constexpr int WT_KT = 64;                      // keys per tile
 constexpr int WT_ROWS = 128;                   // query rows per tile, two tiles per CTA
-constexpr int WT_LOAD = 8, WT_MMA = 9, WT_CLEAN = 10;  // warps 0-3, 4-7: softmax of tile 0, 1
-constexpr int WT_THREADS = 384;                // warp 11 only completes the warp group
-// Registers: 384 x 168 at launch; the loading group gives up what the softmax
-// threads (128 scores each) need: 256 x 200 + 128 x 104 = 384 x 168.
-constexpr int WT_REGS = 168, WT_REGS_SOFTMAX = 200, WT_REGS_LOAD = 104;
-static_assert(256 * WT_REGS_SOFTMAX + 128 * WT_REGS_LOAD <= WT_THREADS * WT_REGS, "register split");
+constexpr int WT_LOAD = 8, WT_MMA = 9, WT_CLEAN = 11;  // warps 0-3, 4-7: softmax of query tile 0, 1; 9, 10: its MMAs
+constexpr int WT_THREADS = 384;
 constexpr float WT_SLACK = 8.f;
 
 template <int HD>
 struct WtLayout {
-  static constexpr uint32_t TILE = 128u * HD * 2u;       // one operand tile: HD / 64 blocks of 128 rows x 128 B
-  static constexpr int SLOTS = HD == 128 ? 5 : 8;        // K and V tiles in turn
-  static constexpr uint32_t BAR = (2 + SLOTS) * TILE;
+  static constexpr uint32_t Q = 128u * HD * 2u;     // a query tile: HD / 64 blocks of 128 rows x 128 B
+  static constexpr uint32_t KV = WT_KT * HD * 2u;   // a key tile of K or V: HD / 64 blocks of 64 rows x 128 B
+  // the first two K tiles, then slots of V of a key tile and K of the next but
+  // one: they are used, and given back, together
+  static constexpr int SLOTS = 4;
+  static constexpr uint32_t K0 = 2 * Q, RING = K0 + 2 * KV;
+  static constexpr uint32_t BAR = RING + SLOTS * 2 * KV;
   static constexpr uint32_t SMEM = 1024 + BAR + 512;
 };
 
@@ -265,17 +266,20 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   const uint32_t raw = smem_u32(wt_raw);
   uint8_t* smem = wt_raw + (((raw + 1023u) & ~1023u) - raw);
   uint8_t* qs = smem;                  // two query tiles
-  uint8_t* ring = smem + 2 * L::TILE;  // SLOTS tiles: K of a key tile, then V
-  uint64_t* qfull = reinterpret_cast<uint64_t*>(smem + L::BAR);
+  uint8_t* k0 = smem + L::K0;          // the first two K tiles
+  uint8_t* ring = smem + L::RING;      // SLOTS x (V, K of the next key tile but one)
+  uint64_t* qfull = reinterpret_cast<uint64_t*>(smem + L::BAR);  // the query tiles and the first K tiles
   uint64_t* full = qfull + 1;          // [SLOTS]
-  uint64_t* empty = full + L::SLOTS;   // [SLOTS]
-  uint64_t* sfull = empty + L::SLOTS;  // [2] S of query tile h written
-  uint64_t* pready = sfull + 2;        // [2] P of query tile h in place
-  uint64_t* pvdone = pready + 2;       // [2] P V of query tile h added
-  uint64_t* vclean = pvdone + 2;       // [3] rows behind a short tile of V zeroed (a run has one at most)
+  uint64_t* empty = full + L::SLOTS;   // [SLOTS] both query tiles' products done
+  uint64_t* sfull = empty + L::SLOTS;  // [2][2] S of query tile h in its buffer b written
+  uint64_t* pready = sfull + 4;        // [2][2] P in place
+  uint64_t* pvdone = pready + 4;       // [2][2] P V added
+  uint64_t* vclean = pvdone + 4;       // [3] rows behind a short tile of V zeroed (a run has one at most)
   uint64_t* vgo = vclean + 3;          // [3] that tile has landed
-  uint64_t* fin = vgo + 3;             // every product done
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 1);  // two words, then the runs (9)
+  uint64_t* fin = vgo + 3;             // [2] every product done
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 2);
+  uint32_t* info = tslot + 1;          // [SLOTS] of a slot's K tile: its keys, and the query tiles that need it
+  int* runs = reinterpret_cast<int*>(info + L::SLOTS);  // [9]
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   WtWork w;
@@ -290,67 +294,75 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     w.qlo[h] = w.sq.pos0 + w.i0 + h * tokens;
     w.qhi[h] = w.sq.pos0 + min(w.sq.n, w.i0 + (h + 1) * tokens) - 1;
   }
-  int* runs = reinterpret_cast<int*>(fin + 2);
   {
     const WaRuns r = wa_runs(p, w.qlo[0], max(w.qhi[0], w.qhi[1]));
     w.nt = wa_tiles<WT_KT>(r);
-    if (tid == 0) {
+    if (tid == WT_LOAD * 32) {
 #pragma unroll
       for (int i = 0; i < 3; i++) {
         runs[i] = r.row[i];
         runs[3 + i] = r.pos[i];
         runs[6 + i] = r.len[i];
       }
+      mbar_init(qfull, 1);
+      for (int i = 0; i < L::SLOTS; i++) {
+        mbar_init(&full[i], 1);
+        mbar_init(&empty[i], 2);
+      }
+      for (int i = 0; i < 4; i++) {
+        mbar_init(&sfull[i], 1);
+        mbar_init(&pready[i], 4);
+        mbar_init(&pvdone[i], 1);
+      }
+      for (int i = 0; i < 3; i++) {
+        mbar_init(&vclean[i], 1);
+        mbar_init(&vgo[i], 2);
+      }
+      mbar_init(&fin[0], 1);
+      mbar_init(&fin[1], 1);
+      fence_mbar_init();
+      // the query tiles and the first K tiles are on their way before the CTA meets
+      mbar_arrive_tx(qfull, 2 * L::Q + (uint32_t)min(w.nt, 2) * L::KV);
+      for (int h = 0; h < 2; h++)
+        for (int kb = 0; kb < HD / 64; kb++)
+          wt_tma3(qs + h * L::Q + kb * 16384, &mq, 64 * kb, w.vh * pack, w.sq.q0 + w.i0 + h * tokens, qfull);
+      WtIter it(runs);
+      for (int t = 0; t < min(w.nt, 2); t++, it.next(runs))
+        for (int kb = 0; kb < HD / 64; kb++)
+          wt_tma4(k0 + t * L::KV + kb * 8192, &mk, 64 * kb, it.x.row, w.kvh, w.sq.slot, qfull);
     }
   }
-
-  if (tid == 0) {
-    mbar_init(qfull, 1);
-    mbar_init(fin, 1);
-    for (int i = 0; i < 3; i++) {
-      mbar_init(&vclean[i], 1);
-      mbar_init(&vgo[i], 1);
-    }
-    for (int i = 0; i < L::SLOTS; i++) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int h = 0; h < 2; h++) {
-      mbar_init(&sfull[h], 1);
-      mbar_init(&pready[h], 4);
-      mbar_init(&pvdone[h], 1);
-    }
-    fence_mbar_init();
-  }
-  if (warp == 0) tmem_alloc(tslot, 512);
+  if (warp == WT_MMA) tmem_alloc(tslot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // the whole of tensor memory, so from column 0 on: S 0 in 0-127, S 1 in 128-255, O 0 from 256, O 1 from 384
+  // The whole of tensor memory, so from column 0 on: S of query tile h, buffer
+  // b from 128 h + 64 b (P over the first half of it), O of query tile h from
+  // 256 + 128 h.
   constexpr uint32_t tmem = 0;
 
   if (warp < WT_LOAD) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(WT_REGS_SOFTMAX));
     // ---- softmax: thread = query row ----
     const int h = warp >> 2, row = tid & 127;
     const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t ts = tmem + lane_base + 128u * (uint32_t)h, to = ts + 256u;
+    const uint32_t to = tmem + lane_base + 256u + 128u * (uint32_t)h;
     const int tok = w.i0 + h * tokens + row / pack, head = w.vh * pack + row % pack;
     const int qpos = w.sq.pos0 + tok;
     const float sl = p.scale_log2;
     float m = -INFINITY, l = 0.f;
     int n = 0;
     bool ok = true;
+    // waits for the last product issued for these rows
+    auto products = [&]() { wt_wait(&pvdone[2 * h + ((n - 1) & 1)], (uint32_t)((n - 1) >> 1 & 1), ok, p.err); };
     WtIter it(runs);
+#pragma unroll 1
     for (int t = 0; t < w.nt; t++, it.next(runs)) {
       const WaTile x = it.x;
       if (!w.needs(p, h, x)) continue;
-      wt_wait(&sfull[h], (uint32_t)(n & 1), ok, p.err);
-      tc_fence_after();
+      const uint32_t ts = tmem + lane_base + 128u * (uint32_t)h + 64u * (uint32_t)(n & 1);
       // columns first .. last are seen, and those before `sink`
       const int last = min(x.n - 1, qpos - x.pos), first = qpos - x.pos - p.window + 1, sink = p.n_sink - x.pos;
-      const bool all = last == WT_KT - 1 && (first <= 0 || sink >= WT_KT);
-      float sum = 0.f;
+      const bool all = __all_sync(0xffffffffu, last == WT_KT - 1 && (first <= 0 || sink >= WT_KT));
       // the maximum is raised to a larger score: the sum and the output so far follow
       auto raise = [&](float top) {
         if (__any_sync(0xffffffffu, top > m + WT_SLACK)) {
@@ -359,7 +371,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
           m = nm;
           l *= f;
           if (n > 0) {
-            wt_wait(&pvdone[h], (uint32_t)((n - 1) & 1), ok, p.err);
+            products();
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
@@ -373,22 +385,23 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
           }
         }
       };
-      if (__all_sync(0xffffffffu, all)) {
-        uint32_t s[128];
-#pragma unroll
-        for (int c = 0; c < 4; c++) wt_ld32(ts + 32u * c, s + 32 * c);
-#pragma unroll
-        for (int c = 0; c < 4; c++) wt_wait_ld(s + 32 * c);
+      wt_wait(&sfull[2 * h + (n & 1)], (uint32_t)(n >> 1 & 1), ok, p.err);
+      tc_fence_after();
+      if (all) {
+        uint32_t s[64];
+        wt_ld32(ts, s);
+        wt_ld32(ts + 32u, s + 32);
+        wt_wait_ld(s);
+        wt_wait_ld(s + 32);
         float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 128; c += 8)
+        for (int c = 0; c < 64; c += 8)
 #pragma unroll
           for (int k = 0; k < 4; k++)
             a[k] = wt_max3(a[k], __uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1]));
         raise(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * sl);
-        sum = wt_weights<T, 128>(s, s, sl, m == -INFINITY ? 0.f : m);
+        l += wt_weights<T, 64>(s, s, sl, m == -INFINITY ? 0.f : m);
         wt_st32(ts, s);
-        wt_st32(ts + 32u, s + 32);
       } else {
         // an edge tile, 32 columns at a time and twice over (few instructions:
         // seldom run, they are never in the instruction cache); P of a block
@@ -425,7 +438,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
           if (__any_sync(0xffffffffu, mask)) {
             uint32_t r[32];
             load(c, mask, r);
-            sum += wt_weights<T, 32>(r, w16, sl, m == -INFINITY ? 0.f : m);
+            l += wt_weights<T, 32>(r, w16, sl, m == -INFINITY ? 0.f : m);
           } else {
 #pragma unroll
             for (int e = 0; e < 16; e++) w16[e] = 0u;
@@ -433,14 +446,13 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
           qg_tmem_st16(ts + (c >> 1), w16);
         }
       }
-      l += sum;
       wt_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive1(&pready[h]);
+      if (lane == 0) mbar_arrive1(&pready[2 * h + (n & 1)]);
       n++;
     }
-    if (n > 0) wt_wait(&pvdone[h], (uint32_t)((n - 1) & 1), ok, p.err);
+    if (n > 0) products();
     tc_fence_after();
     const bool none = n == 0 || l == 0.f;  // no key seen
     const float inv = ok ? 1.0f / l : __int_as_float(0x7fc00000);
@@ -462,152 +474,141 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         }
       }
     }
-  } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WT_REGS_LOAD));
-    if (warp == WT_LOAD) {
-      if (lane == 0) {
-        mbar_arrive_tx(qfull, 2 * L::TILE);
-        for (int h = 0; h < 2; h++)
-          for (int kb = 0; kb < HD / 64; kb++)
-            wt_tma3(qs + h * L::TILE + kb * 16384, &mq, 64 * kb, w.vh * pack, w.sq.q0 + w.i0 + h * tokens, qfull);
-        WtIter it(runs);
-        WtSlot<L::SLOTS> slot;
-        int issued = 0;
-        bool ok = true;
-        for (int j = 0; j < 2 * w.nt; j++) {
-          if (slot.turn) ok = qg_wait(&empty[slot.s], (slot.turn - 1) & 1, p.err);
-          if (!ok) break;
-          mbar_arrive_tx(&full[slot.s], L::TILE);
-          for (int kb = 0; kb < HD / 64; kb++)
-            wt_tma4(ring + slot.s * L::TILE + kb * 16384, (j & 1) ? &mv : &mk, 64 * kb, it.x.row, w.kvh, w.sq.slot,
-                    &full[slot.s]);
-          slot.next();
-          issued = j + 1;
-          if (j & 1) it.next(runs);
-        }
-        // every requested box has landed before the CTA may end
-        qg_wait(qfull, 0, p.err);
-        for (int j = issued > L::SLOTS ? issued - L::SLOTS : 0; j < issued; j++)
-          qg_wait(&full[j % L::SLOTS], (uint32_t)((j / L::SLOTS) & 1), p.err);
-      }
-    } else if (warp == WT_MMA) {
-      // The whole warp walks the loop, so that the operands' descriptors stay in
-      // uniform registers; one elected lane issues.
-      constexpr uint32_t TY = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      constexpr uint32_t BASE = (1u << 4) | (TY << 7) | (TY << 10) | ((uint32_t)(WT_ROWS >> 4) << 24);
-      constexpr uint32_t PV = BASE | (1u << 16) | ((uint32_t)(HD >> 3) << 17);  // B transposed
-      const uint32_t qlo = wt_desc_lo(smem_u32(qs), 16), rlo = wt_desc_lo(smem_u32(ring), 16);
+  } else if (warp == WT_LOAD) {
+    if (lane == 0) {
+      WtIter iv(runs), ik(runs);  // the key tiles whose V, whose K comes next
+      ik.next(runs);
+      ik.next(runs);
+      WtSlot<L::SLOTS> slot;
+      int issued = 0;
       bool ok = true;
-      wt_wait(qfull, 0, ok, p.err);
-      WtIter it(runs);
-      WtSlot<L::SLOTS> slot;
-      uint32_t cleaned = 0;
-      // bit h: query tile h takes part in the key tile; has had a product P V; the parity of their number
-      uint32_t need = 0, begun = 0, par = 0;
-      // S of query tile h with the K tile in slot s
-      auto qk = [&](int h, const WaTile& x, int s) {
-        // its columns held P of the tile before
-        if (begun >> h & 1) wt_wait(&pvdone[h], (par >> h & 1) ^ 1, ok, p.err);
-        tc_fence_after();
-        const uint32_t idesc = BASE | ((uint32_t)((x.n + 15) >> 4) << 18);  // N: the tile's keys, in steps of 16
-        const uint32_t qa = qlo + (uint32_t)h * (L::TILE >> 4), ka = rlo + (uint32_t)s * (L::TILE >> 4);
-        if (wt_elect()) {
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; kk++) {
-            const uint32_t off = (uint32_t)(kk >> 2) * 1024u + 2u * (uint32_t)(kk & 3);
-            tc_mma_ss(tmem + 128u * (uint32_t)h, wt_desc(qa + off), wt_desc(ka + off), idesc, kk > 0);
-          }
-          qg_commit(&sfull[h]);
-        }
-        __syncwarp();
-      };
-      if (w.nt > 0) {
-        need = w.needs(p, 0, it.x) | w.needs(p, 1, it.x) << 1;
-        wt_wait(&full[0], 0, ok, p.err);
-#pragma unroll 1
-        for (int h = 0; h < 2; h++)
-          if (need >> h & 1) qk(h, it.x, 0);
-        if (wt_elect()) qg_commit(&empty[0]);
-        __syncwarp();
-      }
-      // Every step of this loop lies on the path between a weight and the next
-      // score, and its code is refetched each time (the softmax's fills the
-      // instruction caches): one copy for both query tiles, few branches.
-#pragma unroll 1
       for (int t = 0; t < w.nt; t++) {
-        const WaTile x = it.x;
+        const bool more = t + 2 < w.nt;
+        if (slot.turn) ok = qg_wait(&empty[slot.s], (slot.turn - 1) & 1, p.err);
+        if (!ok) break;
+        // what the issuing warps have to know of the slot's K tile
+        info[slot.s] =
+            more ? (uint32_t)ik.x.n | (uint32_t)w.needs(p, 0, ik.x) << 8 | (uint32_t)w.needs(p, 1, ik.x) << 9 : 0u;
+        uint8_t* dst = ring + slot.s * 2 * L::KV;
+        mbar_arrive_tx(&full[slot.s], (more ? 2 : 1) * L::KV);
+        for (int kb = 0; kb < HD / 64; kb++)
+          wt_tma4(dst + kb * 8192, &mv, 64 * kb, iv.x.row, w.kvh, w.sq.slot, &full[slot.s]);
+        if (more)
+          for (int kb = 0; kb < HD / 64; kb++)
+            wt_tma4(dst + L::KV + kb * 8192, &mk, 64 * kb, ik.x.row, w.kvh, w.sq.slot, &full[slot.s]);
         slot.next();
-        const WtSlot<L::SLOTS> v = slot;
-        slot.next();
-        it.next(runs);
-        const bool more = t + 1 < w.nt;
-        const uint32_t next = more ? w.needs(p, 0, it.x) | w.needs(p, 1, it.x) << 1 : 0;
-        wt_wait(&full[v.s], v.turn & 1, ok, p.err);
-        if (more) wt_wait(&full[slot.s], slot.turn & 1, ok, p.err);
-        if (x.n & 15) {
-          if (lane == 0) mbar_arrive1(&vgo[cleaned]);
-          wt_wait(&vclean[cleaned++], 0, ok, p.err);
-        }
-        // 64-wide blocks of the row 16 KB apart
-        const uint32_t va = rlo + (uint32_t)v.s * (L::TILE >> 4) + ((16384u - 16u) >> 4 << 16);
-#pragma unroll 1
-        for (int h = 0; h < 2; h++) {
-          if (need >> h & 1) {
-            const uint32_t o = tmem + 256u + 128u * (uint32_t)h, pa = tmem + 128u * (uint32_t)h;
-            wt_wait(&pready[h], par >> h & 1, ok, p.err);
-            tc_fence_after();
-            if (wt_elect()) {
-#pragma unroll
-              for (int kk = 0; kk < WT_KT / 16; kk++)
-                if (16 * kk < x.n)
-                  qg_mma_ts(o, pa + 8u * kk, wt_desc(va + 128u * kk), PV, kk > 0 ? 1u : begun >> h & 1);
-              qg_commit(&pvdone[h]);
-            }
-            __syncwarp();
-            begun |= 1u << h;
-            par ^= 1u << h;
-          }
-          if (next >> h & 1) qk(h, it.x, slot.s);
-        }
-        if (wt_elect()) {
-          qg_commit(&empty[v.s]);
-          if (more) qg_commit(&empty[slot.s]);
-        }
-        __syncwarp();
-        need = next;
+        iv.next(runs);
+        ik.next(runs);
+        issued = t + 1;
       }
-      // no product is in flight when tensor memory is given back, failed waits or not
-      if (wt_elect()) qg_commit(fin);
+      // every requested box has landed before the CTA may end
+      qg_wait(qfull, 0, p.err);
+      for (int t = issued > L::SLOTS ? issued - L::SLOTS : 0; t < issued; t++)
+        qg_wait(&full[t % L::SLOTS], (uint32_t)((t / L::SLOTS) & 1), p.err);
+    }
+  } else if (warp < WT_CLEAN) {
+    // ---- products of query tile h. The whole warp walks the loop, so that the
+    // operands' descriptors stay in uniform registers; one elected lane issues.
+    const int h = warp - WT_MMA;
+    constexpr uint32_t TY = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t BASE = (1u << 4) | (TY << 7) | (TY << 10) | ((uint32_t)(WT_ROWS >> 4) << 24);
+    constexpr uint32_t PV = BASE | (1u << 16) | ((uint32_t)(HD >> 3) << 17);  // B transposed
+    const uint32_t qa = wt_desc_lo(smem_u32(qs), 16) + (uint32_t)h * (L::Q >> 4);
+    const uint32_t klo = wt_desc_lo(smem_u32(k0), 16), rlo = wt_desc_lo(smem_u32(ring), 16);
+    const uint32_t ts = tmem + 128u * (uint32_t)h, to = tmem + 256u + 128u * (uint32_t)h;
+    bool ok = true;
+    uint32_t cleaned = 0;
+    int nq = 0, np = 0;  // products S and P V issued
+    auto qk = [&](int keys, uint32_t ka) {
+      const int b = nq & 1;
+      // its buffer held P of the key tile two before
+      if (nq >= 2) wt_wait(&pvdone[2 * h + b], (uint32_t)((nq >> 1) - 1) & 1, ok, p.err);
+      tc_fence_after();
+      const uint32_t idesc = BASE | ((uint32_t)((keys + 15) >> 4) << 18);  // N: the tile's keys, in steps of 16
+      if (wt_elect()) {
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; kk++)
+          tc_mma_ss(ts + 64u * (uint32_t)b, wt_desc(qa + (uint32_t)(kk >> 2) * 1024u + 2u * (uint32_t)(kk & 3)),
+                    wt_desc(ka + (uint32_t)(kk >> 2) * 512u + 2u * (uint32_t)(kk & 3)), idesc, kk > 0);
+        qg_commit(&sfull[2 * h + b]);
+      }
       __syncwarp();
-      ok = true;
-      wt_wait(fin, 0, ok, p.err);
-    } else if (warp == WT_CLEAN) {
-      // the last product of 16 keys of a short tile also reads rows behind the
-      // tile's: zero them (their weights are zero, but the rows may hold anything)
+      nq++;
+    };
+    // of the key tiles now, next and next but one: keys | whether this query tile needs them << 8
+    uint32_t now = 0, next = 0;
+    wt_wait(qfull, 0, ok, p.err);
+    {
       WtIter it(runs);
-      WtSlot<L::SLOTS> slot;
-      int cleaned = 0;
-      for (int t = 0; t < w.nt; t++) {
-        slot.next();
-        if (it.x.n & 15) {
-          if (!qg_wait_warp(&vgo[cleaned], 0, p.err)) break;
-          const int rows = 16 - (it.x.n & 15);
-          for (int e = lane; e < rows * (HD / 8); e += 32)
-            *reinterpret_cast<uint4*>(ring + slot.s * L::TILE + (e & 7) * 16 + (it.x.n + (e >> 3) % rows) * 128 +
-                                      ((e >> 3) / rows) * 16384) = make_uint4(0u, 0u, 0u, 0u);
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive1(&vclean[cleaned]);
-          cleaned++;
-        }
-        slot.next();
-        it.next(runs);
+      if (w.nt > 0) now = (uint32_t)it.x.n | (uint32_t)w.needs(p, h, it.x) << 8;
+      it.next(runs);
+      if (w.nt > 1) next = (uint32_t)it.x.n | (uint32_t)w.needs(p, h, it.x) << 8;
+      if (now >> 8) qk((int)(now & 255u), klo);
+      if (next >> 8) qk((int)(next & 255u), klo + (L::KV >> 4));
+    }
+    WtSlot<L::SLOTS> slot;
+#pragma unroll 1
+    for (int t = 0; t < w.nt; t++) {
+      wt_wait(&full[slot.s], slot.turn & 1, ok, p.err);
+      const uint32_t word = info[slot.s], after = (word & 255u) | (word >> (8 + h) & 1) << 8;
+      const int keys = (int)(now & 255u);
+      if (keys & 15) {
+        if (lane == 0) mbar_arrive1(&vgo[cleaned]);
+        wt_wait(&vclean[cleaned++], 0, ok, p.err);
       }
+      const uint32_t base = rlo + (uint32_t)slot.s * (2 * L::KV >> 4);
+      if (now >> 8) {
+        const int b = np & 1;
+        const uint32_t va = base + ((8192u - 16u) >> 4 << 16);  // 64-wide blocks of the row 8 KB apart
+        wt_wait(&pready[2 * h + b], (uint32_t)(np >> 1) & 1, ok, p.err);
+        tc_fence_after();
+        if (wt_elect()) {
+#pragma unroll
+          for (int kk = 0; kk < WT_KT / 16; kk++)
+            if (16 * kk < keys)
+              qg_mma_ts(to, ts + 64u * (uint32_t)b + 8u * kk, wt_desc(va + 128u * kk), PV, kk > 0 ? 1u : np > 0);
+          qg_commit(&pvdone[2 * h + b]);
+        }
+        __syncwarp();
+        np++;
+      }
+      if (after >> 8) qk((int)(after & 255u), base + (L::KV >> 4));
+      if (wt_elect()) qg_commit(&empty[slot.s]);
+      __syncwarp();
+      slot.next();
+      now = next;
+      next = after;
+    }
+    // no product is in flight when tensor memory is given back, failed waits or not
+    if (wt_elect()) qg_commit(&fin[h]);
+    __syncwarp();
+    ok = true;
+    wt_wait(&fin[h], 0, ok, p.err);
+  } else {
+    // the last product of 16 keys of a short tile also reads rows behind the
+    // tile's: zero them (their weights are zero, but the rows may hold anything)
+    WtIter it(runs);
+    WtSlot<L::SLOTS> slot;
+    int cleaned = 0;
+    for (int t = 0; t < w.nt; t++) {
+      if (it.x.n & 15) {
+        if (!qg_wait_warp(&vgo[cleaned], 0, p.err)) break;
+        const int rows = 16 - (it.x.n & 15);
+        for (int e = lane; e < rows * (HD / 8); e += 32)
+          *reinterpret_cast<uint4*>(ring + slot.s * 2 * L::KV + (e & 7) * 16 + (it.x.n + (e >> 3) % rows) * 128 +
+                                    ((e >> 3) / rows) * 8192) = make_uint4(0u, 0u, 0u, 0u);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(&vclean[cleaned]);
+        cleaned++;
+      }
+      slot.next();
+      it.next(runs);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == WT_MMA) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -656,14 +657,6 @@ int wt_launch(const WaParams& in, int dtype, cudaStream_t s, bool* fits) {
           wt_map(&mv, dtype, 4, p.v, kd, kst, kb);
   if (!*fits) return ARMAI_OK;
   ARMAI_CUDA(cudaGetSymbolAddress((void**)&p.err, g_wt_err));
-  // the register split waits for registers that a smaller launch would not have
-  static thread_local int regs = 0;
-  if (!regs) {
-    cudaFuncAttributes fa;
-    ARMAI_CUDA(cudaFuncGetAttributes(&fa, k_wa_tc<T, HD>));
-    regs = fa.numRegs;
-  }
-  if (regs != WT_REGS) return fail(ARMAI_E_INVALID, "window_attn: the tensor-core kernel was built with " + std::to_string(regs) + " registers");
   ARMAI_CUDA(cudaFuncSetAttribute(k_wa_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WtLayout<HD>::SMEM));
   const int tokens = 2 * WT_ROWS / pack;
   const dim3 grid((unsigned)((p.max_q + tokens - 1) / tokens), (unsigned)(p.n_q_heads / pack), (unsigned)p.n_seq);
