@@ -547,16 +547,25 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       if (next >> 8) qk((int)(next & 255u), klo + (L::KV >> 4));
     }
     WtSlot<L::SLOTS> slot;
-#pragma unroll 1
-    for (int t = 0; t < w.nt; t++) {
+    uint32_t word = 0;
+    // the slot's tiles have landed, rows behind a short V tile are zeroed
+    auto arrived = [&](int keys) {
       wt_wait(&full[slot.s], slot.turn & 1, ok, p.err);
-      const uint32_t word = info[slot.s], after = (word & 255u) | (word >> (8 + h) & 1) << 8;
-      const int keys = (int)(now & 255u);
+      word = info[slot.s];
       if (keys & 15) {
         if (lane == 0) mbar_arrive1(&vgo[cleaned]);
         wt_wait(&vclean[cleaned++], 0, ok, p.err);
       }
-      const uint32_t base = rlo + (uint32_t)slot.s * (2 * L::KV >> 4);
+    };
+    if (w.nt > 0) arrived((int)(now & 255u));
+    // The schedulers are busy with the softmax, and every step from a weight to
+    // the next score but one is waited for: what can be done while P V runs
+    // (looking after the next slot) is done there.
+#pragma unroll 1
+    for (int t = 0; t < w.nt; t++) {
+      const uint32_t after = (word & 255u) | (word >> (8 + h) & 1) << 8;
+      const int keys = (int)(now & 255u), s = slot.s;
+      const uint32_t base = rlo + (uint32_t)s * (2 * L::KV >> 4);
       if (now >> 8) {
         const int b = np & 1;
         const uint32_t va = base + ((8192u - 16u) >> 4 << 16);  // 64-wide blocks of the row 8 KB apart
@@ -572,12 +581,13 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         __syncwarp();
         np++;
       }
-      if (after >> 8) qk((int)(after & 255u), base + (L::KV >> 4));
-      if (wt_elect()) qg_commit(&empty[slot.s]);
-      __syncwarp();
-      slot.next();
       now = next;
       next = after;
+      slot.next();
+      if (t + 1 < w.nt) arrived((int)(now & 255u));
+      if (after >> 8) qk((int)(after & 255u), base + (L::KV >> 4));
+      if (wt_elect()) qg_commit(&empty[s]);
+      __syncwarp();
     }
     // no product is in flight when tensor memory is given back, failed waits or not
     if (wt_elect()) qg_commit(&fin[h]);
