@@ -1,5 +1,6 @@
 // window_attn_tc.cu — window attention of many queries on the 5th-generation
-// tensor cores (f16 and bf16, head width 64 or 128).
+// tensor cores (f16 and bf16, head width up to 128: 64 or 128 columns, those
+// behind the head zero-filled by TMA).
 //
 //   S = Q K^T, P = exp2(scale S - m), O += P V, over the visible key tiles
 //
@@ -20,17 +21,24 @@
 // when a score exceeds it by more than 2^8: then weights stay below 2^8, sums
 // far inside f32, and most tiles need no pass over the output.
 //
+// With few query tiles the key tiles are divided over the CTAs of a cluster,
+// whose parts are joined through distributed shared memory in rank order.
+//
 // Rounding: scores, weights and sums f32; the weights rounded once to the
 // tensors' type for P V (half a step each), the output once at the end.
 // Every wait is bounded; rows whose wait gave up are written as NaN.
+#include <cooperative_groups.h>
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
 #include "tcgen05.cuh"
 #include "window_attn.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace armai {
 namespace {
@@ -232,6 +240,16 @@ struct WtIter {
   }
 };
 
+// The share of a run's tiles that lie in [a, b) of all tiles, t0 of them before it.
+__device__ __forceinline__ void wt_share(int& row, int& pos, int& len, int& t0, int a, int b) {
+  const int n = (len + WT_KT - 1) / WT_KT;
+  const int lo = min(max(a - t0, 0), n), hi = min(max(b - t0, 0), n);
+  row += lo * WT_KT;
+  pos += lo * WT_KT;
+  len = max(min(len, hi * WT_KT) - lo * WT_KT, 0);
+  t0 += n;
+}
+
 // Place in a ring of N slots: the slot and how often it has been used before.
 template <int N>
 struct WtSlot {
@@ -260,7 +278,7 @@ __device__ __forceinline__ uint32_t wt_desc_lo(uint32_t saddr, uint32_t lead) {
 template <typename T, int HD>
 __global__ void __launch_bounds__(WT_THREADS, 1)
     k_wa_tc(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-            const __grid_constant__ CUtensorMap mv, const WaParams p, int pack) {
+            const __grid_constant__ CUtensorMap mv, const WaParams p, int pack, int ranks) {
   using L = WtLayout<HD>;
   extern __shared__ uint8_t wt_raw[];
   const uint32_t raw = smem_u32(wt_raw);
@@ -280,13 +298,20 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 2);
   uint32_t* info = tslot + 1;          // [SLOTS] of a slot's K tile: its keys, and the query tiles that need it
   int* runs = reinterpret_cast<int*>(info + L::SLOTS);  // [9]
+  // over the operands, once they are done with: every rank's part of the rows
+  // that this rank joins
+  cg::cluster_group cluster = cg::this_cluster();
+  const int share = 2 * WT_ROWS / ranks;                // rows
+  float4* part_o = reinterpret_cast<float4*>(smem);     // [ranks][HD / 4][share]
+  float2* part_s = reinterpret_cast<float2*>(smem + 2 * WT_ROWS * HD * 4);  // [ranks][share] maximum, sum
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   WtWork w;
   w.sq = wa_seq(p, blockIdx.z);
   const int tokens = WT_ROWS / pack;   // per query tile
-  w.i0 = (int)(gridDim.x - 1 - blockIdx.x) * 2 * tokens;  // the longest causal rows first
-  if (w.i0 >= w.sq.n) return;
+  const int rank = blockIdx.x % ranks;  // in the cluster
+  w.i0 = (int)((gridDim.x - 1 - blockIdx.x) / ranks) * 2 * tokens;  // the longest causal rows first
+  if (w.i0 >= w.sq.n) return;          // the whole cluster
   w.vh = blockIdx.y;
   w.kvh = w.vh * pack / p.group;
 #pragma unroll
@@ -295,15 +320,28 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     w.qhi[h] = w.sq.pos0 + min(w.sq.n, w.i0 + (h + 1) * tokens) - 1;
   }
   {
-    const WaRuns r = wa_runs(p, w.qlo[0], max(w.qhi[0], w.qhi[1]));
+    WaRuns r = wa_runs(p, w.qlo[0], max(w.qhi[0], w.qhi[1]));
     w.nt = wa_tiles<WT_KT>(r);
+    if (ranks > 1) {  // this rank's share
+      const int lo = w.nt * rank / ranks, hi = w.nt * (rank + 1) / ranks;
+      int t0 = 0;
+#pragma unroll
+      for (int i = 0; i < 3; i++) wt_share(r.row[i], r.pos[i], r.len[i], t0, lo, hi);
+      w.nt = hi - lo;
+    }
     if (tid == WT_LOAD * 32) {
+      // without the empty runs: a loop goes from one to the next
+      int k = 0;
 #pragma unroll
       for (int i = 0; i < 3; i++) {
-        runs[i] = r.row[i];
-        runs[3 + i] = r.pos[i];
-        runs[6 + i] = r.len[i];
+        if (r.len[i] > 0) {
+          runs[k] = r.row[i];
+          runs[3 + k] = r.pos[i];
+          runs[6 + k] = r.len[i];
+          k++;
+        }
       }
+      for (; k < 3; k++) runs[k] = runs[3 + k] = runs[6 + k] = 0;
       mbar_init(qfull, 1);
       for (int i = 0; i < L::SLOTS; i++) {
         mbar_init(&full[i], 1);
@@ -454,24 +492,46 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     }
     if (n > 0) products();
     tc_fence_after();
-    const bool none = n == 0 || l == 0.f;  // no key seen
-    const float inv = ok ? 1.0f / l : __int_as_float(0x7fc00000);
-    T* out = static_cast<T*>(p.out) + (int64_t)(w.sq.q0 + tok) * p.o_token + (int64_t)head * p.o_head;
+    if (ranks == 1) {
+      const bool none = n == 0 || l == 0.f;  // no key seen
+      const float inv = ok ? 1.0f / l : __int_as_float(0x7fc00000);
+      T* out = static_cast<T*>(p.out) + (int64_t)(w.sq.q0 + tok) * p.o_token + (int64_t)head * p.o_head;
 #pragma unroll 1
-    for (int c = 0; c < HD; c += 32) {
-      uint32_t o[32];
-      wt_ld32(to + c, o);
-      wt_wait_ld(o);
-      if (tok < w.sq.n) {
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        wt_ld32(to + c, o);
+        wt_wait_ld(o);
+        if (tok < w.sq.n) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          uint32_t v[4];
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t v[4];
 #pragma unroll
-          for (int k = 0; k < 4; k++)
-            v[k] = ok && none ? 0u
-                              : wt_pack<T>(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
-          *reinterpret_cast<uint4*>(out + c + e) = make_uint4(v[0], v[1], v[2], v[3]);
+            for (int k = 0; k < 4; k++)
+              v[k] = ok && none ? 0u
+                                : wt_pack<T>(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
+            if (c + e < p.head_dim) *reinterpret_cast<uint4*>(out + c + e) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
         }
+      }
+    } else {
+      // Each row's part goes to the rank that joins the row (remote stores: no
+      // latency to wait for), once every rank is done with its operands.
+      cluster.sync();
+      const int r = tid, owner = r / share;
+      float4* to_o = cluster.map_shared_rank(part_o, owner) + rank * (HD / 4) * share + r % share;
+      float2* to_s = cluster.map_shared_rank(part_s, owner) + rank * share + r % share;
+      *to_s = make_float2(m, ok ? l : __int_as_float(0x7fc00000));
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        wt_ld32(to + c, o);
+        wt_wait_ld(o);
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+          to_o[(c + e) / 4 * share] =
+              n == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                     : make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                                   __uint_as_float(o[e + 3]));
       }
     }
   } else if (warp == WT_LOAD) {
@@ -616,11 +676,40 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       it.next(runs);
     }
   }
+  if (ranks > 1 && warp >= WT_LOAD) {
+    __syncwarp();
+    cluster.sync();  // the softmax warps' first
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == WT_MMA) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+  if (ranks > 1) {
+    cluster.sync();  // the parts of this rank's rows have come
+    for (int e = tid; e < share * (HD / 4); e += WT_THREADS) {
+      const int i = e % share, c = e / share, r = rank * share + i;
+      const int tok = w.i0 + r / pack, head = w.vh * pack + r % pack;  // query tile 1 follows tile 0
+      if (tok >= w.sq.n || 4 * c >= p.head_dim) continue;
+      float m = -INFINITY, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < ranks; k++) m = fmaxf(m, part_s[k * share + i].x);
+      const float base = m == -INFINITY ? 0.f : m;
+      for (int k = 0; k < ranks; k++) {
+        const float2 st = part_s[k * share + i];
+        const float4 v = part_o[(k * (HD / 4) + c) * share + i];
+        const float f = wt_exp2(st.x - base);
+        l += f * st.y;
+        o.x += f * v.x;
+        o.y += f * v.y;
+        o.z += f * v.z;
+        o.w += f * v.w;
+      }
+      const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key seen: 0 * 0
+      T* out = static_cast<T*>(p.out) + (int64_t)(w.sq.q0 + tok) * p.o_token + (int64_t)head * p.o_head + 4 * c;
+      *reinterpret_cast<uint2*>(out) = make_uint2(wt_pack<T>(o.x * inv, o.y * inv), wt_pack<T>(o.z * inv, o.w * inv));
+    }
   }
 }
 
@@ -649,6 +738,10 @@ bool wt_map(CUtensorMap* map, int dtype, int rank, const void* base, const cuuin
 }
 
 __device__ uint32_t g_wt_err;
+// CTAs in clusters that the device holds at once, one per SM (a few SMs are
+// left over where a cluster does not fit: 132 of 148 with clusters of 4, 120
+// with 8).
+constexpr int64_t WT_FILL = 120;
 
 template <typename T, int HD>
 int wt_launch(const WaParams& in, int dtype, cudaStream_t s, bool* fits) {
@@ -657,10 +750,10 @@ int wt_launch(const WaParams& in, int dtype, cudaStream_t s, bool* fits) {
   int pack = 1;  // heads per token in a tile: the power of two in the group
   while (pack < 128 && p.group % (2 * pack) == 0) pack *= 2;
   CUtensorMap mq, mk, mv;
-  const cuuint64_t qd[3] = {(cuuint64_t)HD, (cuuint64_t)p.n_q_heads, (cuuint64_t)p.n_tokens};
+  const cuuint64_t qd[3] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.n_q_heads, (cuuint64_t)p.n_tokens};
   const cuuint64_t qst[2] = {(cuuint64_t)p.q_head * 2, (cuuint64_t)p.q_token * 2};
   const cuuint32_t qb[3] = {64, (cuuint32_t)pack, (cuuint32_t)(WT_ROWS / pack)};
-  const cuuint64_t kd[4] = {(cuuint64_t)HD, (cuuint64_t)p.kv_rows, (cuuint64_t)n_kv, (cuuint64_t)p.n_slots};
+  const cuuint64_t kd[4] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.kv_rows, (cuuint64_t)n_kv, (cuuint64_t)p.n_slots};
   const cuuint64_t kst[3] = {(cuuint64_t)p.kv_row * 2, (cuuint64_t)p.kv_head * 2, (cuuint64_t)p.kv_slot * 2};
   const cuuint32_t kb[4] = {64, WT_KT, 1, 1};
   *fits = wt_map(&mq, dtype, 3, p.q, qd, qst, qb) && wt_map(&mk, dtype, 4, p.k, kd, kst, kb) &&
@@ -669,19 +762,36 @@ int wt_launch(const WaParams& in, int dtype, cudaStream_t s, bool* fits) {
   ARMAI_CUDA(cudaGetSymbolAddress((void**)&p.err, g_wt_err));
   ARMAI_CUDA(cudaFuncSetAttribute(k_wa_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WtLayout<HD>::SMEM));
   const int tokens = 2 * WT_ROWS / pack;
-  const dim3 grid((unsigned)((p.max_q + tokens - 1) / tokens), (unsigned)(p.n_q_heads / pack), (unsigned)p.n_seq);
-  k_wa_tc<T, HD><<<grid, WT_THREADS, WtLayout<HD>::SMEM, s>>>(mq, mk, mv, p, pack);
-  ARMAI_CUDA(cudaGetLastError());
+  const int64_t blocks = (p.max_q + tokens - 1) / tokens, ctas = blocks * (p.n_q_heads / pack) * p.n_seq;
+  // Fewer CTAs than half the SMs: the keys divided over clusters, four key
+  // tiles at least for each CTA.
+  const int64_t keys = std::min<int64_t>(p.kv_rows, (int64_t)p.window + p.n_sink + tokens);
+  int ranks = 1;
+  while (ranks < 8 && ctas * ranks * 2 <= WT_FILL && keys >= 8 * WT_KT * ranks) ranks *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(blocks * ranks), (unsigned)(p.n_q_heads / pack), (unsigned)p.n_seq);
+  cfg.blockDim = dim3(WT_THREADS);
+  cfg.dynamicSmemBytes = WtLayout<HD>::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  ARMAI_CUDA(cudaLaunchKernelEx(&cfg, k_wa_tc<T, HD>, mq, mk, mv, p, pack, ranks));
   return ARMAI_OK;
 }
 
 }  // namespace
 
 int wa_tc_launch(const WaParams& p, int dtype, cudaStream_t s, bool* fits) {
-  *fits = dtype != ARMAI_F32 && (p.head_dim == 64 || p.head_dim == 128) && p.scale_log2 > 0.f;
+  *fits = dtype != ARMAI_F32 && p.head_dim <= 128 && p.head_dim % 8 == 0 && p.scale_log2 > 0.f;
   if (!*fits) return ARMAI_OK;
-  if (dtype == ARMAI_F16) return p.head_dim == 64 ? wt_launch<__half, 64>(p, dtype, s, fits) : wt_launch<__half, 128>(p, dtype, s, fits);
-  return p.head_dim == 64 ? wt_launch<__nv_bfloat16, 64>(p, dtype, s, fits) : wt_launch<__nv_bfloat16, 128>(p, dtype, s, fits);
+  const bool narrow = p.head_dim <= 64;
+  if (dtype == ARMAI_F16) return narrow ? wt_launch<__half, 64>(p, dtype, s, fits) : wt_launch<__half, 128>(p, dtype, s, fits);
+  return narrow ? wt_launch<__nv_bfloat16, 64>(p, dtype, s, fits) : wt_launch<__nv_bfloat16, 128>(p, dtype, s, fits);
 }
 
 }  // namespace armai
