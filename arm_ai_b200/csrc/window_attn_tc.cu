@@ -278,8 +278,9 @@ __device__ __forceinline__ uint32_t wt_desc_lo(uint32_t saddr, uint32_t lead) {
 template <typename T, int HD>
 __global__ void __launch_bounds__(WT_THREADS, 1)
     k_wa_tc(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-            const __grid_constant__ CUtensorMap mv, const WaParams p, int pack, int ranks) {
+            const __grid_constant__ CUtensorMap mv, const WaParams p, int lpack, int lranks) {
   using L = WtLayout<HD>;
+  const int pack = 1 << lpack, ranks = 1 << lranks;  // heads per token in a query tile; CTAs per cluster
   extern __shared__ uint8_t wt_raw[];
   const uint32_t raw = smem_u32(wt_raw);
   uint8_t* smem = wt_raw + (((raw + 1023u) & ~1023u) - raw);
@@ -301,16 +302,21 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   // over the operands, once they are done with: every rank's part of the rows
   // that this rank joins
   cg::cluster_group cluster = cg::this_cluster();
-  const int share = 2 * WT_ROWS / ranks;                // rows
+  const int lshare = 8 - lranks, share = 1 << lshare;   // rows: 256 / ranks
   float4* part_o = reinterpret_cast<float4*>(smem);     // [ranks][HD / 4][share]
   float2* part_s = reinterpret_cast<float2*>(smem + 2 * WT_ROWS * HD * 4);  // [ranks][share] maximum, sum
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  if (tid == WT_MMA * 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
+  }
   WtWork w;
   w.sq = wa_seq(p, blockIdx.z);
-  const int tokens = WT_ROWS / pack;   // per query tile
-  const int rank = blockIdx.x % ranks;  // in the cluster
-  w.i0 = (int)((gridDim.x - 1 - blockIdx.x) / ranks) * 2 * tokens;  // the longest causal rows first
+  const int tokens = WT_ROWS >> lpack;  // per query tile
+  const int rank = blockIdx.x & (ranks - 1);
+  w.i0 = (int)((gridDim.x - 1 - blockIdx.x) >> lranks) * 2 * tokens;  // the longest causal rows first
   if (w.i0 >= w.sq.n) return;          // the whole cluster
   w.vh = blockIdx.y;
   w.kvh = w.vh * pack / p.group;
@@ -329,6 +335,16 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       for (int i = 0; i < 3; i++) wt_share(r.row[i], r.pos[i], r.len[i], t0, lo, hi);
       w.nt = hi - lo;
     }
+    if (warp == WT_LOAD) {
+      // a lane per barrier
+      const int nb = (int)(reinterpret_cast<uint64_t*>(tslot) - qfull);
+      if (lane < nb) {
+        const uint64_t* b = qfull + lane;
+        mbar_init(qfull + lane, b >= empty && b < sfull ? 2 : b >= pready && b < pvdone ? 4 : b >= vgo && b < fin ? 2 : 1);
+      }
+      fence_mbar_init();
+      __syncwarp();
+    }
     if (tid == WT_LOAD * 32) {
       // without the empty runs: a loop goes from one to the next
       int k = 0;
@@ -342,23 +358,6 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         }
       }
       for (; k < 3; k++) runs[k] = runs[3 + k] = runs[6 + k] = 0;
-      mbar_init(qfull, 1);
-      for (int i = 0; i < L::SLOTS; i++) {
-        mbar_init(&full[i], 1);
-        mbar_init(&empty[i], 2);
-      }
-      for (int i = 0; i < 4; i++) {
-        mbar_init(&sfull[i], 1);
-        mbar_init(&pready[i], 4);
-        mbar_init(&pvdone[i], 1);
-      }
-      for (int i = 0; i < 3; i++) {
-        mbar_init(&vclean[i], 1);
-        mbar_init(&vgo[i], 2);
-      }
-      mbar_init(&fin[0], 1);
-      mbar_init(&fin[1], 1);
-      fence_mbar_init();
       // the query tiles and the first K tiles are on their way before the CTA meets
       mbar_arrive_tx(qfull, 2 * L::Q + (uint32_t)min(w.nt, 2) * L::KV);
       for (int h = 0; h < 2; h++)
@@ -384,7 +383,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     const int h = warp >> 2, row = tid & 127;
     const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t to = tmem + lane_base + 256u + 128u * (uint32_t)h;
-    const int tok = w.i0 + h * tokens + row / pack, head = w.vh * pack + row % pack;
+    const int tok = w.i0 + h * tokens + (row >> lpack), head = w.vh * pack + (row & (pack - 1));
     const int qpos = w.sq.pos0 + tok;
     const float sl = p.scale_log2;
     float m = -INFINITY, l = 0.f;
@@ -517,9 +516,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       // Each row's part goes to the rank that joins the row (remote stores: no
       // latency to wait for), once every rank is done with its operands.
       cluster.sync();
-      const int r = tid, owner = r / share;
-      float4* to_o = cluster.map_shared_rank(part_o, owner) + rank * (HD / 4) * share + r % share;
-      float2* to_s = cluster.map_shared_rank(part_s, owner) + rank * share + r % share;
+      const int r = tid, owner = r >> lshare;
+      float4* to_o = cluster.map_shared_rank(part_o, owner) + rank * (HD / 4) * share + (r & (share - 1));
+      float2* to_s = cluster.map_shared_rank(part_s, owner) + rank * share + (r & (share - 1));
       *to_s = make_float2(m, ok ? l : __int_as_float(0x7fc00000));
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
@@ -688,27 +687,45 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   }
   if (ranks > 1) {
     cluster.sync();  // the parts of this rank's rows have come
-    for (int e = tid; e < share * (HD / 4); e += WT_THREADS) {
-      const int i = e % share, c = e / share, r = rank * share + i;
-      const int tok = w.i0 + r / pack, head = w.vh * pack + r % pack;  // query tile 1 follows tile 0
-      if (tok >= w.sq.n || 4 * c >= p.head_dim) continue;
-      float m = -INFINITY, l = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = 0; k < ranks; k++) m = fmaxf(m, part_s[k * share + i].x);
+    // 256 threads, so that a thread keeps its row where a share is at most 256
+    // rows: the weights of the ranks' parts are made once per row
+    if (warp < WT_LOAD) {
+      const int i = tid & (share - 1), r = rank * share + i;
+      const int tok = w.i0 + (r >> lpack), head = w.vh * pack + (r & (pack - 1));  // query tile 1 follows tile 0
+      float m = -INFINITY, l = 0.f, f[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (k < ranks) m = fmaxf(m, part_s[k * share + i].x);
       const float base = m == -INFINITY ? 0.f : m;
-      for (int k = 0; k < ranks; k++) {
-        const float2 st = part_s[k * share + i];
-        const float4 v = part_o[(k * (HD / 4) + c) * share + i];
-        const float f = wt_exp2(st.x - base);
-        l += f * st.y;
-        o.x += f * v.x;
-        o.y += f * v.y;
-        o.z += f * v.z;
-        o.w += f * v.w;
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        f[k] = 0.f;
+        if (k < ranks) {
+          const float2 st = part_s[k * share + i];
+          f[k] = wt_exp2(st.x - base);
+          l += f[k] * st.y;
+        }
       }
       const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key seen: 0 * 0
-      T* out = static_cast<T*>(p.out) + (int64_t)(w.sq.q0 + tok) * p.o_token + (int64_t)head * p.o_head + 4 * c;
-      *reinterpret_cast<uint2*>(out) = make_uint2(wt_pack<T>(o.x * inv, o.y * inv), wt_pack<T>(o.z * inv, o.w * inv));
+#pragma unroll
+      for (int k = 0; k < 8; k++) f[k] *= inv;
+      T* out = static_cast<T*>(p.out) + (int64_t)(w.sq.q0 + tok) * p.o_token + (int64_t)head * p.o_head;
+      if (tok < w.sq.n) {
+        // eight columns at a time
+        for (int c = 2 * (tid >> lshare); c < HD / 4; c += 2 * (256 >> lshare)) {
+          float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 8; k++)
+            if (k < ranks) {
+              const float4 v = part_o[(k * (HD / 4) + c) * share + i], u = part_o[(k * (HD / 4) + c + 1) * share + i];
+              o[0] += f[k] * v.x, o[1] += f[k] * v.y, o[2] += f[k] * v.z, o[3] += f[k] * v.w;
+              o[4] += f[k] * u.x, o[5] += f[k] * u.y, o[6] += f[k] * u.z, o[7] += f[k] * u.w;
+            }
+          if (4 * c < p.head_dim)
+            *reinterpret_cast<uint4*>(out + 4 * c) = make_uint4(wt_pack<T>(o[0], o[1]), wt_pack<T>(o[2], o[3]),
+                                                                wt_pack<T>(o[4], o[5]), wt_pack<T>(o[6], o[7]));
+        }
+      }
     }
   }
 }
@@ -747,8 +764,9 @@ template <typename T, int HD>
 int wt_launch(const WaParams& in, int dtype, cudaStream_t s, bool* fits) {
   WaParams p = in;
   const int n_kv = p.n_q_heads / p.group;
-  int pack = 1;  // heads per token in a tile: the power of two in the group
-  while (pack < 128 && p.group % (2 * pack) == 0) pack *= 2;
+  int lpack = 0;  // heads per token in a query tile: the power of two in the group
+  while (lpack < 7 && p.group % (2 << lpack) == 0) lpack++;
+  const int pack = 1 << lpack;
   CUtensorMap mq, mk, mv;
   const cuuint64_t qd[3] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.n_q_heads, (cuuint64_t)p.n_tokens};
   const cuuint64_t qst[2] = {(cuuint64_t)p.q_head * 2, (cuuint64_t)p.q_token * 2};
@@ -766,8 +784,9 @@ int wt_launch(const WaParams& in, int dtype, cudaStream_t s, bool* fits) {
   // Fewer CTAs than half the SMs: the keys divided over clusters, four key
   // tiles at least for each CTA.
   const int64_t keys = std::min<int64_t>(p.kv_rows, (int64_t)p.window + p.n_sink + tokens);
-  int ranks = 1;
-  while (ranks < 8 && ctas * ranks * 2 <= WT_FILL && keys >= 8 * WT_KT * ranks) ranks *= 2;
+  int lranks = 0;
+  while (lranks < 3 && (ctas << lranks) * 2 <= WT_FILL && keys >= (int64_t)8 * WT_KT << lranks) lranks++;
+  const int ranks = 1 << lranks;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(blocks * ranks), (unsigned)(p.n_q_heads / pack), (unsigned)p.n_seq);
   cfg.blockDim = dim3(WT_THREADS);
@@ -780,7 +799,7 @@ int wt_launch(const WaParams& in, int dtype, cudaStream_t s, bool* fits) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = ranks > 1 ? 1 : 0;
-  ARMAI_CUDA(cudaLaunchKernelEx(&cfg, k_wa_tc<T, HD>, mq, mk, mv, p, pack, ranks));
+  ARMAI_CUDA(cudaLaunchKernelEx(&cfg, k_wa_tc<T, HD>, mq, mk, mv, p, lpack, lranks));
   return ARMAI_OK;
 }
 
