@@ -8,8 +8,9 @@
 // k_wa_simt takes every type, head width up to 256, alignment and stride. It
 // is bound by f32 arithmetic: a CTA has 64 queries of one head and walks the
 // visible keys in tiles of 64; 256 threads, each 4 queries x 4 keys of the
-// scores and 4 queries x (width / 16) of the output, so that a float4 of q, k
-// or v read from shared memory feeds four to sixteen products.
+// scores and 4 queries x (width / 16) of the output, so that a vector of q, k
+// or v read from shared memory feeds eight to sixteen products. Two CTAs per
+// SM up to a width of 96, so that one computes while the other loads.
 #include <algorithm>
 #include <string>
 
@@ -26,152 +27,167 @@ constexpr size_t ws_smem() {
   return ((size_t)3 * WS_Q * (DM + 4) + WS_Q * WS_PP) * 4;
 }
 
+// n rows of head_dim values into shared rows of DM f32 (zeros behind them);
+// `vec`: f32 rows of whole 16-byte vectors, copied asynchronously.
 template <typename T, int DM>
-__global__ void __launch_bounds__(WS_THREADS, 1) k_wa_simt(const WaParams p) {
+__device__ __forceinline__ void ws_rows(float* dst, const T* src, int64_t stride, int n, int D, bool vec) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (sizeof(T) == 4 && vec) {
+    for (int e = threadIdx.x; e < 64 * (DM / 4); e += WS_THREADS) {
+      const int r = e / (DM / 4), d = e % (DM / 4) * 4;
+      const bool ok = r < n && d < D;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                       (uint32_t)__cvta_generic_to_shared(dst + r * (DM + 4) + d)),
+                   "l"(ok ? src + r * stride + d : src), "r"(ok ? 16 : 0)
+                   : "memory");
+    }
+    return;
+  }
+  for (int r = warp; r < 64; r += WS_THREADS / 32)
+    for (int d = lane; d < DM; d += 32) dst[r * (DM + 4) + d] = r < n && d < D ? to_f32(src[r * stride + d]) : 0.f;
+}
+
+template <typename T, int DM>
+__global__ void __launch_bounds__(WS_THREADS, DM <= 96 ? 2 : 1) k_wa_simt(const WaParams p, int vec) {
   constexpr int DP = DM + 4;
-  constexpr int OJ = DM / 64;  // float4 columns of the output per thread
-  extern __shared__ float ws[];
+  constexpr int OJ = DM / 32;  // pairs of output columns per thread: 2 tx + 32 j
+  extern __shared__ __align__(16) float ws[];
   float* Qs = ws;
   float* Ks = Qs + WS_Q * DP;
   float* Vs = Ks + WS_K * DP;
   float* Ps = Vs + WS_K * DP;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, tx = tid & 15, ty = tid >> 4;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int h = blockIdx.y;
   const WaSeq sq = wa_seq(p, blockIdx.z);
   const int i0 = blockIdx.x * WS_Q;
   if (i0 >= sq.n) return;
   const int rows = min(WS_Q, sq.n - i0);
   const int64_t kv_off = (int64_t)sq.slot * p.kv_slot + (int64_t)(h / p.group) * p.kv_head;
-  const T* qb = static_cast<const T*>(p.q) + (int64_t)(sq.q0 + i0) * p.q_token + (int64_t)h * p.q_head;
+  const T* kb = static_cast<const T*>(p.k) + kv_off;
+  const T* vb = static_cast<const T*>(p.v) + kv_off;
   const int D = p.head_dim;
+  ws_rows<T, DM>(Qs, static_cast<const T*>(p.q) + (int64_t)(sq.q0 + i0) * p.q_token + (int64_t)h * p.q_head, p.q_token,
+                 rows, D, vec);
 
-  for (int r = warp; r < WS_Q; r += WS_THREADS / 32)
-    for (int d = lane; d < DM; d += 32)
-      Qs[r * DP + d] = r < rows && d < D ? to_f32(qb[(int64_t)r * p.q_token + d]) * p.scale_log2 : 0.f;
-
-  float o[4][OJ * 4], m[4], l[4];
+  float m[4], l[4];
+  float2 o[4][OJ];
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
-    for (int j = 0; j < OJ * 4; j++) o[i][j] = 0.f;
+    for (int j = 0; j < OJ; j++) o[i][j] = make_float2(0.f, 0.f);
   }
   const int qpos0 = sq.pos0 + i0 + ty * 4;  // of this thread's first query
-  const WaRuns runs = wa_runs(p, sq.pos0 + i0, sq.pos0 + i0 + rows - 1);
+  const int qlo = sq.pos0 + i0, qhi = qlo + rows - 1;
+  const WaRuns runs = wa_runs(p, qlo, qhi);
+  const int nt = wa_tiles<WS_K>(runs);
 #pragma unroll 1
-  for (int s = 0; s < runs.n; s++) {
-    const int row0 = s == 0 ? runs.row[0] : s == 1 ? runs.row[1] : runs.row[2];
-    const int pos0 = s == 0 ? runs.pos[0] : s == 1 ? runs.pos[1] : runs.pos[2];
-    const int len = s == 0 ? runs.len[0] : s == 1 ? runs.len[1] : runs.len[2];
-#pragma unroll 1
-    for (int t0 = 0; t0 < len; t0 += WS_K) {
-      const int nk = min(WS_K, len - t0);
-      __syncthreads();
-      for (int r = warp; r < WS_K; r += WS_THREADS / 32) {
-        const int64_t off = kv_off + (int64_t)(row0 + t0 + r) * p.kv_row;
-        const T* kr = static_cast<const T*>(p.k) + off;
-        const T* vr = static_cast<const T*>(p.v) + off;
-        for (int d = lane; d < DM; d += 32) {
-          const bool ok = r < nk && d < D;
-          Ks[r * DP + d] = ok ? to_f32(kr[d]) : 0.f;
-          Vs[r * DP + d] = ok ? to_f32(vr[d]) : 0.f;
-        }
-      }
-      __syncthreads();
-      float acc[4][4];
+  for (int t = 0; t < nt; t++) {
+    const WaTile x = wa_tile<WS_K>(runs, t);
+    __syncthreads();
+    ws_rows<T, DM>(Ks, kb + (int64_t)x.row * p.kv_row, p.kv_row, x.n, D, vec);
+    ws_rows<T, DM>(Vs, vb + (int64_t)x.row * p.kv_row, p.kv_row, x.n, D, vec);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    float acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc[i][j] = 0.f;
+#pragma unroll 2
+    for (int d = 0; d < DM; d += 4) {
+      float4 a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) a[i] = *reinterpret_cast<const float4*>(Qs + (ty * 4 + i) * DP + d);
+#pragma unroll
+      for (int j = 0; j < 4; j++) b[j] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * j) * DP + d);
 #pragma unroll
       for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = 0.f;
-#pragma unroll 2
-      for (int d = 0; d < DM; d += 4) {
-        float4 a[4], b[4];
+        for (int j = 0; j < 4; j++)
+          acc[i][j] += a[i].x * b[j].x + a[i].y * b[j].y + a[i].z * b[j].z + a[i].w * b[j].w;
+    }
+    const bool full = x.n == WS_K && x.pos + WS_K - 1 <= qlo && (qhi - x.pos < p.window || x.pos + WS_K - 1 < p.n_sink);
 #pragma unroll
-        for (int i = 0; i < 4; i++) a[i] = *reinterpret_cast<const float4*>(Qs + (ty * 4 + i) * DP + d);
+    for (int i = 0; i < 4; i++) {
+      float mt = m[i];
 #pragma unroll
-        for (int j = 0; j < 4; j++) b[j] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * j) * DP + d);
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-          for (int j = 0; j < 4; j++)
-            acc[i][j] += a[i].x * b[j].x + a[i].y * b[j].y + a[i].z * b[j].z + a[i].w * b[j].w;
+      for (int j = 0; j < 4; j++) {
+        const int kk = tx + 16 * j;
+        acc[i][j] *= p.scale_log2;
+        if (!full && (kk >= x.n || !wa_sees(p, qpos0 + i, x.pos + kk))) acc[i][j] = -INFINITY;
+        mt = fmaxf(mt, acc[i][j]);
       }
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        float mt = m[i];
+      for (int w = 8; w >= 1; w >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, w));
+      const float base = mt == -INFINITY ? 0.f : mt;  // nothing seen yet: every weight is exp2(-inf) = 0
+      const float corr = exp2f(m[i] - base);
+      float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int kk = tx + 16 * j;
-          if (kk >= nk || !wa_sees(p, qpos0 + i, pos0 + t0 + kk)) acc[i][j] = -INFINITY;
-          mt = fmaxf(mt, acc[i][j]);
-        }
-#pragma unroll
-        for (int x = 8; x >= 1; x >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
-        const float base = mt == -INFINITY ? 0.f : mt;  // nothing seen yet: every p is exp2(-inf) = 0
-        const float corr = exp2f(m[i] - base);
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float e = exp2f(acc[i][j] - base);
-          sum += e;
-          Ps[(ty * 4 + i) * WS_PP + tx + 16 * j] = e;
-        }
-#pragma unroll
-        for (int x = 8; x >= 1; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        l[i] = l[i] * corr + sum;
-        m[i] = mt;
-#pragma unroll
-        for (int j = 0; j < OJ * 4; j++) o[i][j] *= corr;
+      for (int j = 0; j < 4; j++) {
+        const float e = exp2f(acc[i][j] - base);
+        sum += e;
+        Ps[(ty * 4 + i) * WS_PP + tx + 16 * j] = e;
       }
-      __syncwarp();  // a query's row of P is written and read by one half-warp
+      l[i] = l[i] * corr + sum;  // this thread's keys; its sixteen are added up at the end
+      m[i] = mt;
+#pragma unroll
+      for (int j = 0; j < OJ; j++) {
+        o[i][j].x *= corr;
+        o[i][j].y *= corr;
+      }
+    }
+    __syncwarp();  // a query's row of P is written and read by one half-warp
 #pragma unroll 2
-      for (int c = 0; c < WS_K; c += 4) {
-        float4 a[4];
+    for (int c = 0; c < WS_K; c += 4) {
+      float4 a[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) a[i] = *reinterpret_cast<const float4*>(Ps + (ty * 4 + i) * WS_PP + c);
+      for (int i = 0; i < 4; i++) a[i] = *reinterpret_cast<const float4*>(Ps + (ty * 4 + i) * WS_PP + c);
 #pragma unroll
-        for (int cc = 0; cc < 4; cc++)
+      for (int cc = 0; cc < 4; cc++)
 #pragma unroll
-          for (int j = 0; j < OJ; j++) {
-            const float4 b = *reinterpret_cast<const float4*>(Vs + (c + cc) * DP + tx * 4 + 64 * j);
+        for (int j = 0; j < OJ; j++) {
+          const float2 b = *reinterpret_cast<const float2*>(Vs + (c + cc) * DP + tx * 2 + 32 * j);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const float w = cc == 0 ? a[i].x : cc == 1 ? a[i].y : cc == 2 ? a[i].z : a[i].w;
-              o[i][4 * j] += w * b.x;
-              o[i][4 * j + 1] += w * b.y;
-              o[i][4 * j + 2] += w * b.z;
-              o[i][4 * j + 3] += w * b.w;
-            }
+          for (int i = 0; i < 4; i++) {
+            const float w = cc == 0 ? a[i].x : cc == 1 ? a[i].y : cc == 2 ? a[i].z : a[i].w;
+            o[i][j].x += w * b.x;
+            o[i][j].y += w * b.y;
           }
-      }
+        }
     }
   }
 #pragma unroll
   for (int i = 0; i < 4; i++) {
+#pragma unroll
+    for (int w = 8; w >= 1; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
     const int r = ty * 4 + i;
     if (r >= rows) continue;
     T* ob = static_cast<T*>(p.out) + (int64_t)(sq.q0 + i0 + r) * p.o_token + (int64_t)h * p.o_head;
-    const float inv = l[i] > 0.f ? 1.0f / l[i] : l[i];  // 0 for an empty row, NaN kept
+    const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];  // 0 for an empty row
 #pragma unroll
-    for (int j = 0; j < OJ * 4; j++) {
-      const int d = tx * 4 + 64 * (j >> 2) + (j & 3);
-      if (d < D) ob[d] = from_f32<T>(l[i] == 0.f ? 0.f : o[i][j] * inv);
+    for (int j = 0; j < OJ; j++) {
+      const int d = tx * 2 + 32 * j;
+      if (d < D) ob[d] = from_f32<T>(o[i][j].x * inv);
+      if (d + 1 < D) ob[d + 1] = from_f32<T>(o[i][j].y * inv);
     }
   }
 }
 
 template <typename T, int DM>
-int ws_launch(const WaParams& p, cudaStream_t s) {
+int ws_launch(const WaParams& p, int vec, cudaStream_t s) {
   ARMAI_CUDA(cudaFuncSetAttribute(k_wa_simt<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ws_smem<DM>()));
   const dim3 grid((unsigned)((p.max_q + WS_Q - 1) / WS_Q), (unsigned)p.n_q_heads, (unsigned)p.n_seq);
-  k_wa_simt<T, DM><<<grid, WS_THREADS, ws_smem<DM>(), s>>>(p);
+  k_wa_simt<T, DM><<<grid, WS_THREADS, ws_smem<DM>(), s>>>(p, vec);
   ARMAI_CUDA(cudaGetLastError());
   return ARMAI_OK;
 }
 template <typename T>
-int ws_dim(const WaParams& p, cudaStream_t s) {
-  return p.head_dim <= 64 ? ws_launch<T, 64>(p, s) : p.head_dim <= 128 ? ws_launch<T, 128>(p, s) : ws_launch<T, 256>(p, s);
+int ws_dim(const WaParams& p, int vec, cudaStream_t s) {
+  if (p.head_dim <= 64) return ws_launch<T, 64>(p, vec, s);
+  if (p.head_dim <= 96) return ws_launch<T, 96>(p, vec, s);
+  return p.head_dim <= 128 ? ws_launch<T, 128>(p, vec, s) : ws_launch<T, 256>(p, vec, s);
 }
 
 }  // namespace
@@ -186,9 +202,9 @@ bool wa_vectors(const WaParams& p, int dtype) {
 }
 
 int wa_simt_launch(const WaParams& p, int dtype, cudaStream_t s) {
-  if (dtype == ARMAI_F32) return ws_dim<float>(p, s);
-  if (dtype == ARMAI_F16) return ws_dim<__half>(p, s);
-  return ws_dim<__nv_bfloat16>(p, s);
+  if (dtype == ARMAI_F32) return ws_dim<float>(p, wa_vectors(p, dtype) && p.head_dim % 4 == 0, s);
+  if (dtype == ARMAI_F16) return ws_dim<__half>(p, 0, s);
+  return ws_dim<__nv_bfloat16>(p, 0, s);
 }
 
 }  // namespace armai
