@@ -27,6 +27,16 @@ constexpr size_t ws_smem() {
   return ((size_t)3 * WS_Q * (DM + 4) + WS_Q * WS_PP) * 4;
 }
 
+// Two f32 products and sums per instruction.
+__device__ __forceinline__ void ws_fma2(float2& c, float2 a, float2 b) {
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%0, %1};\n\t"
+      "fma.rn.f32x2 z, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "+f"(c.x), "+f"(c.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+}
+
 // n rows of head_dim values into shared rows of DM f32 (zeros behind them);
 // `vec`: f32 rows of whole 16-byte vectors, copied asynchronously.
 template <typename T, int DM>
@@ -91,10 +101,11 @@ __global__ void __launch_bounds__(WS_THREADS, DM <= 96 ? 2 : 1) k_wa_simt(const 
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     float acc[4][4];
+    float2 part[4][4];  // of even and of odd values
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-      for (int j = 0; j < 4; j++) acc[i][j] = 0.f;
+      for (int j = 0; j < 4; j++) part[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 2
     for (int d = 0; d < DM; d += 4) {
       float4 a[4], b[4];
@@ -105,8 +116,10 @@ __global__ void __launch_bounds__(WS_THREADS, DM <= 96 ? 2 : 1) k_wa_simt(const 
 #pragma unroll
       for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          acc[i][j] += a[i].x * b[j].x + a[i].y * b[j].y + a[i].z * b[j].z + a[i].w * b[j].w;
+        for (int j = 0; j < 4; j++) {
+          ws_fma2(part[i][j], make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y));
+          ws_fma2(part[i][j], make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w));
+        }
     }
     const bool full = x.n == WS_K && x.pos + WS_K - 1 <= qlo && (qhi - x.pos < p.window || x.pos + WS_K - 1 < p.n_sink);
 #pragma unroll
@@ -115,7 +128,7 @@ __global__ void __launch_bounds__(WS_THREADS, DM <= 96 ? 2 : 1) k_wa_simt(const 
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const int kk = tx + 16 * j;
-        acc[i][j] *= p.scale_log2;
+        acc[i][j] = (part[i][j].x + part[i][j].y) * p.scale_log2;
         if (!full && (kk >= x.n || !wa_sees(p, qpos0 + i, x.pos + kk))) acc[i][j] = -INFINITY;
         mt = fmaxf(mt, acc[i][j]);
       }
@@ -152,8 +165,7 @@ __global__ void __launch_bounds__(WS_THREADS, DM <= 96 ? 2 : 1) k_wa_simt(const 
 #pragma unroll
           for (int i = 0; i < 4; i++) {
             const float w = cc == 0 ? a[i].x : cc == 1 ? a[i].y : cc == 2 ? a[i].z : a[i].w;
-            o[i][j].x += w * b.x;
-            o[i][j].y += w * b.y;
+            ws_fma2(o[i][j], make_float2(w, w), b);
           }
         }
     }
