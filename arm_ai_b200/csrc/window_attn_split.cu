@@ -128,19 +128,46 @@ struct SpCursor {
   __device__ __forceinline__ int keys() const { return min(KT, len - off); }
 };
 
-// Joins the warps' parts ([warp][R] maxima and sums, [warp][R][DT] outputs in
-// shared memory, outputs unnormalised) within the CTA, then over the cluster,
-// and writes the rows. Every rank writes a share of the values.
+__device__ __forceinline__ void sp_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sp_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// What the ranks of a cluster send one another: the outputs of the values
+// (rows x DT / 4 vectors) that a rank joins, from every rank, and all rows'
+// maxima and sums. Behind the ring, which may still be in use.
+template <int R, int DT>
+struct SpMail {
+  float4 o[R * DT / 4 + SP_MAX_SPLIT];
+  float2 s[SP_MAX_SPLIT][R];
+};
+
+// Joins the warps' parts ([warp][R][DT] unnormalised outputs, [warp][R] maxima
+// and sums in shared memory) within the CTA, then over the cluster, and writes
+// the rows. Every rank joins a share of the values; the others send it theirs
+// (remote stores: no latency to wait for). The caller has arrived at the
+// cluster's barrier before, so that every rank's mail box is there.
 template <typename T, int R, int DT>
-__device__ __forceinline__ void sp_join(const WaParams& p, const SpBlock& b, float* part, float* wm, float* wl) {
-  // part: [SP_WARPS][R][DT], wm / wl: [SP_WARPS][R]; the CTA's own result replaces warp 0's
-  const int tid = threadIdx.x;
+__device__ __forceinline__ void sp_join(const WaParams& p, const SpBlock& b, const float* part, const float* wm,
+                                        const float* wl, SpMail<R, DT>* mail) {
+  const int tid = threadIdx.x, items = b.nr * (DT / 4);
+  const int ranks = (int)gridDim.x, rank = (int)blockIdx.x, per = (items + ranks - 1) / ranks;
+  auto write = [&](int r, int d, const float4& acc, float l) {
+    if (d >= p.head_dim) return;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;  // an empty row: 0 * 0; NaN kept
+    const int f = b.f0 + r;
+    T* o = static_cast<T*>(p.out) + (int64_t)(b.sq.q0 + f / p.group) * p.o_token +
+           (int64_t)(b.kvh * p.group + f % p.group) * p.o_head + d;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(o) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    } else {
+      *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+    }
+  };
   cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = (int)gridDim.x, rank = (int)blockIdx.x;
   __syncthreads();
-  for (int e = tid; e < b.nr * (DT / 4); e += SP_THREADS) {
+  if (ranks > 1) sp_cluster_wait();
+  for (int e = tid; e < items; e += SP_THREADS) {
     const int r = e / (DT / 4), d = (e % (DT / 4)) * 4;
-    float m = wm[r];
+    float m = wm[r], l = 0.f;
 #pragma unroll
     for (int w = 1; w < SP_WARPS; w++) m = fmaxf(m, wm[w * R + r]);
     const float base = m == -INFINITY ? 0.f : m;
@@ -149,61 +176,43 @@ __device__ __forceinline__ void sp_join(const WaParams& p, const SpBlock& b, flo
     for (int w = 0; w < SP_WARPS; w++) {
       const float f = sp_exp2(wm[w * R + r] - base);
       const float4 v = *reinterpret_cast<const float4*>(part + (w * R + r) * DT + d);
+      l += f * wl[w * R + r];
       acc.x += f * v.x;
       acc.y += f * v.y;
       acc.z += f * v.z;
       acc.w += f * v.w;
     }
-    *reinterpret_cast<float4*>(part + r * DT + d) = acc;
-  }
-  __syncthreads();
-  if (tid < b.nr) {
-    float m = wm[tid], l = 0.f;
-#pragma unroll
-    for (int w = 1; w < SP_WARPS; w++) m = fmaxf(m, wm[w * R + tid]);
-    const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int w = 0; w < SP_WARPS; w++) l += sp_exp2(wm[w * R + tid] - base) * wl[w * R + tid];
-    wm[tid] = m;
-    wl[tid] = l;
-  }
-  if (ranks > 1) cluster.sync(); else __syncthreads();
-  for (int e = rank * SP_THREADS + tid; e < b.nr * (DT / 4); e += ranks * SP_THREADS) {
-    const int r = e / (DT / 4), d = (e % (DT / 4)) * 4;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
     if (ranks == 1) {
-      acc = *reinterpret_cast<const float4*>(part + r * DT + d);
-      l = wl[r];
+      write(r, d, acc, l);
     } else {
-      float m = -INFINITY;
-#pragma unroll 4
-      for (int k = 0; k < ranks; k++) m = fmaxf(m, *cluster.map_shared_rank(wm + r, k));
-      const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-      for (int k = 0; k < ranks; k++) {
-        const float f = sp_exp2(*cluster.map_shared_rank(wm + r, k) - base);
-        l += f * *cluster.map_shared_rank(wl + r, k);
-        const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part + r * DT + d, k));
-        acc.x += f * v.x;
-        acc.y += f * v.y;
-        acc.z += f * v.z;
-        acc.w += f * v.w;
-      }
-    }
-    if (d < p.head_dim) {
-      const float inv = l == 0.f ? 0.f : 1.0f / l;  // an empty row: 0 * 0; NaN kept
-      const int f = b.f0 + r;
-      T* o = static_cast<T*>(p.out) + (int64_t)(b.sq.q0 + f / p.group) * p.o_token +
-             (int64_t)(b.kvh * p.group + f % p.group) * p.o_head + d;
-      if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4*>(o) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-      } else {
-        *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-      }
+      const int owner = e / per;
+      *cluster.map_shared_rank(&mail->o[rank * per + e - owner * per], owner) = acc;
+      if (d / 4 < ranks) *cluster.map_shared_rank(&mail->s[rank][r], d / 4) = make_float2(m, l);  // DT / 4 >= 8 ranks
+      if (DT / 4 < SP_MAX_SPLIT && d / 4 + DT / 4 < ranks)
+        *cluster.map_shared_rank(&mail->s[rank][r], d / 4 + DT / 4) = make_float2(m, l);
     }
   }
-  if (ranks > 1) cluster.sync();  // the others still read this CTA's part
+  if (ranks == 1) return;
+  sp_cluster_arrive();
+  sp_cluster_wait();
+  for (int e = rank * per + tid; e < min(items, (rank + 1) * per); e += SP_THREADS) {
+    const int r = e / (DT / 4), i = e - rank * per;
+    float m = -INFINITY, l = 0.f;
+    for (int k = 0; k < ranks; k++) m = fmaxf(m, mail->s[k][r].x);
+    const float base = m == -INFINITY ? 0.f : m;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < ranks; k++) {
+      const float2 st = mail->s[k][r];
+      const float4 v = mail->o[k * per + i];
+      const float f = sp_exp2(st.x - base);
+      l += f * st.y;
+      acc.x += f * v.x;
+      acc.y += f * v.y;
+      acc.z += f * v.z;
+      acc.w += f * v.w;
+    }
+    write(r, (e % (DT / 4)) * 4, acc, l);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -223,10 +232,10 @@ __device__ __forceinline__ int sp_swz_k(int key) { return (key & 1) << 2; }
 __device__ __forceinline__ int sp_swz_v(int key) { return key & 6; }
 
 template <typename T, int DT>
-constexpr size_t sp_smem() {
+__host__ __device__ constexpr size_t sp_smem() {
   const size_t ring = (size_t)SP_WARPS * SP_STAGES * 2 * SP_KT * DT * 2;
   const size_t join = (size_t)SP_WARPS * SP_ROWS * (DT + 2) * 4;
-  return ring > join ? ring : join;
+  return ring > join ? ring : join;  // one after the other
 }
 
 template <typename T, int DT>
@@ -237,6 +246,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   SpBlock b;
   if (!sp_block<SP_ROWS>(p, b)) return;
+  if (gridDim.x > 1) sp_cluster_arrive();
   const int chunks = p.head_dim >> 3;             // valid 16-byte chunks of a row
   const bool whole = p.head_dim == DT;
   // copies: 16-byte chunk cc of key ck + RPC i, consecutive lanes consecutive
@@ -426,7 +436,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
           *reinterpret_cast<float4*>(part + (warp * SP_ROWS + r) * DT + 64 * i + 16 * c + 8 * n + e) =
               make_float4(o[i][e][2 * j + n], o[i][e + 1][2 * j + n], o[i][e + 2][2 * j + n], o[i][e + 3][2 * j + n]);
   }
-  sp_join<T, SP_ROWS, DT>(p, b, part, wm, wl);
+  sp_join<T, SP_ROWS, DT>(p, b, part, wm, wl, reinterpret_cast<SpMail<SP_ROWS, DT>*>(sm + sp_smem<T, DT>()));
 }
 
 // ---------------------------------------------------------------------------
@@ -438,10 +448,10 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
 constexpr int SF_KT = 8;
 
 template <int CH>
-constexpr size_t sf_smem(int rows) {
+__host__ __device__ constexpr size_t sf_smem(int rows) {
   const size_t ring = (size_t)SP_WARPS * SP_STAGES * 2 * SF_KT * CH * 32 * 4;
   const size_t join = (size_t)SP_WARPS * rows * (CH * 32 + 2) * 4;
-  return ring > join ? ring : join;
+  return ring > join ? ring : join;  // one after the other
 }
 
 template <int R, int CH>
@@ -452,6 +462,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kg = lane >> 3, x8 = lane & 7;
   SpBlock b;
   if (!sp_block<R>(p, b)) return;
+  if (gridDim.x > 1) sp_cluster_arrive();
   const int chunks = p.head_dim >> 2;
   const int64_t kv_off = (int64_t)b.sq.slot * p.kv_slot + (int64_t)b.kvh * p.kv_head;
   const float* kb = static_cast<const float*>(p.k) + kv_off;
@@ -604,7 +615,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
       }
       if (kg == 0) *reinterpret_cast<float4*>(part + (warp * R + r) * DT + 4 * (x8 + 8 * i)) = v;
     }
-  sp_join<float, R, DT>(p, b, part, wm, wl);
+  sp_join<float, R, DT>(p, b, part, wm, wl, reinterpret_cast<SpMail<R, DT>*>(sm + sf_smem<CH>(R)));
 }
 
 // Splits of one sequence and head: up to three CTAs per SM (what their rings
@@ -646,14 +657,14 @@ int sp_launch(K kernel, size_t smem, const WaParams& p, int rows, int kt, cudaSt
 
 template <typename T>
 int sp_half(const WaParams& p, cudaStream_t s) {
-  if (p.head_dim <= 64) return sp_launch(k_wa_split<T, 64>, sp_smem<T, 64>(), p, SP_ROWS, SP_KT, s);
-  if (p.head_dim <= 128) return sp_launch(k_wa_split<T, 128>, sp_smem<T, 128>(), p, SP_ROWS, SP_KT, s);
-  return sp_launch(k_wa_split<T, 256>, sp_smem<T, 256>(), p, SP_ROWS, SP_KT, s);
+  if (p.head_dim <= 64) return sp_launch(k_wa_split<T, 64>, sp_smem<T, 64>() + sizeof(SpMail<SP_ROWS, 64>), p, SP_ROWS, SP_KT, s);
+  if (p.head_dim <= 128) return sp_launch(k_wa_split<T, 128>, sp_smem<T, 128>() + sizeof(SpMail<SP_ROWS, 128>), p, SP_ROWS, SP_KT, s);
+  return sp_launch(k_wa_split<T, 256>, sp_smem<T, 256>() + sizeof(SpMail<SP_ROWS, 256>), p, SP_ROWS, SP_KT, s);
 }
 
 template <int R, int CH>
 int sp_f32(const WaParams& p, cudaStream_t s) {
-  return sp_launch(k_wa_split_f32<R, CH>, sf_smem<CH>(R), p, R, SF_KT, s);
+  return sp_launch(k_wa_split_f32<R, CH>, sf_smem<CH>(R) + sizeof(SpMail<R, 32 * CH>), p, R, SF_KT, s);
 }
 // Rows per CTA as many as there are, up to eight; four at the widths where
 // eight rows of q and of the output would not fit the registers.
