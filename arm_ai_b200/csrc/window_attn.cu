@@ -274,6 +274,8 @@ extern "C" int armai_dev_window_attention(const armai_window_attention_args* a, 
   p.n_tokens = (int)a->n_tokens;
   p.n_q_heads = (int)a->n_q_heads;
   p.group = (int)(a->n_q_heads / a->n_kv_heads);
+  p.n_kv = (int)a->n_kv_heads;
+  p.group_mul = (uint32_t)(((1ull << 32) + p.group - 1) / p.group);
   p.head_dim = (int)a->head_dim;
   p.n_slots = (int)a->n_slots;
   p.kv_rows = (int)a->kv_rows;

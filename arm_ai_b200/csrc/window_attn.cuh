@@ -25,9 +25,17 @@ struct WaParams {
   int64_t kv_slot, kv_head, kv_row;
   int n_seq, max_q, n_tokens, n_q_heads, group, head_dim, n_slots, kv_rows;
   int window, n_sink, ring;  // ring: rows of the ring, 0 for a linear cache
+  int n_kv;                  // key / value heads
+  uint32_t group_mul;        // ceil(2^32 / group), see wa_token
   float scale_log2;          // scale * log2(e): the kernels use exp2
   uint32_t* err;             // bounded waits that ran out
 };
+
+// Token of (token, query head of the group) pair f, exact for f < 2^16: a
+// product instead of a division.
+__device__ __forceinline__ int wa_token(const WaParams& p, int f) {
+  return p.group == 1 ? f : (int)__umulhi((uint32_t)f, p.group_mul);
+}
 
 // A sequence's queries: rows q0 .. q0 + n - 1 of q, the i-th at position
 // pos0 + i.

@@ -86,17 +86,21 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uin
 struct SpBlock {
   WaSeq sq;
   int kvh, f0, nr;
+  int qmin, qmax;  // positions of its first and last token
   WaRuns runs;
 };
 template <int R>
 __device__ __forceinline__ bool sp_block(const WaParams& p, SpBlock& b) {
-  const int n_kv = p.n_q_heads / p.group;
-  b.kvh = blockIdx.y % n_kv;
-  b.f0 = (blockIdx.y / n_kv) * R;
+  // blockIdx.y: key / value head, then block of rows (one, for single tokens)
+  const int rb = (int)gridDim.y == p.n_kv ? 0 : (int)blockIdx.y / p.n_kv;
+  b.kvh = (int)blockIdx.y - rb * p.n_kv;
+  b.f0 = rb * R;
   b.sq = wa_seq(p, blockIdx.z);
   b.nr = min(R, b.sq.n * p.group - b.f0);
   if (b.nr <= 0) return false;  // the same for the whole cluster
-  b.runs = wa_runs(p, b.sq.pos0 + b.f0 / p.group, b.sq.pos0 + (b.f0 + b.nr - 1) / p.group);
+  b.qmin = b.sq.pos0 + wa_token(p, b.f0);
+  b.qmax = b.sq.pos0 + wa_token(p, b.f0 + b.nr - 1);
+  b.runs = wa_runs(p, b.qmin, b.qmax);
   return true;
 }
 
@@ -153,9 +157,9 @@ __device__ __forceinline__ void sp_join(const WaParams& p, const SpBlock& b, con
   auto write = [&](int r, int d, const float4& acc, float l) {
     if (d >= p.head_dim) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;  // an empty row: 0 * 0; NaN kept
-    const int f = b.f0 + r;
-    T* o = static_cast<T*>(p.out) + (int64_t)(b.sq.q0 + f / p.group) * p.o_token +
-           (int64_t)(b.kvh * p.group + f % p.group) * p.o_head + d;
+    const int f = b.f0 + r, tok = wa_token(p, f);
+    T* o = static_cast<T*>(p.out) + (int64_t)(b.sq.q0 + tok) * p.o_token +
+           (int64_t)(b.kvh * p.group + f - tok * p.group) * p.o_head + d;
     if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<float4*>(o) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     } else {
@@ -302,9 +306,10 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
 #pragma unroll
   for (int j = 0; j < 2; j++) {
     const int r = g + 8 * j, f = b.f0 + (r < b.nr ? r : 0);
-    qpos[j] = b.sq.pos0 + f / p.group;
-    const T* src = static_cast<const T*>(p.q) + (int64_t)(b.sq.q0 + f / p.group) * p.q_token +
-                   (int64_t)(b.kvh * p.group + f % p.group) * p.q_head;
+    const int tok = wa_token(p, f);
+    qpos[j] = b.sq.pos0 + tok;
+    const T* src = static_cast<const T*>(p.q) + (int64_t)(b.sq.q0 + tok) * p.q_token +
+                   (int64_t)(b.kvh * p.group + f - tok * p.group) * p.q_head;
 #pragma unroll
     for (int i = 0; i < KC; i++) {
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -315,7 +320,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
       qa[i][1][2 + j] = v.w ^ flip;
     }
   }
-  const int qmin = b.sq.pos0 + b.f0 / p.group, qmax = b.sq.pos0 + (b.f0 + b.nr - 1) / p.group;
+  const int qmin = b.qmin, qmax = b.qmax;
 
   float o[VB][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -496,8 +501,9 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
 #pragma unroll
   for (int r = 0; r < R; r++) {
     const int f = b.f0 + (r < b.nr ? r : 0);
-    const float* src = static_cast<const float*>(p.q) + (int64_t)(b.sq.q0 + f / p.group) * p.q_token +
-                       (int64_t)(b.kvh * p.group + f % p.group) * p.q_head;
+    const int tok = wa_token(p, f);
+    const float* src = static_cast<const float*>(p.q) + (int64_t)(b.sq.q0 + tok) * p.q_token +
+                       (int64_t)(b.kvh * p.group + f - tok * p.group) * p.q_head;
 #pragma unroll
     for (int i = 0; i < CH; i++) {
       o[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -509,7 +515,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
     }
   }
   const int mine = x8 >> SH;  // the row whose scores this lane ends with
-  const int qpos = b.sq.pos0 + (b.f0 + min(mine, b.nr - 1)) / p.group;
+  const int qpos = b.sq.pos0 + wa_token(p, b.f0 + min(mine, b.nr - 1));
   float m = -INFINITY, l = 0.f;
 
   int slot = 0;
@@ -633,7 +639,7 @@ int sp_split(int64_t blocks, int64_t keys, int kt) {
 template <typename K>
 int sp_launch(K kernel, size_t smem, const WaParams& p, int rows, int kt, cudaStream_t s) {
   const int64_t pairs = (int64_t)p.max_q * p.group, rb = (pairs + rows - 1) / rows;
-  const int64_t blocks = rb * (p.n_q_heads / p.group);
+  const int64_t blocks = rb * p.n_kv;
   const int64_t span = std::min<int64_t>(p.max_q, (rows + p.group - 1) / p.group + 1);
   const int64_t keys = std::min<int64_t>(p.kv_rows, (int64_t)p.window + p.n_sink + span);
   const int split = sp_split(blocks * p.n_seq, keys, kt);
@@ -685,7 +691,7 @@ int sp_f32_rows(const WaParams& p, cudaStream_t s) {
 bool wa_split_fits(const WaParams& p, int dtype) {
   const int es = dtype_size(dtype), v = 16 / es;
   return p.head_dim % v == 0 && p.scale_log2 != 0.f && p.scale_log2 == p.scale_log2 && (dtype != ARMAI_F32 || p.head_dim <= 128) &&
-         ((int64_t)p.max_q * p.group + 3) / 4 * (p.n_q_heads / p.group) <= 65535;
+         (int64_t)p.max_q * p.group < 65536 && ((int64_t)p.max_q * p.group + 3) / 4 * p.n_kv <= 65535;
 }
 
 int wa_split_launch(const WaParams& p, int dtype, cudaStream_t s) {
