@@ -213,6 +213,32 @@ bool wa_vectors(const WaParams& p, int dtype) {
          ok(p.kv_row);
 }
 
+namespace {
+
+// Whether the split form is the faster one. It reads the keys once for each
+// block of 16 rows (16-bit types) and never waits for full tiles of queries.
+// 16-bit: with one block of rows always (32 streams of one token, window 512,
+// 8 heads of 128: 15 us against 24 in tiles of 256 rows); with more as long as
+// its reads stay below 80 MB (4096 keys x 8 heads of 128: 64 rows 16.1 against
+// 15.2 us, 128 rows 24.6 against 15.2, 32 rows 13.6 against 15.4; 8 streams of
+// 2048 keys: 32 rows 25.6 against 28.3, 64 rows 41 against 28.5).
+// f32: a row costs it what 1.8 rows of a full 64-row tile cost on the CUDA
+// cores, whose CTAs fill the SMs one by one: as long as there are fewer than 36
+// rows per SM for each round of tiles (8 streams of 2048 keys, 8 heads of 128:
+// 64 rows 250 against 308 us, 128 rows 476 against 308).
+bool wa_split_better(const WaParams& p, int dtype) {
+  const int64_t pairs = (int64_t)p.max_q * p.group, heads = (int64_t)p.n_seq * p.n_kv;
+  if (dtype != ARMAI_F32) {
+    const int64_t keys = std::min<int64_t>(p.kv_rows, (int64_t)p.window + p.n_sink + p.max_q);
+    return pairs <= 16 || heads * ((pairs + 15) / 16) * keys * 4 * p.head_dim <= 80 * 1000 * 1000;
+  }
+  const int64_t r = p.head_dim <= 64 ? 8 : 4, rows = heads * ((pairs + r - 1) / r) * r;
+  const int64_t tiles = (int64_t)p.n_seq * p.n_q_heads * ((p.max_q + WS_Q - 1) / WS_Q), sms = sm_count();
+  return rows <= 36 * sms * ((tiles + sms - 1) / sms);
+}
+
+}  // namespace
+
 int wa_simt_launch(const WaParams& p, int dtype, cudaStream_t s) {
   if (dtype == ARMAI_F32) return ws_dim<float>(p, wa_vectors(p, dtype) && p.head_dim % 4 == 0, s);
   if (dtype == ARMAI_F16) return ws_dim<__half>(p, 0, s);
@@ -284,9 +310,8 @@ extern "C" int armai_dev_window_attention(const armai_window_attention_args* a, 
   p.ring = a->ring ? (int)(a->kv_rows - sink) : 0;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   const cudaStream_t s = (cudaStream_t)stream;
-  // Few query rows per key / value head: bound by the keys, split over the device.
   if (wa_vectors(p, a->dtype)) {
-    if (wa_split_fits(p, a->dtype) && (int64_t)p.max_q * p.group <= 64) return wa_split_launch(p, a->dtype, s);
+    if (wa_split_fits(p, a->dtype) && wa_split_better(p, a->dtype)) return wa_split_launch(p, a->dtype, s);
     bool fits = false;
     ARMAI_TRY(wa_tc_launch(p, a->dtype, s, &fits));
     if (fits) return ARMAI_OK;

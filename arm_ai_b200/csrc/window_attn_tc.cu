@@ -58,7 +58,10 @@ struct WtLayout {
   static constexpr int SLOTS = 4;
   static constexpr uint32_t K0 = 2 * Q, RING = K0 + 2 * KV;
   static constexpr uint32_t BAR = RING + SLOTS * 2 * KV;
-  static constexpr uint32_t SMEM = 1024 + BAR + 512;
+  // More than half of the SM's, so that two CTAs never share one: the second
+  // would wait for tensor memory, and in a cluster the first for the second's
+  // other ranks.
+  static constexpr uint32_t SMEM = 1024 + BAR + 512 > 116u * 1024 ? 1024 + BAR + 512 : 116u * 1024;
 };
 
 // tcgen05.ld / st of 32 columns of this warp's 32 lanes; the caller waits.
