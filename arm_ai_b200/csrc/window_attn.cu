@@ -19,12 +19,15 @@
 namespace armai {
 namespace {
 
-constexpr int WS_Q = 64, WS_K = 64, WS_THREADS = 256;
+constexpr int WS_K = 64;        // keys per tile; queries: Q, 64 or 32, with 4 Q threads
+#ifndef WSX
+#define WSX 4
+#endif
 constexpr int WS_PP = WS_K + 4;  // row of P, padded
 
-template <int DM>
+template <int DM, int Q>
 constexpr size_t ws_smem() {
-  return ((size_t)3 * WS_Q * (DM + 4) + WS_Q * WS_PP) * 4;
+  return ((size_t)(Q + 2 * WS_K) * (DM + 4) + Q * WS_PP) * 4;
 }
 
 // Two f32 products and sums per instruction.
@@ -39,11 +42,11 @@ __device__ __forceinline__ void ws_fma2(float2& c, float2 a, float2 b) {
 
 // n rows of head_dim values into shared rows of DM f32 (zeros behind them);
 // `vec`: f32 rows of whole 16-byte vectors, copied asynchronously.
-template <typename T, int DM>
+template <typename T, int DM, int ROWS, int THREADS>
 __device__ __forceinline__ void ws_rows(float* dst, const T* src, int64_t stride, int n, int D, bool vec) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (sizeof(T) == 4 && vec) {
-    for (int e = threadIdx.x; e < 64 * (DM / 4); e += WS_THREADS) {
+    for (int e = threadIdx.x; e < ROWS * (DM / 4); e += THREADS) {
       const int r = e / (DM / 4), d = e % (DM / 4) * 4;
       const bool ok = r < n && d < D;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
@@ -53,30 +56,30 @@ __device__ __forceinline__ void ws_rows(float* dst, const T* src, int64_t stride
     }
     return;
   }
-  for (int r = warp; r < 64; r += WS_THREADS / 32)
+  for (int r = warp; r < ROWS; r += THREADS / 32)
     for (int d = lane; d < DM; d += 32) dst[r * (DM + 4) + d] = r < n && d < D ? to_f32(src[r * stride + d]) : 0.f;
 }
 
-template <typename T, int DM>
-__global__ void __launch_bounds__(WS_THREADS, DM <= 96 ? 2 : 1) k_wa_simt(const WaParams p, int vec) {
+template <typename T, int DM, int Q>
+__global__ void __launch_bounds__(4 * Q, DM > 96 ? 1 : Q == 64 ? 2 : 3) k_wa_simt(const WaParams p, int vec) {
   constexpr int DP = DM + 4;
   constexpr int OJ = DM / 32;  // pairs of output columns per thread: 2 tx + 32 j
   extern __shared__ __align__(16) float ws[];
   float* Qs = ws;
-  float* Ks = Qs + WS_Q * DP;
+  float* Ks = Qs + Q * DP;
   float* Vs = Ks + WS_K * DP;
   float* Ps = Vs + WS_K * DP;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int h = blockIdx.y;
   const WaSeq sq = wa_seq(p, blockIdx.z);
-  const int i0 = blockIdx.x * WS_Q;
+  const int i0 = blockIdx.x * Q;
   if (i0 >= sq.n) return;
-  const int rows = min(WS_Q, sq.n - i0);
+  const int rows = min(Q, sq.n - i0);
   const int64_t kv_off = (int64_t)sq.slot * p.kv_slot + (int64_t)(h / p.group) * p.kv_head;
   const T* kb = static_cast<const T*>(p.k) + kv_off;
   const T* vb = static_cast<const T*>(p.v) + kv_off;
   const int D = p.head_dim;
-  ws_rows<T, DM>(Qs, static_cast<const T*>(p.q) + (int64_t)(sq.q0 + i0) * p.q_token + (int64_t)h * p.q_head, p.q_token,
+  ws_rows<T, DM, Q, 4 * Q>(Qs, static_cast<const T*>(p.q) + (int64_t)(sq.q0 + i0) * p.q_token + (int64_t)h * p.q_head, p.q_token,
                  rows, D, vec);
 
   float m[4], l[4];
@@ -91,13 +94,13 @@ __global__ void __launch_bounds__(WS_THREADS, DM <= 96 ? 2 : 1) k_wa_simt(const 
   const int qpos0 = sq.pos0 + i0 + ty * 4;  // of this thread's first query
   const int qlo = sq.pos0 + i0, qhi = qlo + rows - 1;
   const WaRuns runs = wa_runs(p, qlo, qhi);
-  const int nt = wa_tiles<WS_K>(runs);
+  const int nt = wa_tiles<WS_K>(runs), dq = (D + 3) & ~3;
 #pragma unroll 1
   for (int t = 0; t < nt; t++) {
     const WaTile x = wa_tile<WS_K>(runs, t);
     __syncthreads();
-    ws_rows<T, DM>(Ks, kb + (int64_t)x.row * p.kv_row, p.kv_row, x.n, D, vec);
-    ws_rows<T, DM>(Vs, vb + (int64_t)x.row * p.kv_row, p.kv_row, x.n, D, vec);
+    ws_rows<T, DM, WS_K, 4 * Q>(Ks, kb + (int64_t)x.row * p.kv_row, p.kv_row, x.n, D, vec);
+    ws_rows<T, DM, WS_K, 4 * Q>(Vs, vb + (int64_t)x.row * p.kv_row, p.kv_row, x.n, D, vec);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     float acc[4][4];
@@ -107,7 +110,7 @@ __global__ void __launch_bounds__(WS_THREADS, DM <= 96 ? 2 : 1) k_wa_simt(const 
 #pragma unroll
       for (int j = 0; j < 4; j++) part[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 2
-    for (int d = 0; d < DM; d += 4) {
+    for (int d = 0; d < dq; d += 4) {
       float4 a[4], b[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) a[i] = *reinterpret_cast<const float4*>(Qs + (ty * 4 + i) * DP + d);
@@ -187,19 +190,26 @@ __global__ void __launch_bounds__(WS_THREADS, DM <= 96 ? 2 : 1) k_wa_simt(const 
   }
 }
 
-template <typename T, int DM>
+template <typename T, int DM, int Q>
 int ws_launch(const WaParams& p, int vec, cudaStream_t s) {
-  ARMAI_CUDA(cudaFuncSetAttribute(k_wa_simt<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ws_smem<DM>()));
-  const dim3 grid((unsigned)((p.max_q + WS_Q - 1) / WS_Q), (unsigned)p.n_q_heads, (unsigned)p.n_seq);
-  k_wa_simt<T, DM><<<grid, WS_THREADS, ws_smem<DM>(), s>>>(p, vec);
+  constexpr size_t smem = ws_smem<DM, Q>();
+  ARMAI_CUDA(cudaFuncSetAttribute(k_wa_simt<T, DM, Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const dim3 grid((unsigned)((p.max_q + Q - 1) / Q), (unsigned)p.n_q_heads, (unsigned)p.n_seq);
+  k_wa_simt<T, DM, Q><<<grid, 4 * Q, smem, s>>>(p, vec);
   ARMAI_CUDA(cudaGetLastError());
   return ARMAI_OK;
 }
+// 32 queries per CTA where 64 would leave the SMs unevenly filled.
+template <typename T, int DM>
+int ws_rows_per_cta(const WaParams& p, int vec, cudaStream_t s) {
+  const int64_t ctas = (int64_t)p.n_seq * p.n_q_heads * ((p.max_q + 63) / 64);
+  return ctas > WSX * (int64_t)sm_count() ? ws_launch<T, DM, 64>(p, vec, s) : ws_launch<T, DM, 32>(p, vec, s);
+}
 template <typename T>
 int ws_dim(const WaParams& p, int vec, cudaStream_t s) {
-  if (p.head_dim <= 64) return ws_launch<T, 64>(p, vec, s);
-  if (p.head_dim <= 96) return ws_launch<T, 96>(p, vec, s);
-  return p.head_dim <= 128 ? ws_launch<T, 128>(p, vec, s) : ws_launch<T, 256>(p, vec, s);
+  if (p.head_dim <= 64) return ws_rows_per_cta<T, 64>(p, vec, s);
+  if (p.head_dim <= 96) return ws_rows_per_cta<T, 96>(p, vec, s);
+  return p.head_dim <= 128 ? ws_rows_per_cta<T, 128>(p, vec, s) : ws_rows_per_cta<T, 256>(p, vec, s);
 }
 
 }  // namespace
@@ -233,7 +243,7 @@ bool wa_split_better(const WaParams& p, int dtype) {
     return pairs <= 16 || heads * ((pairs + 15) / 16) * keys * 4 * p.head_dim <= 80 * 1000 * 1000;
   }
   const int64_t r = p.head_dim <= 64 ? 8 : 4, rows = heads * ((pairs + r - 1) / r) * r;
-  const int64_t tiles = (int64_t)p.n_seq * p.n_q_heads * ((p.max_q + WS_Q - 1) / WS_Q), sms = sm_count();
+  const int64_t tiles = (int64_t)p.n_seq * p.n_q_heads * ((p.max_q + 63) / 64), sms = sm_count();
   return rows <= 36 * sms * ((tiles + sms - 1) / sms);
 }
 
