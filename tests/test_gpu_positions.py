@@ -230,3 +230,46 @@ def test_device_checks_refuse_host_tensors(built):
     a = wr.rope_args(d, d, torch.zeros(1, dtype=torch.int64), torch.zeros(32), "half")
     assert lib.armai_dev_rope(ctypes.byref(a), None) == -1
     assert b"rope: positions is not device memory" in lib.armai_last_error()
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype,dim,rot", [(F32, 64, 32), (BF16, 128, 64), (F16, 128, 20), (F32, 33, 10)])
+def test_infinities_stay_in_their_pair(built, layout, dtype, dim, rot):
+    """An infinity or NaN reaches its own pair (its head, through the norm) and nothing else."""
+    g = gen(30)
+    x = rnd(g, 5, 4, dim, dtype=dtype)
+    x[1, 2, 0], x[2, 1, dim - 1], x[3, 0, 1] = float("inf"), float("-inf"), float("nan")
+    pos, f = torch.arange(5, device="cuda") + 3, freqs(rot)
+    out = torch.empty_like(x)
+    wr.rope(x, out, pos, f, layout)
+    clean = torch.where(torch.isfinite(x.float()), x, 0.0)
+    want = torch.empty_like(x)
+    wr.rope(clean, want, pos, f, layout)
+    partner = {0: 1, 1: 0} if layout == "interleaved" else {0: rot // 2, 1: 1 + rot // 2}
+    touched = torch.zeros(x.shape, dtype=torch.bool, device="cuda")
+    touched[1, 2, 0] = touched[1, 2, partner[0]] = touched[2, 1, dim - 1] = touched[3, 0, 1] = True
+    touched[3, 0, partner[1]] = True
+    assert torch.equal(out[~touched], want[~touched])
+    assert not torch.isfinite(out[touched].float()).any()
+    one = torch.ones(dim, device="cuda")
+    q_out, k_out = torch.empty(5, 2, dim, dtype=dtype, device="cuda"), torch.empty(5, 2, dim, dtype=dtype, device="cuda")
+    wr.qk_norm_rope(x[:, :2], x[:, 2:], None, q_out, k_out, None, one, one, pos, f, None, layout)
+    bad = ~torch.isfinite(x.float()).all(-1)
+    assert torch.isfinite(torch.cat((q_out, k_out), 1)[~bad].float()).all()
+
+
+def test_many_tokens_share_the_warps(built):
+    """More tokens than the device's warps, odd counts: each warp goes through several tokens."""
+    g = gen(31)
+    for tokens, hq, hkv, dim, layout in ((9001, 5, 3, 64, "half"), (3999, 9, 1, 96, "interleaved"), (5000, 2, 2, 256, "half")):
+        qkv = rnd(g, tokens, hq + 2 * hkv, dim, dtype=BF16)
+        gq, gk = 1 + 0.1 * rnd(g, dim), 1 + 0.1 * rnd(g, dim)
+        pos, f = torch.randint(0, 1 << 20, (tokens,), generator=g, device="cuda"), freqs(dim)
+        q_out = torch.empty(tokens, hq, dim, dtype=BF16, device="cuda")
+        k_out, v_out = (torch.empty(tokens, hkv, dim, dtype=BF16, device="cuda") for _ in range(2))
+        q, k, v = qkv.split([hq, hkv, hkv], 1)
+        wr.qk_norm_rope(q, k, v, q_out, k_out, v_out, gq, gk, pos, f, None, layout)
+        for got, x, gam in ((q_out, q, gq), (k_out, k, gk)):
+            exact, size = wr.rotate64(wr.norm64(x, gam, 1e-5), pos, f, layout)
+            rope_close(got, exact, size, more=NORM)
+        assert torch.equal(v_out, v)

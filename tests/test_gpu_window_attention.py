@@ -330,3 +330,148 @@ def test_device_checks_refuse_host_tensors(built):
     a = wr.attn_args(q, k, k, torch.empty_like(q), i32([3]), 4)
     a.n_seq = 0
     check(lib.armai_dev_window_attention(ctypes.byref(a), None))
+
+
+# ---- many queries: more rows than the split form takes (its reads would pass
+# 80 MB, or 36 f32 rows per SM and round of tiles) ---------------------------
+MANY = [
+    ([1, 127, 128, 129, 300], [0, 0, 0, 0, 0], 10000, 0, False),
+    ([300, 5, 513], [0, 0, 0], 70, 4, False),
+    ([257, 64], [100, 1000], 128, 0, False),
+    ([333, 2, 170], [1000, 0, 90], 64, 4, True),
+    ([260], [777], 500, 1, True),
+    ([330, 340], [3, 500], 1, 0, False),
+    ([400], [300], 1, 5, True),
+]
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(BF16, 64, 16, 128), (F16, 64, 16, 64), (BF16, 48, 16, 64), (F16, 48, 8, 128),
+                                            (F16, 64, 16, 96), (BF16, 80, 16, 80), (F16, 64, 32, 8), (F32, 64, 16, 64),
+                                            (F32, 96, 32, 80)])
+@pytest.mark.parametrize("q_lens,past,window,n_sink,ring", MANY)
+def test_many_queries(built, dtype, hq, hkv, d, q_lens, past, window, n_sink, ring):
+    run(gen(sum(q_lens) + d), dtype, hq, hkv, d, q_lens, [a + b for a, b in zip(past, q_lens)], window, n_sink, ring,
+        extra=3)
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(BF16, 32, 8, 128), (F16, 32, 8, 64), (F16, 16, 2, 96)])
+@pytest.mark.parametrize("q_lens,past,window,n_sink,ring", [
+    ([64], [4000], 3000, 4, False),      # eight tiles, the keys divided over clusters
+    ([100, 90, 97], [5000, 1300, 0], 2048, 4, True),
+    ([200], [2500], 1 << 40, 0, False),
+    ([129, 80], [2100, 30], 1000, 3, True),
+])
+def test_chunks_divided_over_clusters(built, dtype, hq, hkv, d, q_lens, past, window, n_sink, ring):
+    out = run(gen(sum(q_lens) + d), dtype, hq, hkv, d, q_lens, [a + b for a, b in zip(past, q_lens)], window, n_sink, ring,
+              extra=1)
+    again = run(gen(sum(q_lens) + d), dtype, hq, hkv, d, q_lens, [a + b for a, b in zip(past, q_lens)], window, n_sink,
+                ring, extra=1)
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64), (F32, 80)])
+def test_many_queries_that_see_nothing(built, dtype, d):
+    """Queries before the first position, a sequence without keys, a slot that does not exist."""
+    q_lens, kv_len, slots = [300, 260, 290, 280], [150, 0, 290, 400], [2, 0, 9, 1]
+    out = run(gen(21), dtype, 64, 16, d, q_lens, kv_len, 50, 2, False, extra=4, slots=slots, n_slots=3)
+    assert (out[:150] == 0).all() and (out[300:850] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64), (F32, 80)])
+def test_many_queries_infinite_keys(built, dtype, d):
+    g = gen(22)
+    q, rows = 300, 500
+    qq = rnd(g, q, 128, d, dtype=dtype).abs()
+    k, v = rnd(g, 1, 32, rows, d, dtype=dtype), rnd(g, 1, 32, rows, d, dtype=dtype)
+    k[0, :, ::3] = float("-inf")
+    out = torch.empty_like(qq)
+    wr.window_attention(qq, k, v, out, i32([rows]), 90, 0, False)
+    finite = torch.arange(rows, device="cuda") % 3 != 0
+    j = torch.arange(rows, device="cuda")
+    for i in range(0, q, 37):
+        p = rows - q + i
+        keep = finite & (j <= p) & (j > p - 90)
+        e, b = wr.attention64(qq[i:i + 1], k[:, :, keep].contiguous(), v[:, :, keep].contiguous(), [1],
+                              [int(keep.sum())], 1000)
+        wr.close(out[i:i + 1], e, b)
+    k.fill_(float("-inf"))
+    wr.window_attention(qq, k, v, out, i32([rows]), 90, 0, False)
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64), (F32, 64)])
+def test_many_queries_growing_scores(built, dtype, d):
+    """The maximum moves from tile to tile, both ways: the output is rescaled many times."""
+    g = gen(23)
+    q, rows = 260, 700
+    for ramp in (torch.linspace(0.05, 6.0, rows), torch.linspace(6.0, 0.05, rows)):
+        qq = rnd(g, q, 128, d, dtype=dtype)
+        k = (rnd(g, 1, 32, rows, d) * ramp.cuda()[:, None]).to(dtype)
+        v = rnd(g, 1, 32, rows, d, dtype=dtype)
+        out = torch.empty_like(qq)
+        wr.window_attention(qq, k, v, out, i32([rows]), 100000, 0, False, scale=1.0)
+        wr.close(out, *wr.attention64(qq, k, v, [q], [rows], 100000, scale=1.0))
+
+
+@pytest.mark.parametrize("dtype,d,q,hq,hkv", [(BF16, 128, 256, 64, 16), (F16, 64, 64, 64, 8), (F32, 64, 256, 64, 16)])
+def test_many_queries_captured_and_on_two_streams(built, dtype, d, q, hq, hkv):
+    """Graphs on two streams replayed at once, with lengths that change between replays."""
+    g = gen(24)
+    n, rows = 2, q + 1200
+    qq = rnd(g, n * q, hq, d, dtype=dtype)
+    k, v = rnd(g, n, hkv, rows, d, dtype=dtype), rnd(g, n, hkv, rows, d, dtype=dtype)
+    kv_len, outs = i32([q + 200, q + 10]), [torch.zeros_like(qq) for _ in range(3)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs = []
+    torch.cuda.synchronize()
+    for o, s in zip(outs, streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            for _ in range(4):
+                wr.window_attention(qq, k, v, o, kv_len, 900, 4, False)
+        graphs.append(graph)
+    for lens in ([q + 1200, q + 10], [q, q + 299], [q + 7, 0]):
+        kv_len.copy_(i32(lens))
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        wr.window_attention(qq, k, v, outs[2], kv_len, 900, 4, False)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[2])
+        wr.close(outs[2], *wr.attention64(qq, k, v, [q] * n, lens, 900, 4))
+
+
+@pytest.mark.parametrize("dtype,d,q,hq", [(BF16, 128, 300, 64), (F16, 64, 1, 8), (F32, 64, 1, 8), (F32, 64, 300, 64)])
+def test_broadcast_cache_and_negative_scale(built, dtype, d, q, hq):
+    """One cache expanded over slots and heads (strides of 0), keys in descending rows of memory
+    (a negative row stride is no torch tensor: the argument block is changed by hand), and a scale
+    below 0."""
+    g = gen(25)
+    rows = q + 100
+    qq = rnd(g, 2 * q, hq, d, dtype=dtype)
+    k1, v1 = rnd(g, 1, 1, rows, d, dtype=dtype), rnd(g, 1, 1, rows, d, dtype=dtype)
+    k, v = k1.expand(2, hq // 4, rows, d), v1.expand(2, hq // 4, rows, d)
+    out = torch.empty_like(qq)
+    for scale in (0.1, -0.1):
+        wr.window_attention(qq, k, v, out, i32([rows, rows - 5]), 70, 2, False, scale=scale)
+        wr.close(out, *wr.attention64(qq, k, v, [q, q], [rows, rows - 5], 70, 2, scale=abs(scale))
+                 if scale > 0 else wr.attention64(-qq, k, v, [q, q], [rows, rows - 5], 70, 2, scale=-scale))
+    back_k, back_v = k1.flip(2).contiguous(), v1.flip(2).contiguous()
+    a = wr.attn_args(qq, back_k.expand(2, hq // 4, rows, d), back_v.expand(2, hq // 4, rows, d), out,
+                     i32([rows, rows - 5]), 70, 2)
+    last = (rows - 1) * d * qq.element_size()
+    a.k, a.v, a.kv_row_stride = a.k + last, a.v + last, -d
+    check(load_cuda().armai_dev_window_attention(ctypes.byref(a), wr.stream()))
+    wr.close(out, *wr.attention64(qq, k, v, [q, q], [rows, rows - 5], 70, 2))
+
+
+def test_scale_zero_averages(built):
+    """A scale of 0 weighs every visible key alike."""
+    g = gen(26)
+    for dtype in (BF16, F32):
+        qq, k, v = rnd(g, 40, 4, 64, dtype=dtype), rnd(g, 1, 2, 100, 64, dtype=dtype), rnd(g, 1, 2, 100, 64, dtype=dtype)
+        out = torch.empty_like(qq)
+        wr.window_attention(qq, k, v, out, i32([100]), 30, 2, False, scale=0.0)
+        wr.close(out, *wr.attention64(qq, k, v, [40], [100], 30, 2, scale=0.0))
