@@ -20,9 +20,6 @@ namespace armai {
 namespace {
 
 constexpr int WS_K = 64;        // keys per tile; queries: Q, 64 or 32, with 4 Q threads
-#ifndef WSX
-#define WSX 4
-#endif
 constexpr int WS_PP = WS_K + 4;  // row of P, padded
 
 template <int DM, int Q>
@@ -95,14 +92,15 @@ __global__ void __launch_bounds__(4 * Q, DM > 96 ? 1 : Q == 64 ? 2 : 3) k_wa_sim
   const int qlo = sq.pos0 + i0, qhi = qlo + rows - 1;
   const WaRuns runs = wa_runs(p, qlo, qhi);
   const int nt = wa_tiles<WS_K>(runs), dq = (D + 3) & ~3;
+  // V of a key tile is copied while its scores are worked out, K of the next
+  // one during the softmax and P V.
+  WaTile x = wa_tile<WS_K>(runs, 0);
+  if (nt > 0) ws_rows<T, DM, WS_K, 4 * Q>(Ks, kb + (int64_t)x.row * p.kv_row, p.kv_row, x.n, D, vec);
 #pragma unroll 1
   for (int t = 0; t < nt; t++) {
-    const WaTile x = wa_tile<WS_K>(runs, t);
-    __syncthreads();
-    ws_rows<T, DM, WS_K, 4 * Q>(Ks, kb + (int64_t)x.row * p.kv_row, p.kv_row, x.n, D, vec);
-    ws_rows<T, DM, WS_K, 4 * Q>(Vs, vb + (int64_t)x.row * p.kv_row, p.kv_row, x.n, D, vec);
     asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
+    __syncthreads();  // K is here, V of the tile before is done with
+    ws_rows<T, DM, WS_K, 4 * Q>(Vs, vb + (int64_t)x.row * p.kv_row, p.kv_row, x.n, D, vec);
     float acc[4][4];
     float2 part[4][4];  // of even and of odd values
 #pragma unroll
@@ -124,6 +122,10 @@ __global__ void __launch_bounds__(4 * Q, DM > 96 ? 1 : Q == 64 ? 2 : 3) k_wa_sim
           ws_fma2(part[i][j], make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w));
         }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // V is here, K is done with
+    const WaTile y = wa_tile<WS_K>(runs, min(t + 1, nt - 1));
+    if (t + 1 < nt) ws_rows<T, DM, WS_K, 4 * Q>(Ks, kb + (int64_t)y.row * p.kv_row, p.kv_row, y.n, D, vec);
     const bool full = x.n == WS_K && x.pos + WS_K - 1 <= qlo && (qhi - x.pos < p.window || x.pos + WS_K - 1 < p.n_sink);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -156,7 +158,7 @@ __global__ void __launch_bounds__(4 * Q, DM > 96 ? 1 : Q == 64 ? 2 : 3) k_wa_sim
     }
     __syncwarp();  // a query's row of P is written and read by one half-warp
 #pragma unroll 2
-    for (int c = 0; c < WS_K; c += 4) {
+    for (int c = 0; c < x.n; c += 4) {
       float4 a[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) a[i] = *reinterpret_cast<const float4*>(Ps + (ty * 4 + i) * WS_PP + c);
@@ -172,6 +174,7 @@ __global__ void __launch_bounds__(4 * Q, DM > 96 ? 1 : Q == 64 ? 2 : 3) k_wa_sim
           }
         }
     }
+    x = y;
   }
 #pragma unroll
   for (int i = 0; i < 4; i++) {
@@ -203,7 +206,7 @@ int ws_launch(const WaParams& p, int vec, cudaStream_t s) {
 template <typename T, int DM>
 int ws_rows_per_cta(const WaParams& p, int vec, cudaStream_t s) {
   const int64_t ctas = (int64_t)p.n_seq * p.n_q_heads * ((p.max_q + 63) / 64);
-  return ctas > WSX * (int64_t)sm_count() ? ws_launch<T, DM, 64>(p, vec, s) : ws_launch<T, DM, 32>(p, vec, s);
+  return ctas > 4 * (int64_t)sm_count() ? ws_launch<T, DM, 64>(p, vec, s) : ws_launch<T, DM, 32>(p, vec, s);
 }
 template <typename T>
 int ws_dim(const WaParams& p, int vec, cudaStream_t s) {
