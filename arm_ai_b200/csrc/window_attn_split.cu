@@ -342,26 +342,27 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
     cp_wait<SP_STAGES - 1>();
     __syncwarp();
     // s[j][0, 1]: row g, keys 8 j + 2 c, + 1; s[j][2, 3]: row g + 8. Two sums
-    // each, for shorter chains.
-    float s[2][4], s2[2][4];
+    // each, for shorter chains (one at a width of 256, for its registers).
+    constexpr bool TWO = DT < 256;
+    float s[2][4], s2[TWO ? 2 : 1][4];
 #pragma unroll
     for (int j = 0; j < 2; j++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) s[j][k] = s2[j][k] = 0.f;
+      for (int k = 0; k < 4; k++) s[j][k] = s2[TWO ? j : 0][k] = 0.f;
 #pragma unroll
     for (int i = 0; i < KC; i++)
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         const uint4 v = *reinterpret_cast<const uint4*>(src + kread[i & 1] + j * 8 * (RC * 16) + i * 64);
         mma16816<T>(s[j], qa[i][0], v.x, v.y);
-        mma16816<T>(s2[j], qa[i][1], v.z, v.w);
+        mma16816<T>(TWO ? s2[TWO ? j : 0] : s[j], qa[i][1], v.z, v.w);
       }
     const int pos = cur.first_pos(), n = cur.keys();
     cur.advance(b.runs, step);
 #pragma unroll
     for (int j = 0; j < 2; j++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) s[j][k] += s2[j][k];
+      for (int k = 0; k < 4; k++) s[j][k] += TWO ? s2[TWO ? j : 0][k] : 0.f;
     if (!(n == SP_KT && pos + SP_KT - 1 <= qmin && (qmax - pos < p.window || pos + SP_KT - 1 < p.n_sink))) {
 #pragma unroll
       for (int j = 0; j < 2; j++)
