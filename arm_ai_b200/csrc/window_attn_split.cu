@@ -26,7 +26,10 @@ namespace cg = cooperative_groups;
 namespace armai {
 namespace {
 
-constexpr int SP_WARPS = 4, SP_THREADS = 32 * SP_WARPS;
+// Warps per CTA by (padded) head width: beyond 128 a ring fills half an SM's
+// shared memory, so that one CTA has to do; its warps are as many as their
+// rings leave room for.
+__host__ __device__ constexpr int sp_warps(int dt) { return dt > 128 ? 6 : 4; }
 constexpr int SP_STAGES = 2;
 constexpr int SP_MAX_SPLIT = 16;
 // The running maximum is raised (and the output rescaled) only when a score
@@ -152,6 +155,7 @@ struct SpMail {
 template <typename T, int R, int DT>
 __device__ __forceinline__ void sp_join(const WaParams& p, const SpBlock& b, const float* part, const float* wm,
                                         const float* wl, SpMail<R, DT>* mail) {
+  constexpr int WARPS = sp_warps(DT);
   const int tid = threadIdx.x, items = b.nr * (DT / 4);
   const int ranks = (int)gridDim.x, rank = (int)blockIdx.x, per = (items + ranks - 1) / ranks;
   auto write = [&](int r, int d, const float4& acc, float l) {
@@ -169,15 +173,15 @@ __device__ __forceinline__ void sp_join(const WaParams& p, const SpBlock& b, con
   cg::cluster_group cluster = cg::this_cluster();
   __syncthreads();
   if (ranks > 1) sp_cluster_wait();
-  for (int e = tid; e < items; e += SP_THREADS) {
+  for (int e = tid; e < items; e += 32 * WARPS) {
     const int r = e / (DT / 4), d = (e % (DT / 4)) * 4;
     float m = wm[r], l = 0.f;
 #pragma unroll
-    for (int w = 1; w < SP_WARPS; w++) m = fmaxf(m, wm[w * R + r]);
+    for (int w = 1; w < WARPS; w++) m = fmaxf(m, wm[w * R + r]);
     const float base = m == -INFINITY ? 0.f : m;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < SP_WARPS; w++) {
+    for (int w = 0; w < WARPS; w++) {
       const float f = sp_exp2(wm[w * R + r] - base);
       const float4 v = *reinterpret_cast<const float4*>(part + (w * R + r) * DT + d);
       l += f * wl[w * R + r];
@@ -199,7 +203,7 @@ __device__ __forceinline__ void sp_join(const WaParams& p, const SpBlock& b, con
   if (ranks == 1) return;
   sp_cluster_arrive();
   sp_cluster_wait();
-  for (int e = rank * per + tid; e < min(items, (rank + 1) * per); e += SP_THREADS) {
+  for (int e = rank * per + tid; e < min(items, (rank + 1) * per); e += 32 * WARPS) {
     const int r = e / (DT / 4), i = e - rank * per;
     float m = -INFINITY, l = 0.f;
     for (int k = 0; k < ranks; k++) m = fmaxf(m, mail->s[k][r].x);
@@ -237,13 +241,14 @@ __device__ __forceinline__ int sp_swz_v(int key) { return key & 6; }
 
 template <typename T, int DT>
 __host__ __device__ constexpr size_t sp_smem() {
-  const size_t ring = (size_t)SP_WARPS * SP_STAGES * 2 * SP_KT * DT * 2;
-  const size_t join = (size_t)SP_WARPS * SP_ROWS * (DT + 2) * 4;
+  const size_t ring = (size_t)sp_warps(DT) * SP_STAGES * 2 * SP_KT * DT * 2;
+  const size_t join = (size_t)sp_warps(DT) * SP_ROWS * (DT + 2) * 4;
   return ring > join ? ring : join;  // one after the other
 }
 
 template <typename T, int DT>
-__global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
+__global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p) {
+  constexpr int WARPS = sp_warps(DT);
   constexpr int KC = DT / 32, VB = DT / 64;       // k chunks per key and lane; 64-wide blocks of v
   constexpr uint32_t TILE = SP_KT * DT * 2;       // a tile of K or V
   extern __shared__ __align__(16) uint8_t sm[];
@@ -260,12 +265,12 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
   constexpr int RC = DT / 8, RPC = 32 / RC;       // chunks per row, rows per copy instruction
   const int ck = lane / RC, cc = lane % RC;
   const int64_t kv_off = (int64_t)b.sq.slot * p.kv_slot + (int64_t)b.kvh * p.kv_head;
-  const int64_t row = p.kv_row, tile_stride = (int64_t)gridDim.x * SP_WARPS * SP_KT * row;
+  const int64_t row = p.kv_row, tile_stride = (int64_t)gridDim.x * WARPS * SP_KT * row;
   const T* kb = static_cast<const T*>(p.k) + kv_off + ck * row + 8 * cc;
   const T* vb = static_cast<const T*>(p.v) + kv_off + ck * row + 8 * cc;
   const uint8_t* ring = sm + warp * (SP_STAGES * 2 * TILE);
   const uint32_t ring32 = smem_u32(ring);
-  const int step = (int)gridDim.x * SP_WARPS, first = (int)blockIdx.x * SP_WARPS + warp;
+  const int step = (int)gridDim.x * WARPS, first = (int)blockIdx.x * WARPS + warp;
 
   SpCursor<SP_KT> cur(b.runs, first), ahead = cur;
   int64_t at = (int64_t)ahead.first_row() * row;  // of the loads' tile, in values from kb and vb
@@ -422,8 +427,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
   cp_wait<0>();
   __syncthreads();  // the ring becomes the join area
   float* part = reinterpret_cast<float*>(sm);
-  float* wm = part + SP_WARPS * SP_ROWS * DT;
-  float* wl = wm + SP_WARPS * SP_ROWS;
+  float* wm = part + WARPS * SP_ROWS * DT;
+  float* wl = wm + WARPS * SP_ROWS;
 #pragma unroll
   for (int j = 0; j < 2; j++) {
     l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
@@ -451,17 +456,17 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split(const WaParams p) {
 // exchanged so that a lane ends with one row's whole score (R = 8: 7 shuffles
 // for 8 rows), makes that row's weight, and hands it back to the 8 lanes.
 // ---------------------------------------------------------------------------
-constexpr int SF_KT = 8;
+constexpr int SF_KT = 8, SF_WARPS = sp_warps(128);
 
 template <int CH>
 __host__ __device__ constexpr size_t sf_smem(int rows) {
-  const size_t ring = (size_t)SP_WARPS * SP_STAGES * 2 * SF_KT * CH * 32 * 4;
-  const size_t join = (size_t)SP_WARPS * rows * (CH * 32 + 2) * 4;
+  const size_t ring = (size_t)SF_WARPS * SP_STAGES * 2 * SF_KT * CH * 32 * 4;
+  const size_t join = (size_t)SF_WARPS * rows * (CH * 32 + 2) * 4;
   return ring > join ? ring : join;  // one after the other
 }
 
 template <int R, int CH>
-__global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
+__global__ void __launch_bounds__(32 * SF_WARPS) k_wa_split_f32(const WaParams p) {
   constexpr int DT = 32 * CH;
   constexpr int SH = R == 8 ? 0 : R == 4 ? 1 : R == 2 ? 2 : 3;  // lanes per row of the 8: 2^SH
   extern __shared__ __align__(16) uint8_t sm[];
@@ -474,7 +479,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
   const float* kb = static_cast<const float*>(p.k) + kv_off;
   const float* vb = static_cast<const float*>(p.v) + kv_off;
   float4* ring = reinterpret_cast<float4*>(sm) + warp * (SP_STAGES * 4 * CH * 32) + lane;
-  const int step = (int)gridDim.x * SP_WARPS, first = (int)blockIdx.x * SP_WARPS + warp;
+  const int step = (int)gridDim.x * SF_WARPS, first = (int)blockIdx.x * SF_WARPS + warp;
   const int nt = wa_tiles<SF_KT>(b.runs);
 
   auto load = [&](int t, int slot) {
@@ -602,8 +607,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
   l += __shfl_xor_sync(0xffffffffu, l, 8);
   l += __shfl_xor_sync(0xffffffffu, l, 16);
   float* part = reinterpret_cast<float*>(sm);
-  float* wm = part + SP_WARPS * R * DT;
-  float* wl = wm + SP_WARPS * R;
+  float* wm = part + SF_WARPS * R * DT;
+  float* wl = wm + SF_WARPS * R;
   if (kg == 0 && (x8 & ((1 << SH) - 1)) == 0) {
     wm[warp * R + mine] = m;
     wl[warp * R + mine] = l;
@@ -630,25 +635,25 @@ __global__ void __launch_bounds__(SP_THREADS) k_wa_split_f32(const WaParams p) {
 // 32 streams of 4100 visible keys, 8 heads of 128, bf16: 83.0 us = 6.48 TB/s
 // (room for two CTAs with three stages each 86.9; four or eight times the
 // splits 88 to 100).
-int sp_split(int64_t blocks, int64_t keys, int kt) {
-  const int64_t room = 3 * (int64_t)sm_count();
+int sp_split(int64_t blocks, int64_t keys, int kt, int warps, int per_sm) {
+  const int64_t room = per_sm * (int64_t)sm_count();
   int n = 1;
-  while (n < SP_MAX_SPLIT && blocks * n * 2 <= room && (int64_t)n * 2 * SP_WARPS * kt <= keys) n *= 2;
+  while (n < SP_MAX_SPLIT && blocks * n * 2 <= room && (int64_t)n * 2 * warps * kt <= keys) n *= 2;
   return n;
 }
 
 template <typename K>
-int sp_launch(K kernel, size_t smem, const WaParams& p, int rows, int kt, cudaStream_t s) {
+int sp_launch(K kernel, size_t smem, const WaParams& p, int rows, int kt, int dt, cudaStream_t s) {
   const int64_t pairs = (int64_t)p.max_q * p.group, rb = (pairs + rows - 1) / rows;
   const int64_t blocks = rb * p.n_kv;
   const int64_t span = std::min<int64_t>(p.max_q, (rows + p.group - 1) / p.group + 1);
   const int64_t keys = std::min<int64_t>(p.kv_rows, (int64_t)p.window + p.n_sink + span);
-  const int split = sp_split(blocks * p.n_seq, keys, kt);
+  const int split = sp_split(blocks * p.n_seq, keys, kt, sp_warps(dt), dt > 128 ? 1 : 3);
   ARMAI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   if (split > 8) ARMAI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)split, (unsigned)blocks, (unsigned)p.n_seq);
-  cfg.blockDim = dim3(SP_THREADS);
+  cfg.blockDim = dim3(32 * sp_warps(dt));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -664,14 +669,14 @@ int sp_launch(K kernel, size_t smem, const WaParams& p, int rows, int kt, cudaSt
 
 template <typename T>
 int sp_half(const WaParams& p, cudaStream_t s) {
-  if (p.head_dim <= 64) return sp_launch(k_wa_split<T, 64>, sp_smem<T, 64>() + sizeof(SpMail<SP_ROWS, 64>), p, SP_ROWS, SP_KT, s);
-  if (p.head_dim <= 128) return sp_launch(k_wa_split<T, 128>, sp_smem<T, 128>() + sizeof(SpMail<SP_ROWS, 128>), p, SP_ROWS, SP_KT, s);
-  return sp_launch(k_wa_split<T, 256>, sp_smem<T, 256>() + sizeof(SpMail<SP_ROWS, 256>), p, SP_ROWS, SP_KT, s);
+  if (p.head_dim <= 64) return sp_launch(k_wa_split<T, 64>, sp_smem<T, 64>() + sizeof(SpMail<SP_ROWS, 64>), p, SP_ROWS, SP_KT, 64, s);
+  if (p.head_dim <= 128) return sp_launch(k_wa_split<T, 128>, sp_smem<T, 128>() + sizeof(SpMail<SP_ROWS, 128>), p, SP_ROWS, SP_KT, 128, s);
+  return sp_launch(k_wa_split<T, 256>, sp_smem<T, 256>() + sizeof(SpMail<SP_ROWS, 256>), p, SP_ROWS, SP_KT, 256, s);
 }
 
 template <int R, int CH>
 int sp_f32(const WaParams& p, cudaStream_t s) {
-  return sp_launch(k_wa_split_f32<R, CH>, sf_smem<CH>(R) + sizeof(SpMail<R, 32 * CH>), p, R, SF_KT, s);
+  return sp_launch(k_wa_split_f32<R, CH>, sf_smem<CH>(R) + sizeof(SpMail<R, 32 * CH>), p, R, SF_KT, 32 * CH, s);
 }
 // Rows per CTA as many as there are, up to eight; four at the widths where
 // eight rows of q and of the output would not fit the registers.
