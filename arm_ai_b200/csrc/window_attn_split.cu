@@ -17,6 +17,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "llama_kernels.cuh"
 #include "window_attn.cuh"
@@ -630,53 +631,79 @@ __global__ void __launch_bounds__(32 * SF_WARPS) k_wa_split_f32(const WaParams p
   sp_join<float, R, DT>(p, b, part, wm, wl, reinterpret_cast<SpMail<R, DT>*>(sm + sf_smem<CH>(R)));
 }
 
-// Splits of one sequence and head: up to three CTAs per SM (what their rings
-// leave room for; 64 KB of copies in flight each), but no warp without a tile.
-// 32 streams of 4100 visible keys, 8 heads of 128, bf16: 83.0 us = 6.48 TB/s
-// (room for two CTAs with three stages each 86.9; four or eight times the
-// splits 88 to 100).
-int sp_split(int64_t blocks, int64_t keys, int kt, int warps, int per_sm) {
-  const int64_t room = per_sm * (int64_t)sm_count();
-  int n = 1;
-  while (n < SP_MAX_SPLIT && blocks * n * 2 <= room && (int64_t)n * 2 * warps * kt <= keys) n *= 2;
-  return n;
+// Clusters of 2^log2 CTAs that the device holds at once (with one CTA per SM
+// 33 of 4, 15 of 8 and 7 of 16: what is left of a die's groups of SMs stays
+// empty), asked for once per kernel, size and device.
+template <auto K>
+int sp_active(int log2, const cudaLaunchConfig_t& cfg, int& active) {
+  constexpr int DEVICES = 32;
+  static std::atomic<int> known[DEVICES][5];
+  int dev = 0;
+  ARMAI_CUDA(cudaGetDevice(&dev));
+  active = dev < DEVICES ? known[dev][log2].load(std::memory_order_relaxed) : 0;
+  if (active) return ARMAI_OK;
+  ARMAI_CUDA(cudaOccupancyMaxActiveClusters(&active, K, &cfg));
+  active = std::max(active, 1);
+  if (dev < DEVICES) known[dev][log2].store(active, std::memory_order_relaxed);
+  return ARMAI_OK;
 }
 
-template <typename K>
-int sp_launch(K kernel, size_t smem, const WaParams& p, int rows, int kt, int dt, cudaStream_t s) {
+// A sequence and head's keys are split over as many CTAs as run at once, but
+// no warp goes without a tile. A cluster left over would take as long again as
+// the others (one stream, 4096 keys, width 256: 8 heads over 16 CTAs each 23.7
+// us, over 8 each 18.1; 7 heads over 16 each 12.6), unless it is one in fifteen
+// and SMs hold several CTAs (48 heads and streams of 4096 keys, width 128: over
+// 8 CTAs each 18.3 us, 45 clusters at once; over 4 each 23.9).
+// 32 streams of 4100 visible keys, 8 heads of 128, bf16: 82.4 us = 6.53 TB/s.
+template <auto K>
+int sp_launch(size_t smem, const WaParams& p, int rows, int kt, int warps, cudaStream_t s) {
   const int64_t pairs = (int64_t)p.max_q * p.group, rb = (pairs + rows - 1) / rows;
   const int64_t blocks = rb * p.n_kv;
   const int64_t span = std::min<int64_t>(p.max_q, (rows + p.group - 1) / p.group + 1);
   const int64_t keys = std::min<int64_t>(p.kv_rows, (int64_t)p.window + p.n_sink + span);
-  const int split = sp_split(blocks * p.n_seq, keys, kt, sp_warps(dt), dt > 128 ? 1 : 3);
-  ARMAI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  if (split > 8) ARMAI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  ARMAI_CUDA(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)split, (unsigned)blocks, (unsigned)p.n_seq);
-  cfg.blockDim = dim3(32 * sp_warps(dt));
+  cfg.gridDim = dim3(SP_MAX_SPLIT, (unsigned)blocks, (unsigned)p.n_seq);
+  cfg.blockDim = dim3(32 * warps);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  ARMAI_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+  int split = 1;
+  for (int log2 = 1; 1 << log2 <= SP_MAX_SPLIT; log2++) {
+    const int n = 1 << log2;
+    const int64_t clusters = blocks * p.n_seq;
+    if ((int64_t)n * warps * kt > keys || clusters * n > 4 * (int64_t)sm_count()) break;
+    if (n > 8) ARMAI_CUDA(cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    attr[0].val.clusterDim.x = (unsigned)n;
+    int active = 0;
+    ARMAI_TRY(sp_active<K>(log2, cfg, active));
+    const bool several = active * n > sm_count();
+    if (several ? clusters * 15 > (int64_t)active * 16 : clusters > active) break;
+    split = n;
+  }
+  cfg.gridDim.x = attr[0].val.clusterDim.x = (unsigned)split;
+  ARMAI_CUDA(cudaLaunchKernelEx(&cfg, K, p));
   return ARMAI_OK;
 }
 
+template <typename T, int DT>
+int sp_width(const WaParams& p, cudaStream_t s) {
+  return sp_launch<k_wa_split<T, DT>>(sp_smem<T, DT>() + sizeof(SpMail<SP_ROWS, DT>), p, SP_ROWS, SP_KT, sp_warps(DT), s);
+}
 template <typename T>
 int sp_half(const WaParams& p, cudaStream_t s) {
-  if (p.head_dim <= 64) return sp_launch(k_wa_split<T, 64>, sp_smem<T, 64>() + sizeof(SpMail<SP_ROWS, 64>), p, SP_ROWS, SP_KT, 64, s);
-  if (p.head_dim <= 128) return sp_launch(k_wa_split<T, 128>, sp_smem<T, 128>() + sizeof(SpMail<SP_ROWS, 128>), p, SP_ROWS, SP_KT, 128, s);
-  return sp_launch(k_wa_split<T, 256>, sp_smem<T, 256>() + sizeof(SpMail<SP_ROWS, 256>), p, SP_ROWS, SP_KT, 256, s);
+  if (p.head_dim <= 64) return sp_width<T, 64>(p, s);
+  if (p.head_dim <= 128) return sp_width<T, 128>(p, s);
+  return sp_width<T, 256>(p, s);
 }
 
 template <int R, int CH>
 int sp_f32(const WaParams& p, cudaStream_t s) {
-  return sp_launch(k_wa_split_f32<R, CH>, sf_smem<CH>(R) + sizeof(SpMail<R, 32 * CH>), p, R, SF_KT, 32 * CH, s);
+  return sp_launch<k_wa_split_f32<R, CH>>(sf_smem<CH>(R) + sizeof(SpMail<R, 32 * CH>), p, R, SF_KT, SF_WARPS, s);
 }
 // Rows per CTA as many as there are, up to eight; four at the widths where
 // eight rows of q and of the output would not fit the registers.
