@@ -324,10 +324,17 @@ extern "C" int armai_dev_window_attention(const armai_window_attention_args* a, 
   p.scale_log2 = a->scale * 1.4426950408889634f;
   const cudaStream_t s = (cudaStream_t)stream;
   if (wa_vectors(p, a->dtype)) {
-    if (wa_split_fits(p, a->dtype) && wa_split_better(p, a->dtype)) return wa_split_launch(p, a->dtype, s);
+    const bool split = wa_split_fits(p, a->dtype);
+    if (split && wa_split_better(p, a->dtype)) return wa_split_launch(p, a->dtype, s);
     bool fits = false;
     ARMAI_TRY(wa_tc_launch(p, a->dtype, s, &fits));
     if (fits) return ARMAI_OK;
+    // 16-bit tensors that the 5th-generation tensor cores cannot take (heads
+    // wider than 128, strides of 0, a negative scale): reading the keys for
+    // every 16 rows is still faster than products on the CUDA cores (1024
+    // tokens, 8 heads of 256, bf16: 72 us against 535; 8192 rows of 4 heads on
+    // 4096 keys of 256: 2.7 ms against 10.3)
+    if (split && a->dtype != ARMAI_F32) return wa_split_launch(p, a->dtype, s);
   }
   return wa_simt_launch(p, a->dtype, s);
 }

@@ -31,8 +31,9 @@ struct WaParams {
   uint32_t* err;             // bounded waits that ran out
 };
 
-// Token of (token, query head of the group) pair f, exact for f < 2^16: a
-// product instead of a division.
+// Token of (token, query head of the group) pair f, exact for f < 2^32 / group
+// (group_mul exceeds 2^32 / group by less than 1): a product instead of a
+// division.
 __device__ __forceinline__ int wa_token(const WaParams& p, int f) {
   return p.group == 1 ? f : (int)__umulhi((uint32_t)f, p.group_mul);
 }

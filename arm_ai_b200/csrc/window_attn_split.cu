@@ -722,9 +722,10 @@ int sp_f32_rows(const WaParams& p, cudaStream_t s) {
 
 // Head widths of whole 16-byte vectors, and heads that fit the grid.
 bool wa_split_fits(const WaParams& p, int dtype) {
-  const int es = dtype_size(dtype), v = 16 / es;
+  const int v = 16 / dtype_size(dtype), rows = dtype == ARMAI_F32 ? 4 : SP_ROWS;
+  const int64_t pairs = (int64_t)p.max_q * p.group;
   return p.head_dim % v == 0 && p.scale_log2 != 0.f && p.scale_log2 == p.scale_log2 && (dtype != ARMAI_F32 || p.head_dim <= 128) &&
-         (int64_t)p.max_q * p.group < 65536 && ((int64_t)p.max_q * p.group + 3) / 4 * p.n_kv <= 65535;
+         pairs * p.group < int64_t(1) << 32 && (pairs + rows - 1) / rows * p.n_kv <= 65535;
 }
 
 int wa_split_launch(const WaParams& p, int dtype, cudaStream_t s) {

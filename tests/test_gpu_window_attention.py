@@ -354,6 +354,19 @@ def test_many_queries(built, dtype, hq, hkv, d, q_lens, past, window, n_sink, ri
         extra=3)
 
 
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(BF16, 16, 4, 256), (F16, 6, 2, 160), (BF16, 4, 4, 136)])
+@pytest.mark.parametrize("q_lens,past,window,n_sink,ring", MANY)
+def test_many_queries_of_wide_heads(built, dtype, hq, hkv, d, q_lens, past, window, n_sink, ring):
+    run(gen(sum(q_lens) + d), dtype, hq, hkv, d, q_lens, [a + b for a, b in zip(past, q_lens)], window, n_sink, ring,
+        extra=3)
+
+
+@pytest.mark.parametrize("group,q", [(96, 700), (33, 2000)])
+def test_more_than_65536_rows_of_a_head(built, group, q):
+    """Pairs of a token and a head beyond 2^16, a key / value head of width 136."""
+    run(gen(group), F16, group, 1, 136, [q], [q + 3], 70, 2, False)
+
+
 @pytest.mark.parametrize("dtype,hq,hkv,d", [(BF16, 32, 8, 128), (F16, 32, 8, 64), (F16, 16, 2, 96)])
 @pytest.mark.parametrize("q_lens,past,window,n_sink,ring", [
     ([64], [4000], 3000, 4, False),      # eight tiles, the keys divided over clusters
