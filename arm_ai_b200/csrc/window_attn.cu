@@ -239,15 +239,18 @@ namespace {
 // cores, whose CTAs fill the SMs one by one: as long as there are fewer than 36
 // rows per SM for each round of tiles (8 streams of 2048 keys, 8 heads of 128:
 // 64 rows 250 against 308 us, 128 rows 476 against 308).
+// Wider heads leave it two rows at once: 10 rows per SM (8 streams of 1024
+// keys, 8 heads of 256: 16 rows 122 against 173 us, 64 rows 422 against 174;
+// one stream of 4096 keys: 1 row 15.7 against 625, 128 rows 436 against 636).
 bool wa_split_better(const WaParams& p, int dtype) {
   const int64_t pairs = (int64_t)p.max_q * p.group, heads = (int64_t)p.n_seq * p.n_kv;
   if (dtype != ARMAI_F32) {
     const int64_t keys = std::min<int64_t>(p.kv_rows, (int64_t)p.window + p.n_sink + p.max_q);
     return pairs <= 16 || heads * ((pairs + 15) / 16) * keys * 4 * p.head_dim <= 80 * 1000 * 1000;
   }
-  const int64_t r = p.head_dim <= 64 ? 8 : 4, rows = heads * ((pairs + r - 1) / r) * r;
+  const int64_t r = p.head_dim <= 64 ? 8 : p.head_dim <= 128 ? 4 : 2, rows = heads * ((pairs + r - 1) / r) * r;
   const int64_t tiles = (int64_t)p.n_seq * p.n_q_heads * ((p.max_q + 63) / 64), sms = sm_count();
-  return rows <= 36 * sms * ((tiles + sms - 1) / sms);
+  return rows <= (p.head_dim <= 128 ? 36 : 10) * sms * ((tiles + sms - 1) / sms);
 }
 
 }  // namespace

@@ -457,18 +457,18 @@ __global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p
 // exchanged so that a lane ends with one row's whole score (R = 8: 7 shuffles
 // for 8 rows), makes that row's weight, and hands it back to the 8 lanes.
 // ---------------------------------------------------------------------------
-constexpr int SF_KT = 8, SF_WARPS = sp_warps(128);
+constexpr int SF_KT = 8;
 
 template <int CH>
 __host__ __device__ constexpr size_t sf_smem(int rows) {
-  const size_t ring = (size_t)SF_WARPS * SP_STAGES * 2 * SF_KT * CH * 32 * 4;
-  const size_t join = (size_t)SF_WARPS * rows * (CH * 32 + 2) * 4;
+  const size_t ring = (size_t)sp_warps(32 * CH) * SP_STAGES * 2 * SF_KT * CH * 32 * 4;
+  const size_t join = (size_t)sp_warps(32 * CH) * rows * (CH * 32 + 2) * 4;
   return ring > join ? ring : join;  // one after the other
 }
 
 template <int R, int CH>
-__global__ void __launch_bounds__(32 * SF_WARPS) k_wa_split_f32(const WaParams p) {
-  constexpr int DT = 32 * CH;
+__global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const WaParams p) {
+  constexpr int DT = 32 * CH, WARPS = sp_warps(DT);
   constexpr int SH = R == 8 ? 0 : R == 4 ? 1 : R == 2 ? 2 : 3;  // lanes per row of the 8: 2^SH
   extern __shared__ __align__(16) uint8_t sm[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kg = lane >> 3, x8 = lane & 7;
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(32 * SF_WARPS) k_wa_split_f32(const WaParams p
   const float* kb = static_cast<const float*>(p.k) + kv_off;
   const float* vb = static_cast<const float*>(p.v) + kv_off;
   float4* ring = reinterpret_cast<float4*>(sm) + warp * (SP_STAGES * 4 * CH * 32) + lane;
-  const int step = (int)gridDim.x * SF_WARPS, first = (int)blockIdx.x * SF_WARPS + warp;
+  const int step = (int)gridDim.x * WARPS, first = (int)blockIdx.x * WARPS + warp;
   const int nt = wa_tiles<SF_KT>(b.runs);
 
   auto load = [&](int t, int slot) {
@@ -608,8 +608,8 @@ __global__ void __launch_bounds__(32 * SF_WARPS) k_wa_split_f32(const WaParams p
   l += __shfl_xor_sync(0xffffffffu, l, 8);
   l += __shfl_xor_sync(0xffffffffu, l, 16);
   float* part = reinterpret_cast<float*>(sm);
-  float* wm = part + SF_WARPS * R * DT;
-  float* wl = wm + SF_WARPS * R;
+  float* wm = part + WARPS * R * DT;
+  float* wl = wm + WARPS * R;
   if (kg == 0 && (x8 & ((1 << SH) - 1)) == 0) {
     wm[warp * R + mine] = m;
     wl[warp * R + mine] = l;
@@ -703,28 +703,31 @@ int sp_half(const WaParams& p, cudaStream_t s) {
 
 template <int R, int CH>
 int sp_f32(const WaParams& p, cudaStream_t s) {
-  return sp_launch<k_wa_split_f32<R, CH>>(sf_smem<CH>(R) + sizeof(SpMail<R, 32 * CH>), p, R, SF_KT, SF_WARPS, s);
+  return sp_launch<k_wa_split_f32<R, CH>>(sf_smem<CH>(R) + sizeof(SpMail<R, 32 * CH>), p, R, SF_KT, sp_warps(32 * CH), s);
 }
-// Rows per CTA as many as there are, up to eight; four at the widths where
-// eight rows of q and of the output would not fit the registers.
+// Rows per CTA as many as there are, up to eight; four or two at the widths
+// where more rows of q and of the output would not fit the registers.
+int sf_rows(int head_dim) { return head_dim <= 64 ? 8 : head_dim <= 128 ? 4 : 2; }
 template <int CH>
 int sp_f32_rows(const WaParams& p, cudaStream_t s) {
   const int64_t pairs = (int64_t)p.max_q * p.group;
   if (pairs <= 1) return sp_f32<1, CH>(p, s);
-  if (pairs <= 2) return sp_f32<2, CH>(p, s);
+  if constexpr (CH <= 4) {
+    if (pairs > 2 && (CH > 2 || pairs <= 4)) return sp_f32<4, CH>(p, s);
+  }
   if constexpr (CH <= 2) {
     if (pairs > 4) return sp_f32<8, CH>(p, s);
   }
-  return sp_f32<4, CH>(p, s);
+  return sp_f32<2, CH>(p, s);
 }
 
 }  // namespace
 
 // Head widths of whole 16-byte vectors, and heads that fit the grid.
 bool wa_split_fits(const WaParams& p, int dtype) {
-  const int v = 16 / dtype_size(dtype), rows = dtype == ARMAI_F32 ? 4 : SP_ROWS;
+  const int v = 16 / dtype_size(dtype), rows = dtype == ARMAI_F32 ? sf_rows(p.head_dim) : SP_ROWS;
   const int64_t pairs = (int64_t)p.max_q * p.group;
-  return p.head_dim % v == 0 && p.scale_log2 != 0.f && p.scale_log2 == p.scale_log2 && (dtype != ARMAI_F32 || p.head_dim <= 128) &&
+  return p.head_dim % v == 0 && p.scale_log2 != 0.f && p.scale_log2 == p.scale_log2 &&
          pairs * p.group < int64_t(1) << 32 && (pairs + rows - 1) / rows * p.n_kv <= 65535;
 }
 
@@ -735,7 +738,10 @@ int wa_split_launch(const WaParams& p, int dtype, cudaStream_t s) {
     case 1: return sp_f32_rows<1>(p, s);
     case 2: return sp_f32_rows<2>(p, s);
     case 3: return sp_f32_rows<3>(p, s);
-    default: return sp_f32_rows<4>(p, s);
+    case 4: return sp_f32_rows<4>(p, s);
+    case 5:
+    case 6: return sp_f32_rows<6>(p, s);
+    default: return sp_f32_rows<8>(p, s);
   }
 }
 

@@ -361,6 +361,27 @@ def test_many_queries_of_wide_heads(built, dtype, hq, hkv, d, q_lens, past, wind
         extra=3)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 256), (5, 1, 192), (3, 3, 160), (12, 4, 132), (4, 1, 248)])
+@pytest.mark.parametrize("q_lens,past,window,n_sink,ring", [
+    ([1, 1, 1, 1], [0, 62, 700, 4099], 1000, 4, False),
+    ([1, 1], [5000, 1030], 1024, 0, True),
+    ([1], [40000], 1 << 40, 0, False),   # clusters of every size the keys are divided over
+    ([3, 1, 8], [300, 0, 2], 90, 2, True),
+])
+def test_few_queries_of_wide_heads(built, dtype, hq, hkv, d, q_lens, past, window, n_sink, ring):
+    run(gen(sum(past) + d), dtype, hq, hkv, d, q_lens, [a + b for a, b in zip(past, q_lens)], window, n_sink, ring,
+        extra=2)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("seqs,hkv", [(1, 7), (1, 8), (1, 24), (3, 16), (2, 33), (7, 21)])
+def test_divisions_of_the_keys(built, dtype, d, seqs, hkv):
+    """Head and stream counts around those at which clusters of 16, 8, 4 and 2 CTAs no longer run all at once."""
+    run(gen(hkv), dtype, hkv, hkv, d, [1] * seqs, [2100 - 300 * i for i in range(seqs)], 2000, 1, False)
+
+
 @pytest.mark.parametrize("group,q", [(96, 700), (33, 2000)])
 def test_more_than_65536_rows_of_a_head(built, group, q):
     """Pairs of a token and a head beyond 2^16, a key / value head of width 136."""
