@@ -7,9 +7,9 @@
 //   norm (before the rotation): x * 1/sqrt(mean(x^2) + eps) * gamma
 //
 // Bound by memory: every value is read once and written once, with a handful
-// of operations between. A warp has one token: it makes the token's cosines
-// and sines once (instead of once per head), and a lane keeps its own, and its
-// gains, in registers for all heads. A power-of-two group of lanes holds a
+// of operations between. A warp has a token at a time: it makes the token's
+// cosines and sines once (instead of once per head), and a lane keeps its own,
+// and its gains, in registers for all heads. A power-of-two group of lanes holds a
 // head; a lane has both members of its pairs (two 16-byte vectors), so the
 // rotation needs no exchange and the norm's sum a few shuffles per head.
 #include <algorithm>

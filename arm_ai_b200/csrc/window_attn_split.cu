@@ -11,7 +11,12 @@
 // are whole 16-byte chunks.
 //   16-bit types: m16n8k16 tensor instructions, 16 rows = (token, query head)
 //   pairs of one key / value head, so a key is read once for all of them.
-//   f32: products on the CUDA cores, 8 lanes per key.
+//   f32: products on the CUDA cores, 8 lanes per key. One stream of 4096 keys,
+//   8 heads of 256: 15.7 us; 12 streams, 16 heads of 128: 139 us = 5.8 TB/s.
+// Where the 5th-generation tensor cores cannot take 16-bit tensors, many queries
+// come here too, in blocks of 16 rows that each read their keys, from L2 for the
+// most part (4096 tokens, 32 / 8 heads of 128, a negative scale: 0.84 ms = 164
+// TFLOP/s).
 // The cluster's parts are joined in rank order: results do not depend on
 // timing, no workspace, one launch.
 #include <cooperative_groups.h>
@@ -633,19 +638,21 @@ __global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const W
 
 // Clusters of 2^log2 CTAs that the device holds at once (with one CTA per SM
 // 33 of 4, 15 of 8 and 7 of 16: what is left of a die's groups of SMs stays
-// empty), asked for once per kernel, size and device.
+// empty), asked for once per kernel, size and device. 0: it has no such.
 template <auto K>
-int sp_active(int log2, const cudaLaunchConfig_t& cfg, int& active) {
+int sp_active(int log2, const cudaLaunchConfig_t& cfg) {
   constexpr int DEVICES = 32;
-  static std::atomic<int> known[DEVICES][5];
-  int dev = 0;
-  ARMAI_CUDA(cudaGetDevice(&dev));
-  active = dev < DEVICES ? known[dev][log2].load(std::memory_order_relaxed) : 0;
-  if (active) return ARMAI_OK;
-  ARMAI_CUDA(cudaOccupancyMaxActiveClusters(&active, K, &cfg));
-  active = std::max(active, 1);
-  if (dev < DEVICES) known[dev][log2].store(active, std::memory_order_relaxed);
-  return ARMAI_OK;
+  static std::atomic<int> known[DEVICES][5];  // and one more: 0 is not known
+  int dev = 0, active = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  const int k = dev < DEVICES ? known[dev][log2].load(std::memory_order_relaxed) : 0;
+  if (k) return k - 1;
+  if (cudaOccupancyMaxActiveClusters(&active, K, &cfg) != cudaSuccess) {
+    cudaGetLastError();  // clusters of this size cannot be: the answer, not a failure of the call
+    active = 0;
+  }
+  if (dev < DEVICES) known[dev][log2].store(active + 1, std::memory_order_relaxed);
+  return active;
 }
 
 // A sequence and head's keys are split over as many CTAs as run at once, but
@@ -679,8 +686,7 @@ int sp_launch(size_t smem, const WaParams& p, int rows, int kt, int warps, cudaS
     if ((int64_t)n * warps * kt > keys || clusters * n > 4 * (int64_t)sm_count()) break;
     if (n > 8) ARMAI_CUDA(cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr[0].val.clusterDim.x = (unsigned)n;
-    int active = 0;
-    ARMAI_TRY(sp_active<K>(log2, cfg, active));
+    const int active = sp_active<K>(log2, cfg);
     const bool several = active * n > sm_count();
     if (several ? clusters * 15 > (int64_t)active * 16 : clusters > active) break;
     split = n;
