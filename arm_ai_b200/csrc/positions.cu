@@ -88,9 +88,13 @@ __device__ __forceinline__ int rot_locate(const RotParams& p, int h, int& head) 
   return i;
 }
 
-__device__ __forceinline__ void rot_copy16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
-               : "memory");
+template <int BYTES>
+__device__ __forceinline__ void rot_copy(void* dst, const void* src) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
 }
 
 // Destination row of a token in tensor i, or -1.
@@ -100,7 +104,8 @@ __device__ __forceinline__ int64_t rot_row(const RotParams& p, int i, int64_t to
   return r >= 0 && r < p.n_rows ? r : -1;
 }
 
-// Vector form: every head's start and the second vectors 16-byte aligned.
+// Vector form: vectors of VEC values (16, 8 or 4 bytes, the widest that fits),
+// every head's start and the second vectors aligned to them.
 // Lane l of a head's HL lanes (power of two) has the VEC pairs from l * VEC on:
 //   half layout: the vectors at l * VEC and rot / 2 + l * VEC; the lanes behind
 //   rot / 2 one of each half of what is not rotated
@@ -111,12 +116,11 @@ __device__ __forceinline__ int64_t rot_row(const RotParams& p, int i, int64_t to
 // items ahead, as asynchronous copies into a ring in which a lane reads back
 // only what it copied itself: enough bytes in flight for the memory, whatever
 // the registers hold.
-template <typename T, typename KV, bool IL>
+template <typename T, typename KV, bool IL, int VEC>
 __global__ void __launch_bounds__(ROT_THREADS) k_rotate_vec(const RotParams p, int hl, int64_t n_tokens, int splits,
                                                             float inv_dim) {
-  constexpr int VEC = 16 / (int)sizeof(T);
   __shared__ float2 table[ROT_WARPS][ROT_MAX_DIM / 2];
-  __shared__ uint4 ring_[ROT_WARPS][ROT_STAGES][2][32];
+  __shared__ Vec<T, VEC> ring_[ROT_WARPS][ROT_STAGES][2][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t unit = (int64_t)blockIdx.x * ROT_WARPS + warp;
   int64_t token = unit / splits;
@@ -138,7 +142,7 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotate_vec(const RotParams p, i
     }
   }
   // the loads' place in the stream: token, tensor, this lane's head in the item, its address
-  uint4(*ring)[2][32] = ring_[warp];
+  Vec<T, VEC>(*ring)[2][32] = ring_[warp];
   int64_t ahead = token, ahead_step = 0;
   int ahead_i = only, ahead_h = h0 + sub, put = 0;
   const T* ahead_src = nullptr;
@@ -163,8 +167,8 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotate_vec(const RotParams p, i
     if (ahead < n_tokens) {
       const int heads = p.t[ahead_i].heads;
       if (mine && ahead_h < heads) {
-        rot_copy16(&ring[put][0][lane], ahead_src + da);
-        rot_copy16(&ring[put][1][lane], ahead_src + db);
+        rot_copy<VEC * (int)sizeof(T)>(&ring[put][0][lane], ahead_src + da);
+        rot_copy<VEC * (int)sizeof(T)>(&ring[put][1][lane], ahead_src + db);
       }
       ahead_h += hpw;
       ahead_src += ahead_step;
@@ -199,16 +203,24 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotate_vec(const RotParams p, i
       const RotTensor& t = p.t[i];
       const bool norm = t.gamma != nullptr;
       if (norm && mine) {
+        if constexpr (VEC >= 4) {
 #pragma unroll
-        for (int e = 0; e < VEC; e += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(t.gamma + (IL ? da + 2 * e : da + e));
-          const float4 y = *reinterpret_cast<const float4*>(t.gamma + (IL ? da + 2 * e + 4 : db + e));
-          if (IL) {
-            ga[e] = x.x, gb[e] = x.y, ga[e + 1] = x.z, gb[e + 1] = x.w;
-            ga[e + 2] = y.x, gb[e + 2] = y.y, ga[e + 3] = y.z, gb[e + 3] = y.w;
-          } else {
-            ga[e] = x.x, ga[e + 1] = x.y, ga[e + 2] = x.z, ga[e + 3] = x.w;
-            gb[e] = y.x, gb[e + 1] = y.y, gb[e + 2] = y.z, gb[e + 3] = y.w;
+          for (int e = 0; e < VEC; e += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(t.gamma + (IL ? da + 2 * e : da + e));
+            const float4 y = *reinterpret_cast<const float4*>(t.gamma + (IL ? da + 2 * e + 4 : db + e));
+            if (IL) {
+              ga[e] = x.x, gb[e] = x.y, ga[e + 1] = x.z, gb[e + 1] = x.w;
+              ga[e + 2] = y.x, gb[e + 2] = y.y, ga[e + 3] = y.z, gb[e + 3] = y.w;
+            } else {
+              ga[e] = x.x, ga[e + 1] = x.y, ga[e + 2] = x.z, ga[e + 3] = x.w;
+              gb[e] = y.x, gb[e + 1] = y.y, gb[e + 2] = y.z, gb[e + 3] = y.w;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            ga[e] = t.gamma[IL ? da + 2 * e : da + e];
+            gb[e] = t.gamma[IL ? da + 2 * e + 1 : db + e];
           }
         }
       }
@@ -220,8 +232,7 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotate_vec(const RotParams p, i
       for (int h = h0 + sub; h - sub < heads; h += hpw, off += off_step) {
         const bool on = mine && h < heads;
         asm volatile("cp.async.wait_group %0;" ::"n"(ROT_STAGES - 1) : "memory");
-        const Vec<T, VEC> ra = *reinterpret_cast<const Vec<T, VEC>*>(&ring[get][0][lane]);
-        const Vec<T, VEC> rb = *reinterpret_cast<const Vec<T, VEC>*>(&ring[get][1][lane]);
+        const Vec<T, VEC> ra = ring[get][0][lane], rb = ring[get][1][lane];
         get = get + 1 == ROT_STAGES ? 0 : get + 1;
         float a[VEC], b[VEC];
 #pragma unroll
@@ -341,28 +352,19 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotate_any(const RotParams p, i
   }
 }
 
-bool aligned16(const RotTensor& t, int es, int des) {
+// Whether a tensor's heads are whole vectors of `vec` values of es bytes (des
+// in the destination).
+bool rot_aligned(const RotTensor& t, int vec, int es, int des) {
   if (!t.heads) return true;
-  return reinterpret_cast<uintptr_t>(t.gamma) % 16 == 0 &&
-         reinterpret_cast<uintptr_t>(t.src) % 16 == 0 && (t.src_token * es) % 16 == 0 && (t.src_head * es) % 16 == 0 &&
-         // a destination vector is 16 bytes of the source type, so 8 where the cache is narrower
-         reinterpret_cast<uintptr_t>(t.dst) % (16 * des / es) == 0 && (t.dst_token * des) % (16 * des / es) == 0 &&
-         (t.dst_head * des) % (16 * des / es) == 0;
+  const auto ok = [vec](const void* base, int64_t token, int64_t head, int size) {
+    return reinterpret_cast<uintptr_t>(base) % (vec * size) == 0 && token % vec == 0 && head % vec == 0;
+  };
+  return (vec < 4 || reinterpret_cast<uintptr_t>(t.gamma) % 16 == 0) && ok(t.src, t.src_token, t.src_head, es) &&
+         ok(t.dst, t.dst_token, t.dst_head, des);
 }
 
-template <typename T, typename KV>
-int rotate_launch(const RotParams& p, int64_t n_tokens, int layout, cudaStream_t s) {
-  constexpr int VEC = 16 / (int)sizeof(T);
-  const int half = p.rot >> 1;
-  bool vec = p.dim % (2 * VEC) == 0 &&
-             (layout == ARMAI_ROPE_INTERLEAVED || (half % VEC == 0 && (p.dim - p.rot) % (2 * VEC) == 0));
-  for (int i = 0; i < 3; i++) vec = vec && aligned16(p.t[i], sizeof(T), i ? sizeof(KV) : sizeof(T));
-  if (!vec) {
-    const dim3 grid((unsigned)n_tokens, (unsigned)std::min<int64_t>((p.heads + 3) / 4, n_tokens < 64 ? 64 : 1));
-    k_rotate_any<T, KV><<<grid, ROT_THREADS, 0, s>>>(p, layout);
-    ARMAI_CUDA(cudaGetLastError());
-    return ARMAI_OK;
-  }
+template <typename T, typename KV, int VEC>
+int rotate_vectors(const RotParams& p, int64_t n_tokens, int layout, cudaStream_t s) {
   int hl = 1;
   while (hl * 2 * VEC < p.dim) hl <<= 1;
   const int hpw = 32 / hl;
@@ -374,12 +376,34 @@ int rotate_launch(const RotParams& p, int64_t n_tokens, int layout, cudaStream_t
   const int splits = few ? (int)items : 1;
   const int64_t ctas = std::min<int64_t>((n_tokens * splits + ROT_WARPS - 1) / ROT_WARPS,
                                          few ? INT32_MAX : ROT_CTAS * (int64_t)sm_count());
+  const float inv = 1.0f / (float)p.dim;
   if (layout == ARMAI_ROPE_INTERLEAVED)
-    k_rotate_vec<T, KV, true><<<(unsigned)ctas, ROT_THREADS, 0, s>>>(p, hl, n_tokens, splits, 1.0f / (float)p.dim);
+    k_rotate_vec<T, KV, true, VEC><<<(unsigned)ctas, ROT_THREADS, 0, s>>>(p, hl, n_tokens, splits, inv);
   else
-    k_rotate_vec<T, KV, false><<<(unsigned)ctas, ROT_THREADS, 0, s>>>(p, hl, n_tokens, splits, 1.0f / (float)p.dim);
+    k_rotate_vec<T, KV, false, VEC><<<(unsigned)ctas, ROT_THREADS, 0, s>>>(p, hl, n_tokens, splits, inv);
   ARMAI_CUDA(cudaGetLastError());
   return ARMAI_OK;
+}
+
+// The widest vectors that the head, its rotated part and the tensors' alignment
+// allow, a value at a time where none does (8191 tokens of 40 bf16 heads of 80,
+// half of each rotated by halves, so vectors of 4: 32 us against 143).
+template <typename T, typename KV, int VEC = 16 / (int)sizeof(T)>
+int rotate_launch(const RotParams& p, int64_t n_tokens, int layout, cudaStream_t s) {
+  const int half = p.rot >> 1;
+  bool fits = p.dim % (2 * VEC) == 0 && p.dim <= 64 * VEC &&
+              (layout == ARMAI_ROPE_INTERLEAVED || (half % VEC == 0 && (p.dim - p.rot) % (2 * VEC) == 0));
+  for (int i = 0; i < 3; i++) fits = fits && rot_aligned(p.t[i], VEC, sizeof(T), i ? sizeof(KV) : sizeof(T));
+  if (fits) return rotate_vectors<T, KV, VEC>(p, n_tokens, layout, s);
+  if constexpr (VEC > 2) {
+    return rotate_launch<T, KV, VEC / 2>(p, n_tokens, layout, s);
+  } else {
+    const int64_t y = std::max<int64_t>(16 * (int64_t)sm_count() / n_tokens, 1);
+    const dim3 grid((unsigned)n_tokens, (unsigned)std::min<int64_t>((p.heads + ROT_WARPS - 1) / ROT_WARPS, y));
+    k_rotate_any<T, KV><<<grid, ROT_THREADS, 0, s>>>(p, layout);
+    ARMAI_CUDA(cudaGetLastError());
+    return ARMAI_OK;
+  }
 }
 
 int rotate_dispatch(const RotParams& p, int64_t n_tokens, int dtype, int kv_dtype, int layout, cudaStream_t s) {

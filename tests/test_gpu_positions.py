@@ -273,3 +273,45 @@ def test_many_tokens_share_the_warps(built):
             exact, size = wr.rotate64(wr.norm64(x, gam, 1e-5), pos, f, layout)
             rope_close(got, exact, size, more=NORM)
         assert torch.equal(v_out, v)
+
+
+# ---- vectors narrower than 16 bytes ------------------------------------
+NARROW = [(9, 5, 80, 40), (3000, 3, 80, 40), (5, 2, 100, 100), (1100, 9, 100, 36), (4, 3, 52, 20), (2, 1, 4, 4),
+          (3, 2, 12, 8), (600, 7, 132, 132), (70, 3, 248, 124), (65, 33, 18, 10)]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("tokens,heads,dim,rot", NARROW)
+def test_rope_of_narrow_vectors(built, dtype, layout, tokens, heads, dim, rot):
+    test_rope_matches_definition(built, dtype, layout, tokens, heads, dim, rot)
+
+
+@pytest.mark.parametrize("dtype,kv", [(F32, F32), (F32, F16), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("tokens,hq,hkv,dim,rot", [(700, 6, 2, 80, 40), (5, 3, 1, 100, 100), (333, 4, 4, 100, 36),
+                                                  (40, 2, 1, 52, 20), (3, 2, 2, 248, 124)])
+def test_qk_norm_rope_of_narrow_vectors(built, dtype, kv, layout, tokens, hq, hkv, dim, rot):
+    test_qk_norm_rope_matches_definition(built, dtype, kv, layout, tokens, hq, hkv, dim, rot)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("shift,pad", [(4, 4), (2, 2), (1, 1), (0, 6), (8, 4)])
+@pytest.mark.parametrize("tokens", [3, 800])
+def test_rope_of_tensors_that_are_less_aligned(built, dtype, layout, shift, pad, tokens):
+    """Heads that start `shift` values behind an aligned address, `pad` values apart, in and out of place."""
+    g = gen(shift + pad)
+    buf = rnd(g, tokens * 3 * (64 + pad) + shift, dtype=dtype)
+    x = buf[shift:].view(tokens, 3, 64 + pad)[..., :64]
+    pos = torch.randint(0, 9000, (tokens,), generator=g, device="cuda")
+    f = freqs(48)
+    exact, size = wr.rotate64(x, pos, f, layout)
+    before = buf.clone()
+    out = torch.empty(tokens, 3, 64, dtype=dtype, device="cuda")
+    wr.rope(x, out, pos, f, layout)
+    rope_close(out, exact, size)
+    wr.rope(x, x, pos, f, layout)
+    assert torch.equal(x, out)
+    x.copy_(before[shift:].view(tokens, 3, 64 + pad)[..., :64])
+    assert torch.equal(buf, before)  # nothing between the heads was touched
