@@ -224,13 +224,13 @@ int ws_dim(const WaParams& p, int vec, cudaStream_t s) {
 
 }  // namespace
 
-bool wa_vectors(const WaParams& p, int dtype) {
+bool wa_aligned(const WaParams& p, int dtype, int bytes) {
   const int64_t es = dtype_size(dtype);
-  const auto ok = [&](int64_t stride) { return stride * es % 16 == 0; };
+  const auto ok = [&](int64_t values) { return values * es % bytes == 0; };
   return (reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
-          reinterpret_cast<uintptr_t>(p.out)) % 16 == 0 &&
-         ok(p.q_token) && ok(p.q_head) && ok(p.o_token) && ok(p.o_head) && ok(p.kv_slot) && ok(p.kv_head) &&
-         ok(p.kv_row);
+          reinterpret_cast<uintptr_t>(p.out)) % bytes == 0 &&
+         ok(p.head_dim) && ok(p.q_token) && ok(p.q_head) && ok(p.o_token) && ok(p.o_head) && ok(p.kv_slot) &&
+         ok(p.kv_head) && ok(p.kv_row);
 }
 
 namespace {
@@ -263,7 +263,7 @@ bool wa_split_better(const WaParams& p, int dtype) {
 }  // namespace
 
 int wa_simt_launch(const WaParams& p, int dtype, cudaStream_t s) {
-  if (dtype == ARMAI_F32) return ws_dim<float>(p, wa_vectors(p, dtype) && p.head_dim % 4 == 0, s);
+  if (dtype == ARMAI_F32) return ws_dim<float>(p, wa_aligned(p, dtype, 16), s);
   if (dtype == ARMAI_F16) return ws_dim<__half>(p, 0, s);
   return ws_dim<__nv_bfloat16>(p, 0, s);
 }
@@ -333,18 +333,16 @@ extern "C" int armai_dev_window_attention(const armai_window_attention_args* a, 
   p.ring = a->ring ? (int)(a->kv_rows - sink) : 0;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   const cudaStream_t s = (cudaStream_t)stream;
-  if (wa_vectors(p, a->dtype)) {
-    const bool split = wa_split_fits(p, a->dtype);
-    if (split && wa_split_better(p, a->dtype)) return wa_split_launch(p, a->dtype, s);
-    bool fits = false;
-    ARMAI_TRY(wa_tc_launch(p, a->dtype, s, &fits));
-    if (fits) return ARMAI_OK;
-    // 16-bit tensors that the 5th-generation tensor cores cannot take (heads
-    // wider than 128, strides of 0, a negative scale): reading the keys for
-    // every 16 rows is still faster than products on the CUDA cores (1024
-    // tokens, 8 heads of 256, bf16: 72 us against 535; 8192 rows of 4 heads on
-    // 4096 keys of 256: 2.7 ms against 10.3)
-    if (split && a->dtype != ARMAI_F32) return wa_split_launch(p, a->dtype, s);
-  }
+  const bool split = wa_split_fits(p, a->dtype);
+  if (split && wa_split_better(p, a->dtype)) return wa_split_launch(p, a->dtype, s);
+  bool fits = false;
+  if (wa_aligned(p, a->dtype, 16)) ARMAI_TRY(wa_tc_launch(p, a->dtype, s, &fits));
+  if (fits) return ARMAI_OK;
+  // 16-bit tensors that the 5th-generation tensor cores cannot take (heads
+  // wider than 128, strides of 0 or no 16 bytes, a negative scale): reading the
+  // keys for every 16 rows is still faster than products on the CUDA cores (1024
+  // tokens, 8 heads of 256, bf16: 72 us against 535; 8192 rows of 4 heads on
+  // 4096 keys of 256: 2.7 ms against 10.3)
+  if (split && a->dtype != ARMAI_F32) return wa_split_launch(p, a->dtype, s);
   return wa_simt_launch(p, a->dtype, s);
 }

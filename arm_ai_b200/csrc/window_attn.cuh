@@ -131,11 +131,11 @@ __device__ __forceinline__ int wa_tiles(const WaRuns& r) {
   return (r.len[0] + KT - 1) / KT + (r.len[1] + KT - 1) / KT + (r.len[2] + KT - 1) / KT;
 }
 
-// Every pointer and stride a whole number of 16-byte vectors.
-bool wa_vectors(const WaParams& p, int dtype);
+// Every pointer, stride and the head a whole number of so many bytes.
+bool wa_aligned(const WaParams& p, int dtype, int bytes);
 
 int wa_simt_launch(const WaParams& p, int dtype, cudaStream_t s);
-bool wa_split_fits(const WaParams& p, int dtype);  // of aligned tensors (wa_vectors)
+bool wa_split_fits(const WaParams& p, int dtype);
 int wa_split_launch(const WaParams& p, int dtype, cudaStream_t s);
 // Of aligned tensors; *fits false (and nothing launched): not this form's types,
 // widths, scale or strides.

@@ -49,6 +49,9 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp4_or_zero(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {
@@ -158,7 +161,7 @@ struct SpMail {
 // the rows. Every rank joins a share of the values; the others send it theirs
 // (remote stores: no latency to wait for). The caller has arrived at the
 // cluster's barrier before, so that every rank's mail box is there.
-template <typename T, int R, int DT>
+template <typename T, int R, int DT, int CB>
 __device__ __forceinline__ void sp_join(const WaParams& p, const SpBlock& b, const float* part, const float* wm,
                                         const float* wl, SpMail<R, DT>* mail) {
   constexpr int WARPS = sp_warps(DT);
@@ -170,7 +173,17 @@ __device__ __forceinline__ void sp_join(const WaParams& p, const SpBlock& b, con
     const int f = b.f0 + r, tok = wa_token(p, f);
     T* o = static_cast<T*>(p.out) + (int64_t)(b.sq.q0 + tok) * p.o_token +
            (int64_t)(b.kvh * p.group + f - tok * p.group) * p.o_head + d;
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (CB < 16) {
+      const float x[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+#pragma unroll
+      for (int e = 0; e < 4; e += 4 / (int)sizeof(T)) {
+        if (d + e >= p.head_dim) return;
+        if constexpr (sizeof(T) == 4)
+          o[e] = x[e];
+        else
+          *reinterpret_cast<uint32_t*>(o + e) = pack2<T>(x[e], x[e + 1]);
+      }
+    } else if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<float4*>(o) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     } else {
       *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
@@ -252,7 +265,9 @@ __host__ __device__ constexpr size_t sp_smem() {
   return ring > join ? ring : join;  // one after the other
 }
 
-template <typename T, int DT>
+// CB: bytes of a copy, 16 or (rows that do not start on 16 bytes, head widths
+// of no whole 16 bytes) 4.
+template <typename T, int DT, int CB>
 __global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p) {
   constexpr int WARPS = sp_warps(DT);
   constexpr int KC = DT / 32, VB = DT / 64;       // k chunks per key and lane; 64-wide blocks of v
@@ -272,8 +287,8 @@ __global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p
   const int ck = lane / RC, cc = lane % RC;
   const int64_t kv_off = (int64_t)b.sq.slot * p.kv_slot + (int64_t)b.kvh * p.kv_head;
   const int64_t row = p.kv_row, tile_stride = (int64_t)gridDim.x * WARPS * SP_KT * row;
-  const T* kb = static_cast<const T*>(p.k) + kv_off + ck * row + 8 * cc;
-  const T* vb = static_cast<const T*>(p.v) + kv_off + ck * row + 8 * cc;
+  const T* kb = static_cast<const T*>(p.k) + kv_off + (CB == 16 ? ck * row + 8 * cc : 2 * lane);
+  const T* vb = static_cast<const T*>(p.v) + kv_off + (CB == 16 ? ck * row + 8 * cc : 2 * lane);
   const uint8_t* ring = sm + warp * (SP_STAGES * 2 * TILE);
   const uint32_t ring32 = smem_u32(ring);
   const int step = (int)gridDim.x * WARPS, first = (int)blockIdx.x * WARPS + warp;
@@ -285,19 +300,33 @@ __global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p
       const int n = ahead.keys();
       const T* k = kb + at;
       const T* v = vb + at;
+      if constexpr (CB == 16) {
 #pragma unroll
-      for (int i = 0; i < SP_KT / RPC; i++) {
-        const int key = ck + RPC * i;
-        const uint32_t dk = dst + key * (RC * 16) + ((cc ^ sp_swz_k(key)) << 4);
-        const uint32_t dv = dst + TILE + key * (RC * 16) + ((cc ^ sp_swz_v(key)) << 4);
-        if (whole && n == SP_KT) {
-          cp16(dk, k + RPC * i * row);
-          cp16(dv, v + RPC * i * row);
-        } else {  // keys behind a short tile's end and chunks behind the head are zero
-          const bool ok = key < n && cc < chunks;
-          cp16_or_zero(dk, ok ? k + RPC * i * row : static_cast<const T*>(p.k), ok);
-          cp16_or_zero(dv, ok ? v + RPC * i * row : static_cast<const T*>(p.v), ok);
+        for (int i = 0; i < SP_KT / RPC; i++) {
+          const int key = ck + RPC * i;
+          const uint32_t dk = dst + key * (RC * 16) + ((cc ^ sp_swz_k(key)) << 4);
+          const uint32_t dv = dst + TILE + key * (RC * 16) + ((cc ^ sp_swz_v(key)) << 4);
+          if (whole && n == SP_KT) {
+            cp16(dk, k + RPC * i * row);
+            cp16(dv, v + RPC * i * row);
+          } else {  // keys behind a short tile's end and chunks behind the head are zero
+            const bool ok = key < n && cc < chunks;
+            cp16_or_zero(dk, ok ? k + RPC * i * row : static_cast<const T*>(p.k), ok);
+            cp16_or_zero(dv, ok ? v + RPC * i * row : static_cast<const T*>(p.v), ok);
+          }
         }
+      } else {
+        // words lane + 32 i of a row, consecutive lanes consecutive words
+#pragma unroll 4
+        for (int key = 0; key < SP_KT; key++)
+#pragma unroll
+          for (int i = 0; i < DT / 64; i++) {
+            const int word = lane + 32 * i, x = word >> 2;
+            const bool ok = key < n && 2 * word < p.head_dim;
+            const uint32_t at = dst + key * (RC * 16) + (word & 3) * 4;
+            cp4_or_zero(at + ((x ^ sp_swz_k(key)) << 4), ok ? k + key * row + 64 * i : static_cast<const T*>(p.k), ok);
+            cp4_or_zero(at + TILE + ((x ^ sp_swz_v(key)) << 4), ok ? v + key * row + 64 * i : static_cast<const T*>(p.v), ok);
+          }
       }
       const int run = ahead.run;
       ahead.advance(b.runs, step);
@@ -324,7 +353,15 @@ __global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p
 #pragma unroll
     for (int i = 0; i < KC; i++) {
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (r < b.nr && c + 4 * i < chunks) v = *reinterpret_cast<const uint4*>(src + 8 * (c + 4 * i));
+      if constexpr (CB == 16) {
+        if (r < b.nr && c + 4 * i < chunks) v = *reinterpret_cast<const uint4*>(src + 8 * (c + 4 * i));
+      } else {
+        const auto word = [&](int d) {
+          return r < b.nr && d < p.head_dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+        };
+        const int d = 8 * (c + 4 * i);
+        v = make_uint4(word(d), word(d + 2), word(d + 4), word(d + 6));
+      }
       qa[i][0][j] = v.x ^ flip;
       qa[i][0][2 + j] = v.y ^ flip;
       qa[i][1][j] = v.z ^ flip;
@@ -453,7 +490,7 @@ __global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p
           *reinterpret_cast<float4*>(part + (warp * SP_ROWS + r) * DT + 64 * i + 16 * c + 8 * n + e) =
               make_float4(o[i][e][2 * j + n], o[i][e + 1][2 * j + n], o[i][e + 2][2 * j + n], o[i][e + 3][2 * j + n]);
   }
-  sp_join<T, SP_ROWS, DT>(p, b, part, wm, wl, reinterpret_cast<SpMail<SP_ROWS, DT>*>(sm + sp_smem<T, DT>()));
+  sp_join<T, SP_ROWS, DT, CB>(p, b, part, wm, wl, reinterpret_cast<SpMail<SP_ROWS, DT>*>(sm + sp_smem<T, DT>()));
 }
 
 // ---------------------------------------------------------------------------
@@ -471,7 +508,7 @@ __host__ __device__ constexpr size_t sf_smem(int rows) {
   return ring > join ? ring : join;  // one after the other
 }
 
-template <int R, int CH>
+template <int R, int CH, int CB>
 __global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const WaParams p) {
   constexpr int DT = 32 * CH, WARPS = sp_warps(DT);
   constexpr int SH = R == 8 ? 0 : R == 4 ? 1 : R == 2 ? 2 : 3;  // lanes per row of the 8: 2^SH
@@ -498,9 +535,19 @@ __global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const W
         const int64_t off = (int64_t)(x.row + (key < x.n ? key : 0)) * p.kv_row;
 #pragma unroll
         for (int i = 0; i < CH; i++) {
-          const bool ok = key < x.n && x8 + 8 * i < chunks;
-          cp16_or_zero(smem_u32(dst + (j * CH + i) * 32), kb + off + (ok ? 4 * (x8 + 8 * i) : 0), ok);
-          cp16_or_zero(smem_u32(dst + ((2 + j) * CH + i) * 32), vb + off + (ok ? 4 * (x8 + 8 * i) : 0), ok);
+          if constexpr (CB == 16) {
+            const bool ok = key < x.n && x8 + 8 * i < chunks;
+            cp16_or_zero(smem_u32(dst + (j * CH + i) * 32), kb + off + (ok ? 4 * (x8 + 8 * i) : 0), ok);
+            cp16_or_zero(smem_u32(dst + ((2 + j) * CH + i) * 32), vb + off + (ok ? 4 * (x8 + 8 * i) : 0), ok);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int d = 4 * (x8 + 8 * i) + e;
+              const bool ok = key < x.n && d < p.head_dim;
+              cp4_or_zero(smem_u32(dst + (j * CH + i) * 32) + 4 * e, kb + off + (ok ? d : 0), ok);
+              cp4_or_zero(smem_u32(dst + ((2 + j) * CH + i) * 32) + 4 * e, vb + off + (ok ? d : 0), ok);
+            }
+          }
         }
       }
     }
@@ -520,8 +567,14 @@ __global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const W
     for (int i = 0; i < CH; i++) {
       o[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
       q[r][i] = o[r][i];
-      if (r < b.nr && x8 + 8 * i < chunks) {
-        const float4 v = *reinterpret_cast<const float4*>(src + 4 * (x8 + 8 * i));
+      const int d = 4 * (x8 + 8 * i);
+      if (r < b.nr && (CB == 16 ? x8 + 8 * i < chunks : d < p.head_dim)) {
+        float4 v;
+        if constexpr (CB == 16)
+          v = *reinterpret_cast<const float4*>(src + d);
+        else
+          v = make_float4(src[d], d + 1 < p.head_dim ? src[d + 1] : 0.f, d + 2 < p.head_dim ? src[d + 2] : 0.f,
+                          d + 3 < p.head_dim ? src[d + 3] : 0.f);
         q[r][i] = make_float4(v.x * p.scale_log2, v.y * p.scale_log2, v.z * p.scale_log2, v.w * p.scale_log2);
       }
     }
@@ -633,7 +686,7 @@ __global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const W
       }
       if (kg == 0) *reinterpret_cast<float4*>(part + (warp * R + r) * DT + 4 * (x8 + 8 * i)) = v;
     }
-  sp_join<float, R, DT>(p, b, part, wm, wl, reinterpret_cast<SpMail<R, DT>*>(sm + sf_smem<CH>(R)));
+  sp_join<float, R, DT, CB>(p, b, part, wm, wl, reinterpret_cast<SpMail<R, DT>*>(sm + sf_smem<CH>(R)));
 }
 
 // Clusters of 2^log2 CTAs that the device holds at once (with one CTA per SM
@@ -696,59 +749,65 @@ int sp_launch(size_t smem, const WaParams& p, int rows, int kt, int warps, cudaS
   return ARMAI_OK;
 }
 
-template <typename T, int DT>
+template <typename T, int DT, int CB>
 int sp_width(const WaParams& p, cudaStream_t s) {
-  return sp_launch<k_wa_split<T, DT>>(sp_smem<T, DT>() + sizeof(SpMail<SP_ROWS, DT>), p, SP_ROWS, SP_KT, sp_warps(DT), s);
+  return sp_launch<k_wa_split<T, DT, CB>>(sp_smem<T, DT>() + sizeof(SpMail<SP_ROWS, DT>), p, SP_ROWS, SP_KT, sp_warps(DT),
+                                          s);
 }
-template <typename T>
+template <typename T, int CB>
 int sp_half(const WaParams& p, cudaStream_t s) {
-  if (p.head_dim <= 64) return sp_width<T, 64>(p, s);
-  if (p.head_dim <= 128) return sp_width<T, 128>(p, s);
-  return sp_width<T, 256>(p, s);
+  if (p.head_dim <= 64) return sp_width<T, 64, CB>(p, s);
+  if (p.head_dim <= 128) return sp_width<T, 128, CB>(p, s);
+  return sp_width<T, 256, CB>(p, s);
 }
 
-template <int R, int CH>
+template <int R, int CH, int CB>
 int sp_f32(const WaParams& p, cudaStream_t s) {
-  return sp_launch<k_wa_split_f32<R, CH>>(sf_smem<CH>(R) + sizeof(SpMail<R, 32 * CH>), p, R, SF_KT, sp_warps(32 * CH), s);
+  return sp_launch<k_wa_split_f32<R, CH, CB>>(sf_smem<CH>(R) + sizeof(SpMail<R, 32 * CH>), p, R, SF_KT, sp_warps(32 * CH),
+                                              s);
 }
 // Rows per CTA as many as there are, up to eight; four or two at the widths
 // where more rows of q and of the output would not fit the registers.
 int sf_rows(int head_dim) { return head_dim <= 64 ? 8 : head_dim <= 128 ? 4 : 2; }
-template <int CH>
+template <int CH, int CB>
 int sp_f32_rows(const WaParams& p, cudaStream_t s) {
   const int64_t pairs = (int64_t)p.max_q * p.group;
-  if (pairs <= 1) return sp_f32<1, CH>(p, s);
+  if (pairs <= 1) return sp_f32<1, CH, CB>(p, s);
   if constexpr (CH <= 4) {
-    if (pairs > 2 && (CH > 2 || pairs <= 4)) return sp_f32<4, CH>(p, s);
+    if (pairs > 2 && (CH > 2 || pairs <= 4)) return sp_f32<4, CH, CB>(p, s);
   }
   if constexpr (CH <= 2) {
-    if (pairs > 4) return sp_f32<8, CH>(p, s);
+    if (pairs > 4) return sp_f32<8, CH, CB>(p, s);
   }
-  return sp_f32<2, CH>(p, s);
+  return sp_f32<2, CH, CB>(p, s);
+}
+template <int CB>
+int sp_launch_by_type(const WaParams& p, int dtype, cudaStream_t s) {
+  if (dtype == ARMAI_F16) return sp_half<__half, CB>(p, s);
+  if (dtype == ARMAI_BF16) return sp_half<__nv_bfloat16, CB>(p, s);
+  switch ((p.head_dim + 31) / 32) {
+    case 1: return sp_f32_rows<1, CB>(p, s);
+    case 2: return sp_f32_rows<2, CB>(p, s);
+    case 3: return sp_f32_rows<3, CB>(p, s);
+    case 4: return sp_f32_rows<4, CB>(p, s);
+    case 5:
+    case 6: return sp_f32_rows<6, CB>(p, s);
+    default: return sp_f32_rows<8, CB>(p, s);
+  }
 }
 
 }  // namespace
 
-// Head widths of whole 16-byte vectors, and heads that fit the grid.
+// Tensors of whole 16-byte vectors or 4-byte words, and heads that fit the grid.
 bool wa_split_fits(const WaParams& p, int dtype) {
-  const int v = 16 / dtype_size(dtype), rows = dtype == ARMAI_F32 ? sf_rows(p.head_dim) : SP_ROWS;
+  const int rows = dtype == ARMAI_F32 ? sf_rows(p.head_dim) : SP_ROWS;
   const int64_t pairs = (int64_t)p.max_q * p.group;
-  return p.head_dim % v == 0 && p.scale_log2 != 0.f && p.scale_log2 == p.scale_log2 &&
+  return wa_aligned(p, dtype, 4) && p.scale_log2 != 0.f && p.scale_log2 == p.scale_log2 &&
          pairs * p.group < int64_t(1) << 32 && (pairs + rows - 1) / rows * p.n_kv <= 65535;
 }
 
 int wa_split_launch(const WaParams& p, int dtype, cudaStream_t s) {
-  if (dtype == ARMAI_F16) return sp_half<__half>(p, s);
-  if (dtype == ARMAI_BF16) return sp_half<__nv_bfloat16>(p, s);
-  switch ((p.head_dim + 31) / 32) {
-    case 1: return sp_f32_rows<1>(p, s);
-    case 2: return sp_f32_rows<2>(p, s);
-    case 3: return sp_f32_rows<3>(p, s);
-    case 4: return sp_f32_rows<4>(p, s);
-    case 5:
-    case 6: return sp_f32_rows<6>(p, s);
-    default: return sp_f32_rows<8>(p, s);
-  }
+  return wa_aligned(p, dtype, 16) ? sp_launch_by_type<16>(p, dtype, s) : sp_launch_by_type<4>(p, dtype, s);
 }
 
 }  // namespace armai

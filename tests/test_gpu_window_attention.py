@@ -4,6 +4,7 @@ chunks behind a cache, single tokens; linear and ring caches; grouped heads;
 every type. The bound of each element's error is derived in
 window_reference.attention64 from the roundings that the kernels make."""
 import ctypes
+import math
 
 import pytest
 
@@ -509,3 +510,37 @@ def test_scale_zero_averages(built):
         out = torch.empty_like(qq)
         wr.window_attention(qq, k, v, out, i32([100]), 30, 2, False, scale=0.0)
         wr.close(out, *wr.attention64(qq, k, v, [40], [100], 30, 2, scale=0.0))
+
+
+# ---- heads and rows of no whole 16 bytes -------------------------------
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 100), (3, 3, 98), (16, 2, 36), (4, 1, 130), (2, 2, 250), (5, 1, 2), (4, 2, 63)])
+@pytest.mark.parametrize("q_lens,past,window,n_sink,ring", [
+    ([1, 1, 1, 1], [0, 62, 700, 3099], 1000, 4, False),
+    ([1, 1], [5000, 1030], 1024, 0, True),
+    ([3, 1, 8], [300, 0, 2], 90, 2, True),
+    ([40, 7, 150], [0, 1000, 31], 64, 1, False),
+])
+def test_heads_of_no_whole_vectors(built, dtype, hq, hkv, d, q_lens, past, window, n_sink, ring):
+    run(gen(sum(past) + d), dtype, hq, hkv, d, q_lens, [a + b for a, b in zip(past, q_lens)], window, n_sink, ring,
+        extra=2)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d,shift,pad", [(64, 2, 2), (128, 1, 1), (96, 0, 4), (64, 4, 12)])
+@pytest.mark.parametrize("q", [1, 90])
+def test_tensors_that_are_less_aligned(built, dtype, d, shift, pad, q):
+    """Every tensor starts `shift` values behind an aligned address, its rows `pad` values apart."""
+    g = gen(d + shift)
+    rows = 400
+
+    def view(*shape):
+        n = math.prod(shape) * (d + pad) + shift
+        return rnd(g, n, dtype=dtype)[shift:].view(*shape, d + pad)[..., :d]
+
+    qq, k, v, out = view(2 * q, 8), view(2, 2, rows), view(2, 2, rows), view(2 * q, 8)
+    around = out._base.clone()
+    wr.window_attention(qq, k, v, out, i32([rows, 123]), 150, 3, False)
+    wr.close(out, *wr.attention64(qq, k, v, [q, q], [rows, 123], 150, 3))
+    out.copy_(around[shift:].view(2 * q, 8, d + pad)[..., :d])
+    assert torch.equal(out._base, around)  # nothing between the rows was touched
