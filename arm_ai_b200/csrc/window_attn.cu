@@ -44,8 +44,8 @@ __device__ __forceinline__ void ws_fma2(float2& c, float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
 }
 
-// n rows of head_dim values into shared rows of DM f32 (zeros behind them);
-// `vec`: f32 rows of whole 16-byte vectors, copied asynchronously.
+// n rows of head_dim values into shared rows of DM f32 (zeros behind them), f32
+// copied asynchronously; `vec`: rows of whole 16-byte vectors.
 template <typename T, int DM, int ROWS, int THREADS>
 __device__ __forceinline__ void ws_rows(float* dst, const T* src, int64_t stride, int n, int D, bool vec) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -60,8 +60,21 @@ __device__ __forceinline__ void ws_rows(float* dst, const T* src, int64_t stride
     }
     return;
   }
-  for (int r = warp; r < ROWS; r += THREADS / 32)
-    for (int d = lane; d < DM; d += 32) dst[r * (DM + 4) + d] = r < n && d < D ? to_f32(src[r * stride + d]) : 0.f;
+  if constexpr (sizeof(T) == 4) {  // a value at a time, asynchronously all the same
+    for (int r = warp; r < ROWS; r += THREADS / 32)
+      for (int d = lane; d < DM; d += 32) {
+        const bool ok = r < n && d < D;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                         (uint32_t)__cvta_generic_to_shared(dst + r * (DM + 4) + d)),
+                     "l"(ok ? src + r * stride + d : src), "r"(ok ? 4 : 0)
+                     : "memory");
+      }
+  } else {
+#pragma unroll 4
+    for (int r = warp; r < ROWS; r += THREADS / 32)
+#pragma unroll
+      for (int d = lane; d < DM; d += 32) dst[r * (DM + 4) + d] = r < n && d < D ? to_f32(src[r * stride + d]) : 0.f;
+  }
 }
 
 template <typename T, int DM, int Q>
