@@ -102,12 +102,12 @@ struct SpBlock {
   WaRuns runs;
 };
 template <int R>
-__device__ __forceinline__ bool sp_block(const WaParams& p, SpBlock& b) {
-  // blockIdx.y: key / value head, then block of rows (one, for single tokens)
-  const int rb = (int)gridDim.y == p.n_kv ? 0 : (int)blockIdx.y / p.n_kv;
-  b.kvh = (int)blockIdx.y - rb * p.n_kv;
+__device__ __forceinline__ bool sp_block(const WaParams& p, int split, SpBlock& b) {
+  // blockIdx.x: rank of 2^split in the cluster, key / value head, block of rows (one, for single tokens)
+  const int block = (int)blockIdx.x >> split, rb = (int)gridDim.x >> split == p.n_kv ? 0 : block / p.n_kv;
+  b.kvh = block - rb * p.n_kv;
   b.f0 = rb * R;
-  b.sq = wa_seq(p, blockIdx.z);
+  b.sq = wa_seq(p, blockIdx.y);
   b.nr = min(R, b.sq.n * p.group - b.f0);
   if (b.nr <= 0) return false;  // the same for the whole cluster
   b.qmin = b.sq.pos0 + wa_token(p, b.f0);
@@ -162,11 +162,11 @@ struct SpMail {
 // (remote stores: no latency to wait for). The caller has arrived at the
 // cluster's barrier before, so that every rank's mail box is there.
 template <typename T, int R, int DT, int CB>
-__device__ __forceinline__ void sp_join(const WaParams& p, const SpBlock& b, const float* part, const float* wm,
-                                        const float* wl, SpMail<R, DT>* mail) {
+__device__ __forceinline__ void sp_join(const WaParams& p, int split, const SpBlock& b, const float* part,
+                                        const float* wm, const float* wl, SpMail<R, DT>* mail) {
   constexpr int WARPS = sp_warps(DT);
   const int tid = threadIdx.x, items = b.nr * (DT / 4);
-  const int ranks = (int)gridDim.x, rank = (int)blockIdx.x, per = (items + ranks - 1) / ranks;
+  const int ranks = 1 << split, rank = (int)blockIdx.x & (ranks - 1), per = (items + ranks - 1) / ranks;
   auto write = [&](int r, int d, const float4& acc, float l) {
     if (d >= p.head_dim) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;  // an empty row: 0 * 0; NaN kept
@@ -268,15 +268,15 @@ __host__ __device__ constexpr size_t sp_smem() {
 // CB: bytes of a copy, 16 or (rows that do not start on 16 bytes, head widths
 // of no whole 16 bytes) 4.
 template <typename T, int DT, int CB>
-__global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p) {
+__global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p, int split) {
   constexpr int WARPS = sp_warps(DT);
   constexpr int KC = DT / 32, VB = DT / 64;       // k chunks per key and lane; 64-wide blocks of v
   constexpr uint32_t TILE = SP_KT * DT * 2;       // a tile of K or V
   extern __shared__ __align__(16) uint8_t sm[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   SpBlock b;
-  if (!sp_block<SP_ROWS>(p, b)) return;
-  if (gridDim.x > 1) sp_cluster_arrive();
+  if (!sp_block<SP_ROWS>(p, split, b)) return;
+  if (split) sp_cluster_arrive();
   const int chunks = p.head_dim >> 3;             // valid 16-byte chunks of a row
   const bool whole = p.head_dim == DT;
   // copies: 16-byte chunk cc of key ck + RPC i, consecutive lanes consecutive
@@ -286,12 +286,12 @@ __global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p
   constexpr int RC = DT / 8, RPC = 32 / RC;       // chunks per row, rows per copy instruction
   const int ck = lane / RC, cc = lane % RC;
   const int64_t kv_off = (int64_t)b.sq.slot * p.kv_slot + (int64_t)b.kvh * p.kv_head;
-  const int64_t row = p.kv_row, tile_stride = (int64_t)gridDim.x * WARPS * SP_KT * row;
+  const int64_t row = p.kv_row, tile_stride = (int64_t)(WARPS * SP_KT << split) * row;
   const T* kb = static_cast<const T*>(p.k) + kv_off + (CB == 16 ? ck * row + 8 * cc : 2 * lane);
   const T* vb = static_cast<const T*>(p.v) + kv_off + (CB == 16 ? ck * row + 8 * cc : 2 * lane);
   const uint8_t* ring = sm + warp * (SP_STAGES * 2 * TILE);
   const uint32_t ring32 = smem_u32(ring);
-  const int step = (int)gridDim.x * WARPS, first = (int)blockIdx.x * WARPS + warp;
+  const int step = WARPS << split, first = ((int)blockIdx.x & ((1 << split) - 1)) * WARPS + warp;
 
   SpCursor<SP_KT> cur(b.runs, first), ahead = cur;
   int64_t at = (int64_t)ahead.first_row() * row;  // of the loads' tile, in values from kb and vb
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p
           *reinterpret_cast<float4*>(part + (warp * SP_ROWS + r) * DT + 64 * i + 16 * c + 8 * n + e) =
               make_float4(o[i][e][2 * j + n], o[i][e + 1][2 * j + n], o[i][e + 2][2 * j + n], o[i][e + 3][2 * j + n]);
   }
-  sp_join<T, SP_ROWS, DT, CB>(p, b, part, wm, wl, reinterpret_cast<SpMail<SP_ROWS, DT>*>(sm + sp_smem<T, DT>()));
+  sp_join<T, SP_ROWS, DT, CB>(p, split, b, part, wm, wl, reinterpret_cast<SpMail<SP_ROWS, DT>*>(sm + sp_smem<T, DT>()));
 }
 
 // ---------------------------------------------------------------------------
@@ -509,20 +509,20 @@ __host__ __device__ constexpr size_t sf_smem(int rows) {
 }
 
 template <int R, int CH, int CB>
-__global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const WaParams p) {
+__global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const WaParams p, int split) {
   constexpr int DT = 32 * CH, WARPS = sp_warps(DT);
   constexpr int SH = R == 8 ? 0 : R == 4 ? 1 : R == 2 ? 2 : 3;  // lanes per row of the 8: 2^SH
   extern __shared__ __align__(16) uint8_t sm[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kg = lane >> 3, x8 = lane & 7;
   SpBlock b;
-  if (!sp_block<R>(p, b)) return;
-  if (gridDim.x > 1) sp_cluster_arrive();
+  if (!sp_block<R>(p, split, b)) return;
+  if (split) sp_cluster_arrive();
   const int chunks = p.head_dim >> 2;
   const int64_t kv_off = (int64_t)b.sq.slot * p.kv_slot + (int64_t)b.kvh * p.kv_head;
   const float* kb = static_cast<const float*>(p.k) + kv_off;
   const float* vb = static_cast<const float*>(p.v) + kv_off;
   float4* ring = reinterpret_cast<float4*>(sm) + warp * (SP_STAGES * 4 * CH * 32) + lane;
-  const int step = (int)gridDim.x * WARPS, first = (int)blockIdx.x * WARPS + warp;
+  const int step = WARPS << split, first = ((int)blockIdx.x & ((1 << split) - 1)) * WARPS + warp;
   const int nt = wa_tiles<SF_KT>(b.runs);
 
   auto load = [&](int t, int slot) {
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const W
       }
       if (kg == 0) *reinterpret_cast<float4*>(part + (warp * R + r) * DT + 4 * (x8 + 8 * i)) = v;
     }
-  sp_join<float, R, DT, CB>(p, b, part, wm, wl, reinterpret_cast<SpMail<R, DT>*>(sm + sf_smem<CH>(R)));
+  sp_join<float, R, DT, CB>(p, split, b, part, wm, wl, reinterpret_cast<SpMail<R, DT>*>(sm + sf_smem<CH>(R)));
 }
 
 // Clusters of 2^log2 CTAs that the device holds at once (with one CTA per SM
@@ -723,7 +723,7 @@ int sp_launch(size_t smem, const WaParams& p, int rows, int kt, int warps, cudaS
   const int64_t keys = std::min<int64_t>(p.kv_rows, (int64_t)p.window + p.n_sink + span);
   ARMAI_CUDA(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(SP_MAX_SPLIT, (unsigned)blocks, (unsigned)p.n_seq);
+  cfg.gridDim = dim3((unsigned)(SP_MAX_SPLIT * blocks), (unsigned)p.n_seq);
   cfg.blockDim = dim3(32 * warps);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -732,7 +732,7 @@ int sp_launch(size_t smem, const WaParams& p, int rows, int kt, int warps, cudaS
   attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  int split = 1;
+  int split = 0;
   for (int log2 = 1; 1 << log2 <= SP_MAX_SPLIT; log2++) {
     const int n = 1 << log2;
     const int64_t clusters = blocks * p.n_seq;
@@ -742,10 +742,11 @@ int sp_launch(size_t smem, const WaParams& p, int rows, int kt, int warps, cudaS
     const int active = sp_active<K>(log2, cfg);
     const bool several = active * n > sm_count();
     if (several ? clusters * 15 > (int64_t)active * 16 : clusters > active) break;
-    split = n;
+    split = log2;
   }
-  cfg.gridDim.x = attr[0].val.clusterDim.x = (unsigned)split;
-  ARMAI_CUDA(cudaLaunchKernelEx(&cfg, K, p));
+  cfg.gridDim.x = (unsigned)(blocks << split);
+  attr[0].val.clusterDim.x = 1u << split;
+  ARMAI_CUDA(cudaLaunchKernelEx(&cfg, K, p, split));
   return ARMAI_OK;
 }
 
@@ -803,7 +804,7 @@ bool wa_split_fits(const WaParams& p, int dtype) {
   const int rows = dtype == ARMAI_F32 ? sf_rows(p.head_dim) : SP_ROWS;
   const int64_t pairs = (int64_t)p.max_q * p.group;
   return wa_aligned(p, dtype, 4) && p.scale_log2 != 0.f && p.scale_log2 == p.scale_log2 &&
-         pairs * p.group < int64_t(1) << 32 && (pairs + rows - 1) / rows * p.n_kv <= 65535;
+         pairs * p.group < int64_t(1) << 32 && (pairs + rows - 1) / rows * p.n_kv * SP_MAX_SPLIT <= 0x7fffffff;
 }
 
 int wa_split_launch(const WaParams& p, int dtype, cudaStream_t s) {

@@ -362,6 +362,21 @@ def test_many_queries_of_wide_heads(built, dtype, hq, hkv, d, q_lens, past, wind
         extra=3)
 
 
+def test_more_than_65536_blocks_of_rows(built):
+    """One call with many heads gives what calls with parts of the heads give."""
+    g = gen(31)
+    q, hq, hkv, d = 1100, 1024, 16, 136
+    qq, k, v = (rnd(g, *s, dtype=BF16) for s in ((q, hq, d), (1, hkv, q, d), (1, hkv, q, d)))
+    out, part = torch.empty_like(qq), torch.empty_like(qq)
+    wr.window_attention(qq, k, v, out, i32([q]), 300, 2, False)
+    for i in range(0, hkv, 4):
+        h = slice(i * (hq // hkv), (i + 4) * (hq // hkv))
+        wr.window_attention(qq[:, h], k[:, i:i + 4], v[:, i:i + 4], part[:, h], i32([q]), 300, 2, False)
+    assert torch.equal(out, part)
+    h = slice(hq - hq // hkv, hq)
+    wr.close(out[:, h], *wr.attention64(qq[:, h], k[:, -1:], v[:, -1:], [q], [q], 300, 2))
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("hq,hkv,d", [(8, 2, 256), (5, 1, 192), (3, 3, 160), (12, 4, 132), (4, 1, 248)])
 @pytest.mark.parametrize("q_lens,past,window,n_sink,ring", [
