@@ -10,7 +10,7 @@
 // of operations between. A warp has a token at a time: it makes the token's
 // cosines and sines once (instead of once per head), and a lane keeps its own,
 // and its gains, in registers for all heads. A power-of-two group of lanes holds a
-// head; a lane has both members of its pairs (two 16-byte vectors), so the
+// head; a lane has both members of its pairs (two vectors), so the
 // rotation needs no exchange and the norm's sum a few shuffles per head.
 #include <algorithm>
 #include <cmath>

@@ -5,8 +5,8 @@
 // Bound by the bytes of the visible keys and values. A warp takes tiles of 16
 // keys in turn with the cluster's other warps and keeps its own running
 // maximum, sum and output, so no warp waits for another until the end. Its
-// tiles arrive by asynchronous 16-byte copies, whole lines at a time, into a
-// two-deep ring of its own. The order of the values within a row is free in
+// tiles arrive by asynchronous 16-byte copies (4-byte ones where rows do not
+// start on 16 bytes), whole lines at a time, into a two-deep ring of its own. The order of the values within a row is free in
 // both products, as long as q and k (or p and v) agree, so each lane's operands
 // are whole 16-byte chunks.
 //   16-bit types: m16n8k16 tensor instructions, 16 rows = (token, query head)
