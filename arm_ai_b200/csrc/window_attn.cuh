@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "dev_call.cuh"
 
 namespace armai {
@@ -110,6 +112,22 @@ __device__ __forceinline__ WaRuns wa_runs(const WaParams& p, int plo, int phi) {
 __device__ __forceinline__ bool wa_sees(const WaParams& p, int qpos, int kpos) {
   return kpos <= qpos && (qpos - kpos < p.window || kpos < p.n_sink);
 }
+
+// The running maximum is raised (and the output rescaled) only when a score
+// exceeds it by more than this many powers of two: the weights stay below 2^8
+// times their largest and their sum far inside f32, and most tiles need no pass
+// over the output.
+constexpr float WA_SLACK = 8.f;
+// The weights of 16-bit tensors are exp2(score - maximum + this), rounded to
+// the tensors' type for P V; the f32 sum has the same factor, which cancels. f16
+// runs out of exponents: from 2^-14 down a weight loses bits. Seven powers of two
+// up its largest is 2^15 (with the slack; f16 ends below 2^16), and a weight is
+// rounded to half a step, 2^-11 of itself, down to 2^-21 of the row's largest, and
+// to 2^-32 of the largest below. (Keys 17 nats below a first token whose value is
+// 0: with no factor an output 44 % off, the weights being rounded to 2^-24 or 0.)
+// bf16 has f32's exponents.
+template <typename T>
+__host__ __device__ constexpr float wa_weight_shift() { return std::is_same<T, __half>::value ? 7.f : 0.f; }
 
 // Tile t of KT keys of the runs: its first cache row, first position and keys.
 struct WaTile {

@@ -38,10 +38,6 @@ namespace {
 __host__ __device__ constexpr int sp_warps(int dt) { return dt > 128 ? 6 : 4; }
 constexpr int SP_STAGES = 2;
 constexpr int SP_MAX_SPLIT = 16;
-// The running maximum is raised (and the output rescaled) only when a score
-// exceeds it by more than this many powers of two: the weights stay below 2^8
-// and their sum far inside f32, and most tiles need no exchange between lanes.
-constexpr float SP_SLACK = 8.f;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -422,7 +418,7 @@ __global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p
     }
     const float top[2] = {fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])) * sl,
                           fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])) * sl};
-    if (__any_sync(0xffffffffu, top[0] > m[0] + SP_SLACK || top[1] > m[1] + SP_SLACK)) {
+    if (__any_sync(0xffffffffu, top[0] > m[0] + WA_SLACK || top[1] > m[1] + WA_SLACK)) {
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         float y = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 1));
@@ -443,11 +439,11 @@ __global__ void __launch_bounds__(32 * sp_warps(DT)) k_wa_split(const WaParams p
     uint32_t pa[4];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      const float base = m[j] == -INFINITY ? 0.f : m[j];
+      const float base = (m[j] == -INFINITY ? 0.f : m[j]) - wa_weight_shift<T>();
       const float p0 = sp_exp2(fmaf(s[0][2 * j], sl, -base)), p1 = sp_exp2(fmaf(s[0][2 * j + 1], sl, -base));
       const float p2 = sp_exp2(fmaf(s[1][2 * j], sl, -base)), p3 = sp_exp2(fmaf(s[1][2 * j + 1], sl, -base));
       l[j] += (p0 + p1) + (p2 + p3);
-      pa[j] = pack2<T>(p0, p1);      // rounded to T for the product: half a step of each weight
+      pa[j] = pack2<T>(p0, p1);      // rounded to T for the product, see wa_weight_shift
       pa[2 + j] = pack2<T>(p2, p3);
     }
 #pragma unroll
@@ -622,7 +618,7 @@ __global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const W
       s[j] = key < x.n && wa_sees(p, qpos, x.pos + key) ? d[0] : -INFINITY;
     }
     const float top = fmaxf(s[0], s[1]);
-    if (__any_sync(0xffffffffu, top > m + SP_SLACK)) {
+    if (__any_sync(0xffffffffu, top > m + WA_SLACK)) {
       float y = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
       y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
       const float nm = fmaxf(m, y);

@@ -28,17 +28,13 @@
 // heads of 64 34 us, where a CTA takes 18000 cycles, 8000 of them before its first
 // and after its last key tile.
 //
-// The row's maximum is raised, and its output in tensor memory rescaled, only
-// when a score exceeds it by more than 2^8: then weights stay below 2^8, sums
-// far inside f32, and most tiles need no pass over the output.
-//
 // With few query tiles the key tiles are divided over the CTAs of a cluster,
 // whose parts are joined through distributed shared memory in rank order
 // (chunks of 33 to 61 tokens behind a window of 2048, 64 / 8 heads of 128: 45 ->
 // 27.6 us).
 //
 // Rounding: scores, weights and sums f32; the weights rounded once to the
-// tensors' type for P V (half a step each), the output once at the end.
+// tensors' type for P V (wa_weight_shift), the output once at the end.
 // Every wait is bounded; rows whose wait gave up are written as NaN.
 #include <cooperative_groups.h>
 #include <cuda.h>
@@ -60,7 +56,6 @@ constexpr int WT_KT = 64;                      // keys per tile
 constexpr int WT_ROWS = 128;                   // query rows per tile, two tiles per CTA
 constexpr int WT_LOAD = 8, WT_MMA = 9, WT_CLEAN = 11;  // warps 0-3, 4-7: softmax of query tile 0, 1; 9, 10: its MMAs
 constexpr int WT_THREADS = 384;
-constexpr float WT_SLACK = 8.f;
 
 template <int HD>
 struct WtLayout {
@@ -155,11 +150,13 @@ __device__ __forceinline__ uint32_t wt_pack<__nv_bfloat16>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The weights exp2(scale s - base) of N scores, as pairs of T in w[0 .. N/2 - 1]
-// (which may be the start of s); returns their f32 sum (of the unrounded values).
+// The weights exp2(scale s - base) of N scores, times the type's factor, as pairs
+// of T in w[0 .. N/2 - 1] (which may be the start of s); returns their f32 sum (of
+// the unrounded values).
 template <typename T, int N>
 __device__ __forceinline__ float wt_weights(const uint32_t* s, uint32_t* w, float sl, float base) {
-  const uint64_t sl2 = wt_pair(sl, sl), nb2 = wt_pair(-base, -base);
+  const float nb = wa_weight_shift<T>() - base;
+  const uint64_t sl2 = wt_pair(sl, sl), nb2 = wt_pair(nb, nb);
   uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
   for (int c = 0; c < N / 2; c++) {
@@ -418,7 +415,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       const bool all = __all_sync(0xffffffffu, last == WT_KT - 1 && (first <= 0 || sink >= WT_KT));
       // the maximum is raised to a larger score: the sum and the output so far follow
       auto raise = [&](float top) {
-        if (__any_sync(0xffffffffu, top > m + WT_SLACK)) {
+        if (__any_sync(0xffffffffu, top > m + WA_SLACK)) {
           const float nm = fmaxf(m, top);
           const float f = nm == -INFINITY ? 1.f : wt_exp2(m - nm);
           m = nm;

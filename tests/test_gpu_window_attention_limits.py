@@ -1,0 +1,48 @@
+"""Window attention at the limits of its types and lengths, against its
+definition in f64 (window_reference.attention64): weights far below a row's
+largest."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import window_reference as wr
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("q,hq,hkv,d", [(1, 8, 2, 64), (1, 8, 8, 128), (1, 2, 1, 100), (20, 4, 2, 256), (300, 128, 32, 64),
+                                        (300, 128, 32, 128), (70, 32, 4, 128), (200, 8, 2, 256)])
+@pytest.mark.parametrize("gap", [8.0, 12.0, 14.5, 17.0])
+def test_first_token_far_above_the_rest(built, dtype, q, hq, hkv, d, gap):
+    """The first token's score stands `gap` nats above all others and its value is 0, so the output
+    is made of weights of e^-gap alone. They count as the definition has them, to the rounding of
+    the weights: half a step of the type, and for f16, whose exponents end, 2^-25 where the row's
+    largest weight is 2^7 or more: 2^-32 of the largest."""
+    g = gen(int(gap) + d)
+    rows = 1300 + q
+    k = torch.zeros(1, hkv, rows, d, device="cuda")
+    k[..., 0] = 0.01 * torch.randn(1, hkv, rows, generator=g, device="cuda")
+    k[:, :, 0, 0] = gap
+    v = 1024 * (1 + torch.rand(1, hkv, rows, d, generator=g, device="cuda"))
+    v[:, :, 0] = 0
+    qq = torch.zeros(q, hq, d, device="cuda")
+    qq[..., 0] = 1
+    qq, k, v = qq.to(dtype), k.to(dtype), v.to(dtype)
+    out = torch.empty_like(qq)
+    wr.window_attention(qq, k, v, out, i32([rows]), 1000, 1, False, scale=1.0)
+    exact, tol = wr.attention64(qq, k, v, [q], [rows], 1000, 1, scale=1.0)
+    assert exact.abs().min().item() > 0.01  # far above the type's smallest values
+    if dtype == F16:
+        tol += 2.0 ** -32 * v.double().sum(2).amax(1)[0]
+    wr.close(out, exact, tol)
