@@ -531,17 +531,23 @@ extern "C" int armai_dev_qk_norm_rope(const armai_qk_norm_rope_args* a, void* st
     ARMAI_TRY(dev.check("positions", a->positions));
     ARMAI_TRY(dev.check("inv_freq", a->inv_freq));
   }
+  // Of a tensor without heads no pointer has been checked, and none goes
+  // further: the kernel reads gains and cache rows before it looks at the heads.
   RotParams p{};
-  p.t[0] = {a->q, a->q_out, a->q_gamma, a->token_stride, a->head_stride, a->q_out_token_stride, a->q_out_head_stride,
-            (int)a->n_q_heads};
-  p.t[1] = {a->k, a->k_out, a->k_gamma, a->token_stride, a->head_stride, a->kv_row_stride, a->kv_head_stride,
-            (int)a->n_kv_heads};
-  p.t[2] = {a->v, a->v_out, nullptr, a->token_stride, a->head_stride, a->kv_row_stride, a->kv_head_stride,
-            a->v ? (int)a->n_kv_heads : 0};
+  if (a->n_q_heads)
+    p.t[0] = {a->q, a->q_out, a->q_gamma, a->token_stride, a->head_stride, a->q_out_token_stride,
+              a->q_out_head_stride, (int)a->n_q_heads};
+  if (a->n_kv_heads) {
+    p.t[1] = {a->k, a->k_out, a->k_gamma, a->token_stride, a->head_stride, a->kv_row_stride, a->kv_head_stride,
+              (int)a->n_kv_heads};
+    if (a->v)
+      p.t[2] = {a->v, a->v_out, nullptr, a->token_stride, a->head_stride, a->kv_row_stride, a->kv_head_stride,
+                (int)a->n_kv_heads};
+    p.kv_rows = a->kv_rows;
+    p.n_rows = a->n_rows;
+  }
   p.positions = a->positions;
   p.inv_freq = a->inv_freq;
-  p.kv_rows = a->kv_rows;
-  p.n_rows = a->n_rows;
   p.dim = (int)a->head_dim;
   p.rot = (int)a->rot_dim;
   p.heads = p.t[0].heads + p.t[1].heads + p.t[2].heads;
