@@ -59,12 +59,14 @@ __device__ __forceinline__ uint64_t rot_turns(float f) {
   t -= floor(t);
   return __double2ull_rz(t * 18446744073709551616.0);
 }
-// cos and sin of the angle, times m. The remainder, below half a turn, is
-// rounded to f32: 2e-7 absolute, at any position.
-__device__ __forceinline__ float2 rot_angle(int64_t pos, uint64_t turns, float m) {
-  const int32_t r = (int32_t)(((uint64_t)pos * turns) >> 32);  // signed, in 2^-32 turns
+// cos and sin of position * f, times m. The remainder, below half a turn, is
+// rounded to f32: 2e-7 absolute, at any position. A frequency that is no finite
+// number has no fraction of a turn: NaN.
+__device__ __forceinline__ float2 rot_angle(int64_t pos, float f, float m) {
+  const int32_t r = (int32_t)(((uint64_t)pos * rot_turns(f)) >> 32);  // signed, in 2^-32 turns
   float s, c;
   sincospif((float)r * 4.656612873077392578125e-10f, &s, &c);  // half turns: 2^-31
+  m += f - f;
   return make_float2(c * m, s * m);
 }
 
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotate_vec(const RotParams p, i
     __syncwarp();
     if (half) {
       const int64_t pos = p.positions[token];
-      for (int i = lane; i < half; i += 32) cs[i] = rot_angle(pos, rot_turns(p.inv_freq[i]), p.mscale);
+      for (int i = lane; i < half; i += 32) cs[i] = rot_angle(pos, p.inv_freq[i], p.mscale);
     }
     __syncwarp();
 #pragma unroll
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotate_any(const RotParams p, i
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int half = p.rot >> 1;
   for (int i = threadIdx.x; i < half; i += ROT_THREADS)
-    cs[i] = rot_angle(p.positions[token], rot_turns(p.inv_freq[i]), p.mscale);
+    cs[i] = rot_angle(p.positions[token], p.inv_freq[i], p.mscale);
   __syncthreads();
   for (int h = blockIdx.y * (ROT_THREADS / 32) + warp; h < p.heads; h += gridDim.y * (ROT_THREADS / 32)) {
     int head;

@@ -33,3 +33,24 @@ def test_tensors_without_heads(built, dtype, layout, tokens, hq, hkv, dim, rot):
     wr.check(wr.load_cuda().armai_dev_qk_norm_rope(wr.ctypes.byref(a), wr.stream()))
     exact, size = wr.rotate64(wr.norm64(x, gam, 1e-5), pos, f, layout)
     rope_close(out if hq else out[rows], exact, size, more=NORM)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype,dim", [(F32, 64), (BF16, 128), (F16, 33)])
+@pytest.mark.parametrize("tokens", [3, 2000])
+def test_frequencies_that_are_no_numbers(built, layout, dtype, dim, tokens):
+    """A NaN or infinite frequency makes its own pair NaN at every position (0 times infinity too), as
+    the definition does, and no other value."""
+    g = gen(dim)
+    x = rnd(g, tokens, 3, dim, dtype=dtype)
+    pos, f = torch.arange(tokens, device="cuda"), freqs(32)
+    bad = f.clone()
+    bad[[1, 6, 15]] = torch.tensor([float("nan"), float("inf"), float("-inf")], device="cuda")
+    out, want = torch.empty_like(x), torch.empty_like(x)
+    wr.rope(x, out, pos, bad, layout)
+    wr.rope(x, want, pos, f, layout)
+    pairs = torch.zeros(dim, dtype=torch.bool, device="cuda")
+    for i in (1, 6, 15):
+        pairs[[2 * i, 2 * i + 1] if layout == "interleaved" else [i, i + 16]] = True
+    assert torch.isnan(out[..., pairs]).all()
+    assert torch.equal(out[..., ~pairs], want[..., ~pairs])
