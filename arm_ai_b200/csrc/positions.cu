@@ -51,17 +51,20 @@ struct RotParams {
 };
 
 // Turns per position of frequency f, as a 64-bit fraction of a turn. Times a
-// position it wraps modulo one turn by itself (negative positions too), with
-// an error of 2^-53 of the angle and 2^-64 turns per position: the f64 product
-// reduced exactly, without f64 work per position.
+// position it wraps modulo one turn by itself (negative positions too). f / 2 pi
+// is made as a sum of two f64 (1 / 2 pi as two, the first product's rounding by
+// FMA: a product alone is off by 2^-53 of itself, 1e-4 rad at position 2^40), so
+// that the fraction is off by less than two of its own steps for f below 2^10.
 __device__ __forceinline__ uint64_t rot_turns(float f) {
-  double t = (double)f * 0.15915494309189533577;
-  t -= floor(t);
-  return __double2ull_rz(t * 18446744073709551616.0);
+  const double hi = 0.15915494309189535, lo = -9.839338337591243e-18;
+  const double x = f, t = x * hi, rest = fma(x, hi, -t) + x * lo;
+  return __double2ull_rz((t - floor(t)) * 18446744073709551616.0) +
+         (uint64_t)__double2ll_rd(rest * 18446744073709551616.0);
 }
 // cos and sin of position * f, times m. The remainder, below half a turn, is
-// rounded to f32: 2e-7 absolute, at any position. A frequency that is no finite
-// number has no fraction of a turn: NaN.
+// rounded to f32: 2e-7, and 2^-60 per position of the fraction's steps (2e-7
+// more at position 2^38). A frequency that is no finite number has no fraction
+// of a turn: NaN.
 __device__ __forceinline__ float2 rot_angle(int64_t pos, float f, float m) {
   const int32_t r = (int32_t)(((uint64_t)pos * rot_turns(f)) >> 32);  // signed, in 2^-32 turns
   float s, c;

@@ -377,9 +377,9 @@ typedef struct armai_rope_args {
   int32_t layout;           /* ARMAI_ROPE_* */
 } armai_rope_args;
 /* out[t][h] = x[t][h] with pair i turned by positions[t] * inv_freq[i]. The
- * angle is the exact product, reduced to one turn before it is rounded to f32,
- * so far positions keep their accuracy (armai_rope_f32 rounds the product as
- * the reference does). */
+ * angle is the product to 2^-60 rad per position, reduced to one turn before it
+ * is rounded to f32, so far positions keep their accuracy (armai_rope_f32 rounds
+ * the product as the reference does). A NaN or infinite frequency gives NaN. */
 ARMAI_API int armai_dev_rope(const armai_rope_args* args, void* stream);
 /* Host form, f32: input [n_rows][head_dim] as armai_rope_f32, the first
  * 2 * inv_freq_len values of each row rotated. */

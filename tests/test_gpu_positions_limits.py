@@ -1,5 +1,6 @@
 """Rotary positions and head norms at the limits of their arguments, against
 their definitions in f64 (tolerances as in test_gpu_positions)."""
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -54,3 +55,29 @@ def test_frequencies_that_are_no_numbers(built, layout, dtype, dim, tokens):
         pairs[[2 * i, 2 * i + 1] if layout == "interleaved" else [i, i + 16]] = True
     assert torch.isnan(out[..., pairs]).all()
     assert torch.equal(out[..., ~pairs], want[..., ~pairs])
+
+
+@pytest.mark.parametrize("layout,dim", [("half", 128), ("interleaved", 64), ("half", 33)])
+@pytest.mark.parametrize("base,factor", [(10000.0, 1.0), (5e5, 8.0), (10000.0, 0.125)])
+def test_positions_up_to_2_40(built, layout, dim, base, factor):
+    """The product of a 40-bit position and a 24-bit frequency is exact in 64 bits, where its cosine
+    and sine are taken; the kernel's angle may be off by 2^-60 rad per position on top of a turn's
+    other roundings."""
+    assert np.finfo(np.longdouble).nmant >= 63
+    g = gen(dim)
+    pos = [0, 1, -1, 1 << 24, (1 << 31) + 12345, -(1 << 33) - 7, (1 << 36) + 1, (1 << 39) + 987654321, (1 << 40) - 1,
+           1 - (1 << 40)]
+    f = freqs(dim // 2 * 2, base=base, scaling="linear", factor=factor)
+    x = rnd(g, len(pos), 2, dim)
+    pos = torch.tensor(pos, device="cuda")
+    out = torch.empty_like(x)
+    wr.rope(x, out, pos, f, layout)
+    ang = pos.cpu().numpy().astype(np.longdouble)[:, None] * f.cpu().numpy().astype(np.longdouble)
+    c, s = (torch.from_numpy(t.astype(np.float64)).cuda()[:, None] for t in (np.cos(ang), np.sin(ang)))
+    r = dim // 2
+    a, b = ((x[..., 0:2 * r:2], x[..., 1:2 * r:2]) if layout == "interleaved" else (x[..., :r], x[..., r:2 * r]))
+    a, b = a.double(), b.double()
+    want, size = torch.stack((a * c - b * s, a * s + b * c), -1), torch.hypot(a, b)[..., None].expand(-1, -1, -1, 2)
+    got = (torch.stack((out[..., 0:2 * r:2], out[..., 1:2 * r:2]), -1) if layout == "interleaved"
+           else torch.stack((out[..., :r], out[..., r:2 * r]), -1))
+    rope_close(got, want, size, more=pos.abs().double()[:, None, None, None] * 2.0 ** -60)
