@@ -150,6 +150,7 @@ _SIGS = {
                                        c_size_t, c_void_p, c_size_t, c_void_p, c_size_t, c_size_t, c_size_t,
                                        c_size_t, c_int, c_double, c_double, c_void_p, c_void_p]),
     "armai_dev_window_attention": (c_int, [POINTER(WindowAttentionArgs), c_void_p]),
+    "armai_dev_window_attention_status": (c_int, []),
     "armai_window_attention_f32": (c_int, [c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_size_t, c_double,
                                            c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t,
                                            c_size_t, c_void_p]),

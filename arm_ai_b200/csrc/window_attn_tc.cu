@@ -35,7 +35,12 @@
 //
 // Rounding: scores, weights and sums f32; the weights rounded once to the
 // tensors' type for P V (wa_weight_shift), the output once at the end.
-// Every wait is bounded; rows whose wait gave up are written as NaN.
+// Every wait is bounded. What a softmax warp needs comes to it through the warp
+// that issues its products: the loader's or the cleaning warp's wait that gives up
+// makes a later wait of that warp give up. So an issuing warp that has given up
+// says so before it hands over anything more, and the rows of the CTA (with
+// divided keys of its cluster) are written as NaN; the device's error word tells
+// the host (armai_dev_window_attention_status).
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -201,11 +206,20 @@ struct WtWork {
 
 // Waits of a converged warp: one look, and the bounded loop only where that
 // was not enough. After a wait that gave up (ok false) no further one waits,
-// so the role runs to its end.
-__device__ __forceinline__ bool wt_wait_slow(uint64_t* bar, uint32_t parity, bool ok, uint32_t* err) {
-  return ok && qg_wait_warp(bar, parity, err);
+// so the role runs to its end. `failed` (of the CTA, in shared memory) is set by
+// the wait that gives up, before the caller commits a product or arrives
+// anywhere again.
+__device__ __forceinline__ bool wt_wait_slow(uint64_t* bar, uint32_t parity, bool ok, uint32_t* err, uint32_t* failed) {
+  if (!ok) return false;
+  ok = qg_wait_warp(bar, parity, err);
+  if (!ok && failed) {
+    *static_cast<volatile uint32_t*>(failed) = 1u;
+    __threadfence_block();
+  }
+  return ok;
 }
-__device__ __forceinline__ void wt_wait(uint64_t* bar, uint32_t parity, bool& ok, uint32_t* err) {
+__device__ __forceinline__ void wt_wait(uint64_t* bar, uint32_t parity, bool& ok, uint32_t* err,
+                                        uint32_t* failed = nullptr) {
   uint32_t done;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -214,7 +228,7 @@ __device__ __forceinline__ void wt_wait(uint64_t* bar, uint32_t parity, bool& ok
       : "=r"(done)
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
-  if (!__all_sync(0xffffffffu, done)) ok = wt_wait_slow(bar, parity, ok, err);
+  if (!__all_sync(0xffffffffu, done)) ok = wt_wait_slow(bar, parity, ok, err, failed);
 }
 
 // One lane of a converged warp.
@@ -312,6 +326,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 2);
   uint32_t* info = tslot + 1;          // [SLOTS] of a slot's K tile: its keys, and the query tiles that need it
   int* runs = reinterpret_cast<int*>(info + L::SLOTS);  // [9]
+  uint32_t* failed = reinterpret_cast<uint32_t*>(runs + 9);  // an issuing warp's wait gave up
   // over the operands, once they are done with: every rank's part of the rows
   // that this rank joins
   cg::cluster_group cluster = cg::this_cluster();
@@ -359,6 +374,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       __syncwarp();
     }
     if (tid == WT_LOAD * 32) {
+      *failed = 0u;
       // without the empty runs: a loop goes from one to the next
       int k = 0;
 #pragma unroll
@@ -502,7 +518,10 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       if (lane == 0) mbar_arrive1(&pready[2 * h + (n & 1)]);
       n++;
     }
-    if (n > 0) products();
+    if (n > 0) {
+      products();
+      ok = ok && !*static_cast<volatile uint32_t*>(failed);
+    }
     tc_fence_after();
     if (ranks == 1) {
       const bool none = n == 0 || l == 0.f;  // no key seen
@@ -594,7 +613,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     auto qk = [&](int keys, uint32_t ka) {
       const int b = nq & 1;
       // its buffer held P of the key tile two before
-      if (nq >= 2) wt_wait(&pvdone[2 * h + b], (uint32_t)((nq >> 1) - 1) & 1, ok, p.err);
+      if (nq >= 2) wt_wait(&pvdone[2 * h + b], (uint32_t)((nq >> 1) - 1) & 1, ok, p.err, failed);
       tc_fence_after();
       const uint32_t idesc = BASE | ((uint32_t)((keys + 15) >> 4) << 18);  // N: the tile's keys, in steps of 16
       if (wt_elect()) {
@@ -609,7 +628,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     };
     // of the key tiles now, next and next but one: keys | whether this query tile needs them << 8
     uint32_t now = 0, next = 0;
-    wt_wait(qfull, 0, ok, p.err);
+    wt_wait(qfull, 0, ok, p.err, failed);
     {
       WtIter it(runs);
       if (w.nt > 0) now = (uint32_t)it.x.n | (uint32_t)w.needs(p, h, it.x) << 8;
@@ -622,11 +641,11 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     uint32_t word = 0;
     // the slot's tiles have landed, rows behind a short V tile are zeroed
     auto arrived = [&](int keys) {
-      wt_wait(&full[slot.s], slot.turn & 1, ok, p.err);
+      wt_wait(&full[slot.s], slot.turn & 1, ok, p.err, failed);
       word = info[slot.s];
       if (keys & 15) {
         if (lane == 0) mbar_arrive1(&vgo[cleaned]);
-        wt_wait(&vclean[cleaned++], 0, ok, p.err);
+        wt_wait(&vclean[cleaned++], 0, ok, p.err, failed);
       }
     };
     if (w.nt > 0) arrived((int)(now & 255u));
@@ -641,7 +660,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       if (now >> 8) {
         const int b = np & 1;
         const uint32_t va = base + ((8192u - 16u) >> 4 << 16);  // 64-wide blocks of the row 8 KB apart
-        wt_wait(&pready[2 * h + b], (uint32_t)(np >> 1) & 1, ok, p.err);
+        wt_wait(&pready[2 * h + b], (uint32_t)(np >> 1) & 1, ok, p.err, failed);
         tc_fence_after();
         if (wt_elect()) {
 #pragma unroll
@@ -665,7 +684,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     if (wt_elect()) qg_commit(&fin[h]);
     __syncwarp();
     ok = true;
-    wt_wait(&fin[h], 0, ok, p.err);
+    wt_wait(&fin[h], 0, ok, p.err, failed);
   } else {
     // the last product of 16 keys of a short tile also reads rows behind the
     // tile's: zero them (their weights are zero, but the rows may hold anything)
@@ -767,6 +786,8 @@ bool wt_map(CUtensorMap* map, int dtype, int rank, const void* base, const cuuin
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Error word of this kernel's bounded waits (one per device that loads the
+// library); read and cleared by armai_dev_window_attention_status.
 __device__ uint32_t g_wt_err;
 // CTAs in clusters that the device holds at once, one per SM (a few SMs are
 // left over where a cluster does not fit: 132 of 148 with clusters of 4, 120
@@ -827,3 +848,14 @@ int wa_tc_launch(const WaParams& p, int dtype, cudaStream_t s, bool* fits) {
 }
 
 }  // namespace armai
+
+extern "C" int armai_dev_window_attention_status(void) {
+  using namespace armai;
+  uint32_t e = 0;
+  ARMAI_CUDA(cudaMemcpyFromSymbol(&e, g_wt_err, sizeof e));
+  if (!e) return ARMAI_OK;
+  const uint32_t zero = 0;
+  ARMAI_CUDA(cudaMemcpyToSymbol(g_wt_err, &zero, sizeof zero));
+  return fail(ARMAI_E_DEVICE, "window_attn: a wait of the tensor-core kernel gave up (error word " + std::to_string(e) +
+                                  "); its rows are NaN");
+}

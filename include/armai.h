@@ -448,6 +448,11 @@ typedef struct armai_window_attention_args {
  * keys) of a row that only some queries of a call see must be finite. Rows of
  * out behind the last sequence are left as they are. */
 ARMAI_API int armai_dev_window_attention(const armai_window_attention_args* args, void* stream);
+/* Every wait inside a kernel is bounded. ARMAI_E_DEVICE where one has given up on
+ * the current device since the last such question (the rows that it concerned
+ * were written as NaN), else ARMAI_OK. Asked when the work of the calls is done,
+ * and not while a stream is captured. */
+ARMAI_API int armai_dev_window_attention_status(void);
 /* Host form, f32: q [B,Hq,Sq,D], k / v [B,Hkv,Sk,D] as armai_flash_attention_f32
  * (but with query i at position Sk - Sq + i) -> out [B,Hq,Sq,D]. */
 ARMAI_API int armai_window_attention_f32(const float* q, size_t q_len, const float* k, size_t k_len,

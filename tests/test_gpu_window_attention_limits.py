@@ -6,6 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import window_reference as wr
+from arm_ai_b200._lib import check, load_cuda
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +47,18 @@ def test_first_token_far_above_the_rest(built, dtype, q, hq, hkv, d, gap):
     if dtype == F16:
         tol += 2.0 ** -32 * v.double().sum(2).amax(1)[0]
     wr.close(out, exact, tol)
+
+
+def test_status_after_calls(built):
+    """No wait has given up in calls of every form: the question is answered, and answered again."""
+    lib = load_cuda()
+    check(lib.armai_dev_window_attention_status())
+    for dtype, q, hq, hkv, d in ((BF16, 400, 64, 16, 128), (F16, 40, 64, 8, 64), (BF16, 1, 8, 2, 128), (F32, 300, 64, 16, 64)):
+        g = gen(q)
+        qq = torch.randn(q, hq, d, generator=g, device="cuda").to(dtype)
+        k, v = (torch.randn(1, hkv, q + 2000, d, generator=g, device="cuda").to(dtype) for _ in range(2))
+        out = torch.empty_like(qq)
+        wr.window_attention(qq, k, v, out, i32([q + 2000]), 1500, 4, False)
+        torch.cuda.synchronize()
+        check(lib.armai_dev_window_attention_status())
+        assert torch.isfinite(out.float()).all()
