@@ -433,7 +433,8 @@ typedef struct armai_window_attention_args {
   int64_t n_slots, kv_rows;
   int64_t window;           /* >= 1 */
   int64_t n_sink;           /* >= 0: first positions that stay visible */
-  int32_t ring;             /* 0: position p is cache row p. 1: rows n_sink .. kv_rows - 1 are a ring of
+  int32_t ring;             /* 0: position p is cache row p; positions from kv_rows on have no row and are seen by
+                               no query (kv_len may pass kv_rows: queries there see what is held). 1: rows n_sink .. kv_rows - 1 are a ring of
                                R = kv_rows - n_sink rows, R >= window + max_q - 1: position p >= n_sink is row
                                n_sink + (p - n_sink) % R */
   float scale;              /* of the scores */

@@ -62,3 +62,28 @@ def test_status_after_calls(built):
         torch.cuda.synchronize()
         check(lib.armai_dev_window_attention_status())
         assert torch.isfinite(out.float()).all()
+
+
+@pytest.mark.parametrize("dtype,q,hq,hkv,d", [(BF16, 1, 8, 2, 128), (F32, 1, 4, 2, 64), (F16, 1, 4, 2, 100),
+                                              (F16, 300, 64, 16, 64), (BF16, 300, 64, 16, 128), (F32, 300, 64, 16, 80),
+                                              (BF16, 90, 8, 2, 256), (F32, 20, 4, 2, 64), (F16, 50, 2, 1, 33)])
+@pytest.mark.parametrize("rows,past,window,n_sink", [(400, 90, 100, 2), (400, 390, 64, 0), (310, 900, 200, 3),
+                                                     (64, 1500, 70, 0)])
+def test_positions_behind_a_linear_cache(built, dtype, q, hq, hkv, d, rows, past, window, n_sink):
+    """A linear cache has no row for positions from kv_rows on: they are seen by nobody, the queries
+    there see what the cache holds, and nothing is read beyond it."""
+    g = gen(rows + d)
+    length = past + q
+    qq = torch.randn(q, hq, d, generator=g, device="cuda").to(dtype)
+    # the cache between rows that nobody may look at
+    whole = torch.full((2, 1, hkv, rows + 128, d), float("nan"), dtype=dtype, device="cuda")
+    whole[..., 64:64 + rows, :] = torch.randn(2, 1, hkv, rows, d, generator=g, device="cuda").to(dtype)
+    k, v = whole[:, :, :, 64:64 + rows]
+    out = torch.empty_like(qq)
+    wr.window_attention(qq, k, v, out, i32([length]), window, n_sink, False)
+    j = torch.arange(rows, device="cuda")
+    for i in range(0, q, max(1, q // 9)):
+        p = past + i
+        keep = (j <= p) & ((j > p - window) | (j < n_sink))
+        wr.close(out[i:i + 1], *wr.attention64(qq[i:i + 1], k[:, :, keep].contiguous(), v[:, :, keep].contiguous(), [1],
+                                              [int(keep.sum())], 1 << 40))
