@@ -443,7 +443,12 @@ typedef struct armai_window_attention_args {
 /* The i-th of a sequence's n queries is at position p = kv_len - n + i and
  * sees the keys j <= p with j > p - window or j < n_sink; out = softmax(scale
  * q k^T) v over them (query head h with key / value head h / (n_q_heads /
- * n_kv_heads)), scores, softmax and sums in f32. A query that sees no key
+ * n_kv_heads)), scores, softmax and sums in f32. The softmax's weights of
+ * f16 and bf16 tensors are rounded once to their type for the product with v, as
+ * the tensor cores take them: half a step of each weight (f16: down to 2^-21 of a
+ * row's largest weight, and 2^-32 of the largest below), which makes the error of
+ * an output up to 1.45 times that of its own rounding alone. Weights of f32
+ * tensors are not rounded. A query that sees no key
  * (p < 0, kv_len <= 0, a slot outside 0 .. n_slots - 1) gets zeros. Cache rows
  * that no query of the sequence sees may hold anything; the values (not the
  * keys) of a row that only some queries of a call see must be finite. Rows of
