@@ -687,7 +687,9 @@ __global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const W
 
 // Clusters of 2^log2 CTAs that the device holds at once (with one CTA per SM
 // 33 of 4, 15 of 8 and 7 of 16: what is left of a die's groups of SMs stays
-// empty), asked for once per kernel, size and device. 0: it has no such.
+// empty), asked for once per kernel, size and device. 0: it has no such. A
+// question that fails is none for this call alone (no division over such
+// clusters) and is asked again at the next.
 template <auto K>
 int sp_active(int log2, const cudaLaunchConfig_t& cfg) {
   constexpr int DEVICES = 32;
@@ -697,8 +699,8 @@ int sp_active(int log2, const cudaLaunchConfig_t& cfg) {
   const int k = dev < DEVICES ? known[dev][log2].load(std::memory_order_relaxed) : 0;
   if (k) return k - 1;
   if (cudaOccupancyMaxActiveClusters(&active, K, &cfg) != cudaSuccess) {
-    cudaGetLastError();  // clusters of this size cannot be: the answer, not a failure of the call
-    active = 0;
+    cudaGetLastError();  // not a failure of the call
+    return 0;
   }
   if (dev < DEVICES) known[dev][log2].store(active + 1, std::memory_order_relaxed);
   return active;
