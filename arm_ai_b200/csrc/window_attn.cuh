@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "dev_call.cuh"
@@ -147,6 +148,27 @@ __device__ __forceinline__ WaTile wa_tile(const WaRuns& r, int t) {
 template <int KT>
 __device__ __forceinline__ int wa_tiles(const WaRuns& r) {
   return (r.len[0] + KT - 1) / KT + (r.len[1] + KT - 1) / KT + (r.len[2] + KT - 1) / KT;
+}
+
+// Clusters of 2^log2 CTAs of a kernel that the device holds at once (with one CTA
+// per SM 33 of 4, 15 of 8 and 7 of 16: what is left of a die's groups of SMs stays
+// empty), asked for once per kernel, size and device. 0: it has no such. A
+// question that fails is none for this call alone (no division over such
+// clusters) and is asked again at the next.
+template <auto K>
+int wa_clusters(int log2, const cudaLaunchConfig_t& cfg) {
+  constexpr int DEVICES = 32;
+  static std::atomic<int> known[DEVICES][5];  // and one more: 0 is not known
+  int dev = 0, active = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  const int k = dev < DEVICES ? known[dev][log2].load(std::memory_order_relaxed) : 0;
+  if (k) return k - 1;
+  if (cudaOccupancyMaxActiveClusters(&active, K, &cfg) != cudaSuccess) {
+    cudaGetLastError();  // not a failure of the call
+    return 0;
+  }
+  if (dev < DEVICES) known[dev][log2].store(active + 1, std::memory_order_relaxed);
+  return active;
 }
 
 // Every pointer, stride and the head a whole number of so many bytes.

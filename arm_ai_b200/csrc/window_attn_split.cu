@@ -22,7 +22,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "llama_kernels.cuh"
 #include "window_attn.cuh"
@@ -685,27 +684,6 @@ __global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const W
   sp_join<float, R, DT, CB>(p, split, b, part, wm, wl, reinterpret_cast<SpMail<R, DT>*>(sm + sf_smem<CH>(R)));
 }
 
-// Clusters of 2^log2 CTAs that the device holds at once (with one CTA per SM
-// 33 of 4, 15 of 8 and 7 of 16: what is left of a die's groups of SMs stays
-// empty), asked for once per kernel, size and device. 0: it has no such. A
-// question that fails is none for this call alone (no division over such
-// clusters) and is asked again at the next.
-template <auto K>
-int sp_active(int log2, const cudaLaunchConfig_t& cfg) {
-  constexpr int DEVICES = 32;
-  static std::atomic<int> known[DEVICES][5];  // and one more: 0 is not known
-  int dev = 0, active = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  const int k = dev < DEVICES ? known[dev][log2].load(std::memory_order_relaxed) : 0;
-  if (k) return k - 1;
-  if (cudaOccupancyMaxActiveClusters(&active, K, &cfg) != cudaSuccess) {
-    cudaGetLastError();  // not a failure of the call
-    return 0;
-  }
-  if (dev < DEVICES) known[dev][log2].store(active + 1, std::memory_order_relaxed);
-  return active;
-}
-
 // A sequence and head's keys are split over as many CTAs as run at once, but
 // no warp goes without a tile. A cluster left over would take as long again as
 // the others (one stream, 4096 keys, width 256: 8 heads over 16 CTAs each 23.7
@@ -737,7 +715,7 @@ int sp_launch(size_t smem, const WaParams& p, int rows, int kt, int warps, cudaS
     if ((int64_t)n * warps * kt > keys || clusters * n > 4 * (int64_t)sm_count()) break;
     if (n > 8) ARMAI_CUDA(cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr[0].val.clusterDim.x = (unsigned)n;
-    const int active = sp_active<K>(log2, cfg);
+    const int active = wa_clusters<K>(log2, cfg);
     const bool several = active * n > sm_count();
     if (several ? clusters * 15 > (int64_t)active * 16 : clusters > active) break;
     split = log2;

@@ -789,10 +789,6 @@ bool wt_map(CUtensorMap* map, int dtype, int rank, const void* base, const cuuin
 // Error word of this kernel's bounded waits (one per device that loads the
 // library); read and cleared by armai_dev_window_attention_status.
 __device__ uint32_t g_wt_err;
-// CTAs in clusters that the device holds at once, one per SM (a few SMs are
-// left over where a cluster does not fit: 132 of 148 with clusters of 4, 120
-// with 8).
-constexpr int64_t WT_FILL = 120;
 
 template <typename T, int HD>
 int wt_launch(const WaParams& in, int dtype, cudaStream_t s, bool* fits) {
@@ -815,23 +811,31 @@ int wt_launch(const WaParams& in, int dtype, cudaStream_t s, bool* fits) {
   ARMAI_CUDA(cudaFuncSetAttribute(k_wa_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WtLayout<HD>::SMEM));
   const int tokens = 2 * WT_ROWS / pack;
   const int64_t blocks = (p.max_q + tokens - 1) / tokens, ctas = blocks * (p.n_q_heads / pack) * p.n_seq;
-  // Fewer CTAs than half the SMs: the keys divided over clusters, four key
-  // tiles at least for each CTA.
+  // The keys divided over clusters, as long as these run all at once and four
+  // key tiles at least are left for each CTA (4100 visible keys, heads of 128: 64
+  // or 72 CTAs by two 41 against 66 us; 32 by four 26.8 against 39.6 by two; 80,
+  // which do not fit twice, 66.7).
   const int64_t keys = std::min<int64_t>(p.kv_rows, (int64_t)p.window + p.n_sink + tokens);
-  int lranks = 0;
-  while (lranks < 3 && (ctas << lranks) * 2 <= WT_FILL && keys >= (int64_t)8 * WT_KT << lranks) lranks++;
-  const int ranks = 1 << lranks;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(blocks * ranks), (unsigned)(p.n_q_heads / pack), (unsigned)p.n_seq);
+  cfg.gridDim = dim3((unsigned)blocks, (unsigned)(p.n_q_heads / pack), (unsigned)p.n_seq);
   cfg.blockDim = dim3(WT_THREADS);
   cfg.dynamicSmemBytes = WtLayout<HD>::SMEM;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ranks;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int lranks = 0;
+  for (int log2 = 1; log2 <= 3 && keys >= (int64_t)4 * WT_KT << log2 && ctas << log2 <= sm_count(); log2++) {
+    cfg.gridDim.x = (unsigned)(blocks << log2);
+    attr[0].val.clusterDim.x = 1u << log2;
+    if (ctas > wa_clusters<k_wa_tc<T, HD>>(log2, cfg)) break;
+    lranks = log2;
+  }
+  const int ranks = 1 << lranks;
+  cfg.gridDim.x = (unsigned)(blocks * ranks);
+  attr[0].val.clusterDim.x = (unsigned)ranks;
   cfg.numAttrs = ranks > 1 ? 1 : 0;
   ARMAI_CUDA(cudaLaunchKernelEx(&cfg, k_wa_tc<T, HD>, mq, mk, mv, p, lpack, lranks));
   return ARMAI_OK;
