@@ -196,6 +196,7 @@ __global__ void __launch_bounds__(4 * Q, DM > 96 ? 1 : Q == 64 ? 2 : 3) k_wa_sim
     }
     x = y;
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");  // of the queries, where there was no key tile
 #pragma unroll
   for (int i = 0; i < 4; i++) {
 #pragma unroll
