@@ -223,11 +223,16 @@ int ws_launch(const WaParams& p, int vec, cudaStream_t s) {
   ARMAI_CUDA(cudaGetLastError());
   return ARMAI_OK;
 }
-// 32 queries per CTA where 64 would leave the SMs unevenly filled.
+// 32 queries per CTA where 64 would leave the SMs unevenly filled: up to four CTAs
+// of 64 per SM (f32, 2 x 8 heads of 80, no window: 256 CTAs of 64 187 us, their
+// halves 146; 640: 738 against 688; 1184: 2020 against 2023; 1808: 3492 against
+// 3597; 32 / 8 heads of 64, window 300, 896: 178 against 184). Beyond a width of
+// 128 an SM has room for one CTA of either kind: up to two (8 heads of 256: 256
+// CTAs 535 against 520, 448: 803 against 974, 888: 1602 against 2011).
 template <typename T, int DM>
 int ws_rows_per_cta(const WaParams& p, int vec, cudaStream_t s) {
   const int64_t ctas = (int64_t)p.n_seq * p.n_q_heads * ((p.max_q + 63) / 64);
-  return ctas > 4 * (int64_t)sm_count() ? ws_launch<T, DM, 64>(p, vec, s) : ws_launch<T, DM, 32>(p, vec, s);
+  return ctas > (DM > 128 ? 2 : 4) * (int64_t)sm_count() ? ws_launch<T, DM, 64>(p, vec, s) : ws_launch<T, DM, 32>(p, vec, s);
 }
 template <typename T>
 int ws_dim(const WaParams& p, int vec, cudaStream_t s) {
