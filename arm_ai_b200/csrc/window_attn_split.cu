@@ -690,6 +690,10 @@ __global__ void __launch_bounds__(32 * sp_warps(32 * CH)) k_wa_split_f32(const W
 // us, over 8 each 18.1; 7 heads over 16 each 12.6), unless it is one in fifteen
 // and SMs hold several CTAs (48 heads and streams of 4096 keys, width 128: over
 // 8 CTAs each 18.3 us, 45 clusters at once; over 4 each 23.9).
+// Narrow heads leave room for more, but four CTAs per SM are enough (single heads
+// of 64, bf16, 4096 keys: 75 streams over 4 CTAs each 18.1 us, over 8 20.2; 300
+// over 1 58.3, over 2 66.8; f32 of 32: 148 over 4 29.6, over 8 35.2, but 75 over 4
+// 21.0, over 8 15.4).
 // 32 streams of 4100 visible keys, 8 heads of 128, bf16: 82.4 us = 6.53 TB/s.
 template <auto K>
 int sp_launch(size_t smem, const WaParams& p, int rows, int kt, int warps, cudaStream_t s) {
