@@ -36,9 +36,13 @@ class DeviceScope {
   ~DeviceScope() {
     if (prev_ >= 0) cudaSetDevice(prev_);
   }
-  // Refuses a pointer that the device cannot read; the first device pointer
-  // decides the device, the others have to be on the same one.
-  int check(const char* what, const void* p) {
+  // Refuses a pointer that is no multiple of its values' size or that the device
+  // cannot read; the first device pointer decides the device, the others have to
+  // be on the same one.
+  int check(const char* what, const void* p, int value_size) {
+    if (reinterpret_cast<uintptr_t>(p) % value_size)
+      return fail(ARMAI_E_INVALID, std::string(op_) + ": " + what + " is not aligned to its values of " +
+                                       std::to_string(value_size) + " bytes");
     cudaPointerAttributes a;
     ARMAI_CUDA(cudaPointerGetAttributes(&a, p));
     if (a.type == cudaMemoryTypeUnregistered)

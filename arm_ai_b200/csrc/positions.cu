@@ -485,11 +485,12 @@ extern "C" int armai_dev_rope(const armai_rope_args* a, void* stream) {
   if (a->x == a->out && (a->x_token_stride != a->out_token_stride || a->x_head_stride != a->out_head_stride))
     return fail(ARMAI_E_INVALID, "rope: in place, x and out must have the same strides");
   DeviceScope dev("rope");
-  ARMAI_TRY(dev.check("x", a->x));
-  ARMAI_TRY(dev.check("out", a->out));
+  const int es = dtype_size(a->dtype);
+  ARMAI_TRY(dev.check("x", a->x, es));
+  ARMAI_TRY(dev.check("out", a->out, es));
   if (a->rot_dim) {
-    ARMAI_TRY(dev.check("positions", a->positions));
-    ARMAI_TRY(dev.check("inv_freq", a->inv_freq));
+    ARMAI_TRY(dev.check("positions", a->positions, 8));
+    ARMAI_TRY(dev.check("inv_freq", a->inv_freq, 4));
   }
   RotParams p{};
   p.t[0] = {a->x, a->out, nullptr, a->x_token_stride, a->x_head_stride, a->out_token_stride, a->out_head_stride,
@@ -523,24 +524,25 @@ extern "C" int armai_dev_qk_norm_rope(const armai_qk_norm_rope_args* a, void* st
                                  "and no kv_rows");
   if (a->n_rows < 0) return fail(ARMAI_E_INVALID, "qk_norm_rope: n_rows is negative");
   DeviceScope dev("qk_norm_rope");
+  const int es = dtype_size(a->dtype), kv = dtype_size(a->kv_dtype);
   if (a->n_q_heads) {
-    ARMAI_TRY(dev.check("q", a->q));
-    ARMAI_TRY(dev.check("q_out", a->q_out));
-    if (a->q_gamma) ARMAI_TRY(dev.check("q_gamma", a->q_gamma));
+    ARMAI_TRY(dev.check("q", a->q, es));
+    ARMAI_TRY(dev.check("q_out", a->q_out, es));
+    if (a->q_gamma) ARMAI_TRY(dev.check("q_gamma", a->q_gamma, 4));
   }
   if (a->n_kv_heads) {
-    ARMAI_TRY(dev.check("k", a->k));
-    ARMAI_TRY(dev.check("k_out", a->k_out));
-    if (a->k_gamma) ARMAI_TRY(dev.check("k_gamma", a->k_gamma));
-    if (a->kv_rows) ARMAI_TRY(dev.check("kv_rows", a->kv_rows));
+    ARMAI_TRY(dev.check("k", a->k, es));
+    ARMAI_TRY(dev.check("k_out", a->k_out, kv));
+    if (a->k_gamma) ARMAI_TRY(dev.check("k_gamma", a->k_gamma, 4));
+    if (a->kv_rows) ARMAI_TRY(dev.check("kv_rows", a->kv_rows, 8));
     if (a->v) {
-      ARMAI_TRY(dev.check("v", a->v));
-      ARMAI_TRY(dev.check("v_out", a->v_out));
+      ARMAI_TRY(dev.check("v", a->v, es));
+      ARMAI_TRY(dev.check("v_out", a->v_out, kv));
     }
   }
   if (a->rot_dim) {
-    ARMAI_TRY(dev.check("positions", a->positions));
-    ARMAI_TRY(dev.check("inv_freq", a->inv_freq));
+    ARMAI_TRY(dev.check("positions", a->positions, 8));
+    ARMAI_TRY(dev.check("inv_freq", a->inv_freq, 4));
   }
   // Of a tensor without heads no pointer has been checked, and none goes
   // further: the kernel reads gains and cache rows before it looks at the heads.

@@ -315,13 +315,14 @@ extern "C" int armai_dev_window_attention(const armai_window_attention_args* a, 
     return bad("a ring needs kv_rows - n_sink >= window + max_q - 1 = " + std::to_string(window + a->max_q - 1) +
                ", got " + std::to_string(a->kv_rows - sink));
   DeviceScope dev("window_attn");
-  ARMAI_TRY(dev.check("q", a->q));
-  ARMAI_TRY(dev.check("k", a->k));
-  ARMAI_TRY(dev.check("v", a->v));
-  ARMAI_TRY(dev.check("out", a->out));
-  ARMAI_TRY(dev.check("kv_len", a->kv_len));
-  if (a->q_start) ARMAI_TRY(dev.check("q_start", a->q_start));
-  if (a->slots) ARMAI_TRY(dev.check("slots", a->slots));
+  const int es = dtype_size(a->dtype);
+  ARMAI_TRY(dev.check("q", a->q, es));
+  ARMAI_TRY(dev.check("k", a->k, es));
+  ARMAI_TRY(dev.check("v", a->v, es));
+  ARMAI_TRY(dev.check("out", a->out, es));
+  ARMAI_TRY(dev.check("kv_len", a->kv_len, 4));
+  if (a->q_start) ARMAI_TRY(dev.check("q_start", a->q_start, 4));
+  if (a->slots) ARMAI_TRY(dev.check("slots", a->slots, 4));
   WaParams p{};
   p.q = a->q;
   p.k = a->k;

@@ -342,7 +342,8 @@ ARMAI_API int armai_dev_dequant_matmul_f16_f32(const float* act, const uint16_t*
 /* `stream`, neither synchronise nor allocate, and may be captured into a    */
 /* CUDA graph. A block may be reused from call to call. They run on the      */
 /* device their tensors are on, whichever is current, and refuse host        */
-/* memory that the device cannot read.                                       */
+/* memory that the device cannot read and addresses that are no multiple of  */
+/* their values' size.                                                       */
 /* ------------------------------------------------------------------ */
 #define ARMAI_F32 0
 #define ARMAI_F16 1
