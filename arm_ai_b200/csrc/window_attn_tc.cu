@@ -350,8 +350,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   w.kvh = w.vh * pack / p.group;
 #pragma unroll
   for (int h = 0; h < 2; h++) {
-    w.qlo[h] = w.sq.pos0 + w.i0 + h * tokens;
-    w.qhi[h] = w.sq.pos0 + min(w.sq.n, w.i0 + (h + 1) * tokens) - 1;
+    const int t0 = w.i0 + h * tokens;  // behind the last token there may be no position in 32 bits
+    w.qlo[h] = t0 < w.sq.n ? w.sq.pos0 + t0 : INT32_MAX;
+    w.qhi[h] = t0 < w.sq.n ? w.sq.pos0 + min(w.sq.n, t0 + tokens) - 1 : INT32_MIN;
   }
   {
     WaRuns r = wa_runs(p, w.qlo[0], max(w.qhi[0], w.qhi[1]));
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
     const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t to = tmem + lane_base + 256u + 128u * (uint32_t)h;
     const int tok = w.i0 + h * tokens + (row >> lpack), head = w.vh * pack + (row & (pack - 1));
-    const int qpos = w.sq.pos0 + tok;
+    const int qpos = w.sq.pos0 + min(tok, w.sq.n - 1);  // rows behind the last token: as that, not written
     const float sl = p.scale_log2;
     float m = -INFINITY, l = 0.f;
     int n = 0;

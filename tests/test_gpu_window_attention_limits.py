@@ -87,3 +87,29 @@ def test_positions_behind_a_linear_cache(built, dtype, q, hq, hkv, d, rows, past
         keep = (j <= p) & ((j > p - window) | (j < n_sink))
         wr.close(out[i:i + 1], *wr.attention64(qq[i:i + 1], k[:, :, keep].contiguous(), v[:, :, keep].contiguous(), [1],
                                               [int(keep.sum())], 1 << 40))
+
+
+@pytest.mark.parametrize("dtype,q,hq,hkv,d", [(BF16, 1, 8, 2, 128), (F32, 1, 4, 2, 64), (F16, 1, 4, 2, 100),
+                                              (F16, 300, 64, 16, 64), (BF16, 300, 64, 16, 128), (BF16, 40, 64, 8, 128),
+                                              (F32, 300, 64, 16, 80), (BF16, 90, 8, 2, 256), (F16, 50, 2, 1, 33)])
+@pytest.mark.parametrize("ring", [True, False])
+def test_positions_up_to_2_31(built, dtype, q, hq, hkv, d, ring):
+    """Sequences as long as kv_len can say: in a ring the same rows, so bit for bit the same output,
+    as a whole number of turns before; in a linear cache, far behind its rows, the first tokens."""
+    g = gen(d)
+    window, n_sink = 700, 3
+    turn = window + q + 40
+    rows = n_sink + turn
+    qq = torch.randn(2 * q, hq, d, generator=g, device="cuda").to(dtype)
+    k, v = (torch.randn(2, hkv, rows, d, generator=g, device="cuda").to(dtype) for _ in range(2))
+    longest = (1 << 31) - 1
+    near = [longest - (longest // turn - 5) * turn, longest - 7 - (longest // turn - 5) * turn]
+    outs = []
+    for lens in ([longest, longest - 7], near):
+        out = torch.full_like(qq, 9.0)
+        wr.window_attention(qq, k, v, out, i32(lens), window, n_sink, ring)
+        outs.append(out)
+    assert torch.equal(*outs) and torch.isfinite(outs[0].float()).all()
+    if not ring:
+        wr.close(outs[0][:1], *wr.attention64(qq[:1], k[:1, :, :n_sink].contiguous(), v[:1, :, :n_sink].contiguous(), [1],
+                                             [n_sink], 100))
