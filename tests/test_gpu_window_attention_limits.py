@@ -113,3 +113,19 @@ def test_positions_up_to_2_31(built, dtype, q, hq, hkv, d, ring):
     if not ring:
         wr.close(outs[0][:1], *wr.attention64(qq[:1], k[:1, :, :n_sink].contiguous(), v[:1, :, :n_sink].contiguous(), [1],
                                              [n_sink], 100))
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("ctas", [14, 15, 16, 30, 33, 34, 37, 63, 72, 74, 75])
+def test_clusters_that_fit_at_once(built, dtype, d, ctas):
+    """CTA counts (of four tokens of 64 heads) around those up to which clusters of 8, 4 and 2 run
+    all at once; the last CTA has fewer tokens."""
+    g = gen(ctas)
+    q, past, window, n_sink = 4 * ctas - 1, 1800, 2040, 3
+    rows = n_sink + window + q - 1
+    qq = torch.randn(q, 64, d, generator=g, device="cuda").to(dtype)
+    k, v = (torch.randn(1, 1, rows, d, generator=g, device="cuda").to(dtype) for _ in range(2))
+    out = torch.empty_like(qq)
+    for length, ring in ((past + q, False), (5000, True)):
+        wr.window_attention(qq, k, v, out, i32([length]), window, n_sink, ring)
+        wr.close(out, *wr.attention64(qq, k, v, [q], [length], window, n_sink, ring))
